@@ -1,0 +1,366 @@
+"""Timed passes through the 8-bit activation operators and their plain torch forms.
+
+Three operators:
+
+  conv8     one layer of the 8-bit Predictor: the pixels of an fp32 channel view become 8-bit codes with one scale per
+            pixel, then a conv / transposed conv (a matrix product per tap; one tap is the plain product of tokens
+            and weights) on integer codes with a scale per output channel, + bias + ReLU, into a channel view
+  tape_fwd  training BatchNorm + ReLU that keeps its pre-activation as an 8-bit tape (64-channel blocks of a pixel,
+            one scale each), and the tape read back as values
+  tape_bwd  the backward of that BatchNorm + ReLU from the tape
+
+`own` False: elementary torch operations; True: the calls a user makes of the package.
+"""
+import torch
+
+own = False
+
+BLOCK = 64          # channels of a pixel that share a tape scale
+EPS = 1e-3
+
+# Layers of the depth networks at the sizes of the training and prediction configurations (192x256 batch 8 / 32, twin
+# batches of two images, 224x224, 240x720 with 11 input channels), and a plain product of tokens.
+_LISTED = [
+    # cnv6b of a single 224x224 prediction: sixteen pixels, all time is weights and launches
+    dict(name="conv8_224_b1_cnv6b", kind="conv8", N=1, H=4, W=4, C=512, K=512, k=3, s=1, deconv=False, relu=True),
+    # cnv1 of the 240x720 flow-stack prediction: 11 channels in a 12-channel buffer, stride 2, odd output widths of taps
+    dict(name="conv8_240x720_cnv1", kind="conv8", N=1, H=240, W=720, C=11, K=32, k=7, s=2, deconv=False, relu=True),
+    # icnv4 at batch 8: the middle of the decoder, a 256-channel concat buffer
+    dict(name="conv8_b8_icnv4", kind="conv8", N=8, H=24, W=32, C=256, K=128, k=3, s=1, deconv=False, relu=True),
+    # upcnv3 at batch 8: stride-2 transposed conv
+    dict(name="conv8_b8_upcnv3", kind="conv8", N=8, H=24, W=32, C=128, K=64, k=3, s=2, deconv=True, relu=True),
+    # cnv1b at batch 32: few channels, 49 taps
+    dict(name="conv8_b32_cnv1b", kind="conv8", N=32, H=96, W=128, C=32, K=32, k=7, s=1, deconv=False, relu=True),
+    # one tap: a plain product of tokens and weights, no ReLU
+    dict(name="conv8_tokens", kind="conv8", N=1, H=1, W=8192, C=2048, K=2048, k=1, s=1, deconv=False, relu=False),
+    # cnv6b at batch 8: 96 rows, launch-bound
+    dict(name="tape_fwd_b8_cnv6b", kind="tape_fwd", M=96, C=512, groups=1, cs=1024, co=512),
+    # cnv2b of a twin batch (two images of 8): two BatchNorm groups, written into the skip slot of a concat buffer
+    dict(name="tape_fwd_twin_cnv2b", kind="tape_fwd", M=49152, C=64, groups=2, cs=132, co=64),
+    # icnv1 at batch 32, the widest map: 16 channels at full resolution
+    dict(name="tape_fwd_b32_icnv1", kind="tape_fwd", M=1572864, C=16, groups=1, cs=16, co=0),
+    # cnv6b of a twin batch
+    dict(name="tape_bwd_twin_cnv6b", kind="tape_bwd", M=192, C=512, groups=2, cs=1024, co=512),
+    # a 7x11 map of 36 channels: ragged blocks, odd rows
+    dict(name="tape_bwd_odd", kind="tape_bwd", M=26565, C=36, groups=1, cs=36, co=0),
+    # cnv1b at batch 32, its gradient read from the skip slot of a concat buffer
+    dict(name="tape_bwd_b32_cnv1b", kind="tape_bwd", M=393216, C=32, groups=1, cs=68, co=32),
+]
+
+
+def listed():
+    return [dict(c) for c in _LISTED]
+
+
+def _log(rng, lo, hi):
+    return int(round(lo * (hi / lo) ** rng.random()))
+
+
+def draw(rng):
+    kind = rng.choice(["conv8", "tape_fwd", "tape_bwd"])
+    if kind == "conv8":
+        while True:
+            form = rng.choice(["conv", "conv", "deconv", "tokens"])
+            c = dict(kind=kind, N=_log(rng, 1, 32), H=_log(rng, 1, 480), W=_log(rng, 1, 640), C=_log(rng, 3, 1024),
+                     K=_log(rng, 2, 512), k=rng.choice([3, 3, 5, 7]), s=rng.choice([1, 1, 2]), deconv=False,
+                     relu=rng.random() < 0.8)
+            if form == "deconv":
+                c.update(deconv=True, s=2)
+            elif form == "tokens":
+                c.update(N=1, H=1, W=_log(rng, 1, 8192), C=_log(rng, 16, 2048), K=_log(rng, 16, 2048), k=1, s=1)
+            w = work(c)
+            if w["flops"] <= 5e10 and w["bytes"] <= 3e8 and c["N"] * c["H"] * c["W"] * max(c["C"], c["K"]) <= 4e7:
+                return c
+    while True:
+        g = rng.choice([1, 1, 2])
+        C = 4 * _log(rng, 1, 256)
+        M = g * _log(rng, 1, 800000)
+        if M * C <= 2.4e7:
+            break
+    cs, co = C, 0
+    if rng.random() < 0.5:
+        co = 4 * rng.randrange(0, 17)
+        cs = C + co + 4 * rng.randrange(0, 17)
+    return dict(kind=kind, M=M, C=C, groups=g, cs=cs, co=co)
+
+
+def _same(n, k, s):
+    out = -(-n // s)
+    return out, max((out - 1) * s + k - n, 0) // 2
+
+
+def _geometry(case):
+    """Output size and the (input pixel, tap) pairs of every output row / column: [(o, i, t), ...] per axis."""
+    H, W, k, s = case["H"], case["W"], case["k"], case["s"]
+    if not case["deconv"]:
+        OH, pt = _same(H, k, s)
+        OW, pl = _same(W, k, s)
+    else:
+        OH, OW = H * s, W * s
+        _, pt = _same(OH, k, s)
+        _, pl = _same(OW, k, s)
+    return OH, OW, pt, pl
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def randn(*shape):
+        return torch.randn(shape, generator=g, device="cuda")
+
+    def rand(*shape):
+        return torch.rand(shape, generator=g, device="cuda")
+
+    st = dict(case=dict(case))
+    C = case["C"]
+    if case["kind"] == "conv8":
+        N, H, W, K, k = (case[n] for n in ("N", "H", "W", "K", "k"))
+        # what a layer reads: activations after a ReLU (channels of different strength), the last channel a disparity
+        cp = (C + 3) // 4 * 4
+        buf = torch.zeros(N, H, W, cp, device="cuda")
+        buf[..., :C] = (randn(N, H, W, C) * (0.5 + rand(C))).clamp_(min=0)
+        buf[..., C - 1] = 4 * torch.sigmoid(buf[..., C - 1])
+        st["x"] = buf[..., :C]
+        lim = (6.0 / (k * k * (C + K))) ** 0.5
+        w = (2 * rand(k, k, C, K) - 1) * lim * (0.5 + 2 * rand(K))      # folded weights: a factor per channel
+        st["w"] = w.permute(0, 1, 3, 2).contiguous() if case["deconv"] else w
+        st["b"] = 0.3 * randn(K)
+        OH, OW, _, _ = _geometry(case)
+        st["y"] = torch.empty(N, OH, OW, K, device="cuda")
+        if own:
+            from tf_depth_estimation_amd import int8
+            st["conv"] = int8.Conv8(st["w"], st["b"], stride=case["s"], deconv=case["deconv"], relu=case["relu"])
+        else:
+            w2 = st["w"].transpose(2, 3) if case["deconv"] else st["w"]           # [k, k, C, K]
+            wd = w2.double()
+            a = wd.abs().amax(dim=(0, 1, 2))
+            inv = torch.where(a > 0, a, torch.ones_like(a))
+            st["wq"] = torch.round(wd * 127 / inv).float()
+            st["ws"] = (a / 127).float()
+        return st
+    M, G = case["M"], case["groups"]
+    st["beta"] = 0.3 * randn(C)
+    if case["kind"] == "tape_fwd":
+        st["z"] = randn(M, C) * (0.2 + rand(C)) + 0.5 * randn(C)
+        st["y"] = torch.zeros(M, case["cs"], device="cuda")
+        return st
+    # the tape of a forward pass, as codes and scales; the gradient of a loss (a mean over pixels) with its holes
+    u = randn(M, C) + st["beta"]
+    st["codes"], st["scales"] = _code(u.double())
+    st["invstd"] = 0.5 + 2 * rand(G, C)
+    st["dy"] = randn(M, case["cs"]) * (10 ** (rand(M, 1) * 2 - 6)) * (rand(M, 1) < 0.9)
+    if own:
+        from tf_depth_estimation_amd import int8
+        st["tape"] = int8.Tape8(st["codes"], st["scales"], st["invstd"])
+    return st
+
+
+def _blocks(u):
+    """[M, C] -> [M, blocks, BLOCK], zero padded."""
+    M, C = u.shape
+    nb = (C + BLOCK - 1) // BLOCK
+    return torch.nn.functional.pad(u, (0, nb * BLOCK - C)).view(M, nb, BLOCK)
+
+
+def _code(u):
+    """8-bit codes [M, C] and scales [M, blocks] of pre-activations (float64)."""
+    M, C = u.shape
+    a = _blocks(u).abs().amax(dim=2)
+    ac = a.repeat_interleave(BLOCK, dim=1)[:, :C]
+    t = (u.abs() * 128 / torch.where(ac > 0, ac, torch.ones_like(ac))).floor_().clamp_(max=127)
+    q = torch.where(u > 0, t, -1 - t)
+    return q.to(torch.int8), a.float() / 128
+
+
+def _value(codes, scales):
+    C = codes.shape[1]
+    return (codes.float() + 0.5) * scales.repeat_interleave(BLOCK, dim=1)[:, :C]
+
+
+# ---------------------------------------------------------------- one pass
+
+def run(st):
+    case = st["case"]
+    return (_run_own if own else _run_plain)(case["kind"], case, st)
+
+
+def _run_own(kind, case, st):
+    from tf_depth_estimation_amd import int8
+    if kind == "conv8":
+        return st["conv"](st["x"], out=st["y"])
+    C, co = case["C"], case["co"]
+    if kind == "tape_fwd":
+        y, tape = int8.bn_relu_forward(st["z"], st["beta"], groups=case["groups"], eps=EPS, out=st["y"][:, co:co + C])
+        return dict(y=y, mean=tape.mean, invstd=tape.invstd, tape=tape.restore(relu=False))
+    dz, dbeta = int8.bn_relu_backward(st["tape"], st["beta"], st["dy"][:, co:co + C])
+    return dict(dz=dz, dbeta=dbeta)
+
+
+def _run_plain(kind, case, st):
+    C = case["C"]
+    if kind == "conv8":
+        return _plain_conv(case, st)
+    G, co = case["groups"], case["co"]
+    M = case["M"]
+    if kind == "tape_fwd":
+        z = st["z"].double().view(G, M // G, C)
+        mean = z.mean(dim=1, keepdim=True)
+        var = ((z - mean) ** 2).mean(dim=1, keepdim=True)
+        invstd = 1 / torch.sqrt(var + EPS)
+        u = ((z - mean) * invstd + st["beta"].double()).view(M, C)
+        st["y"][:, co:co + C] = u.clamp(min=0).float()
+        codes, scales = _code(u)
+        return dict(y=st["y"][:, co:co + C], mean=mean.float().view(G, C), invstd=invstd.float().view(G, C),
+                    tape=_value(codes, scales))
+    dy = st["dy"][:, co:co + C].view(G, M // G, C) if co == 0 and case["cs"] == C else \
+        st["dy"][:, co:co + C].reshape(G, M // G, C)
+    codes = st["codes"].view(G, M // G, C)
+    xh = _value(st["codes"], st["scales"]).view(G, M // G, C) - st["beta"]
+    gr = torch.where(codes >= 0, dy, torch.zeros_like(dy))
+    sg = gr.double().sum(dim=1, keepdim=True)
+    sx = (gr * xh).double().sum(dim=1, keepdim=True)
+    n = M // G
+    dz = st["invstd"].view(G, 1, C) * (gr - (sg / n).float() - xh * (sx / n).float())
+    return dict(dz=dz.view(M, C), dbeta=sg.sum(dim=(0, 1)).float())
+
+
+def _plain_conv(case, st):
+    N, H, W, C, K, k, s = (case[n] for n in ("N", "H", "W", "C", "K", "k", "s"))
+    x, wq, ws = st["x"], st["wq"], st["ws"]
+    OH, OW, pt, pl = _geometry(case)
+    a = x.abs().amax(dim=3, keepdim=True)
+    q = torch.round(x.double() * 127 / torch.where(a > 0, a, torch.ones_like(a))).float()
+    sx = (a.double() / 127).float()
+    y = torch.zeros(N, OH, OW, K, device=x.device)
+    for ky in range(k):
+        for kx in range(k):
+            if case["deconv"]:
+                # out(o) gets in(i) through tap t where o = s i + t - pad
+                i0, i1 = _span(H, OH, s, ky - pt)
+                j0, j1 = _span(W, OW, s, kx - pl)
+                if i0 >= i1 or j0 >= j1:
+                    continue
+                p = (q[:, i0:i1, j0:j1].reshape(-1, C) @ wq[ky, kx]).view(N, i1 - i0, j1 - j0, K)
+                y[:, s * i0 + ky - pt:s * (i1 - 1) + ky - pt + 1:s, s * j0 + kx - pl:s * (j1 - 1) + kx - pl + 1:s] += \
+                    p * sx[:, i0:i1, j0:j1]
+            else:
+                # out(o) reads in(i) through tap t where i = s o + t - pad
+                i0, i1 = _span(OH, H, s, ky - pt)
+                j0, j1 = _span(OW, W, s, kx - pl)
+                if i0 >= i1 or j0 >= j1:
+                    continue
+                si = slice(s * i0 + ky - pt, s * (i1 - 1) + ky - pt + 1, s)
+                sj = slice(s * j0 + kx - pl, s * (j1 - 1) + kx - pl + 1, s)
+                p = (q[:, si, sj].reshape(-1, C) @ wq[ky, kx]).view(N, i1 - i0, j1 - j0, K)
+                y[:, i0:i1, j0:j1] += p * sx[:, si, sj]
+    y = y * ws + st["b"]
+    return torch.where(y < 0, torch.zeros_like(y), y) if case["relu"] else y
+
+
+def _span(n, limit, s, off):
+    """Half-open range of r in [0, n) with 0 <= s r + off < limit."""
+    lo = max(0, -(off // s)) if off < 0 else 0
+    hi = min(n, (limit - 1 - off) // s + 1)
+    return lo, hi
+
+
+# ---------------------------------------------------------------- cost and definition
+
+def work(case):
+    if case["kind"] == "conv8":
+        N, H, W, C, K, k = (case[n] for n in ("N", "H", "W", "C", "K", "k"))
+        OH, OW, _, _ = _geometry(case)
+        rows = N * H * W if case["deconv"] else N * OH * OW
+        return {"bytes": 4 * N * H * W * C + k * k * C * K + 8 * K + 4 * N * OH * OW * K,
+                "flops": 2 * rows * k * k * C * K}
+    M, C = case["M"], case["C"]
+    nb = (C + BLOCK - 1) // BLOCK
+    tape = M * C + 4 * M * nb
+    if case["kind"] == "tape_fwd":
+        # z in, y and the tape out, the tape in again and its values out
+        return {"bytes": 4 * M * C + 4 * M * C + 2 * tape + 4 * M * C, "flops": 12 * M * C}
+    return {"bytes": tape + 4 * M * C + 4 * M * C, "flops": 10 * M * C}
+
+
+def exact(case, seed):
+    """The outputs from the definition, in 64 bits."""
+    if work(case)["flops"] > 2e11:
+        return None
+    global own
+    was, own = own, False
+    try:
+        st = prepare(case, seed)
+    finally:
+        own = was
+    C = case["C"]
+    if case["kind"] == "conv8":
+        return _exact_conv(case, st)
+    M, G = case["M"], case["groups"]
+    n = M // G
+    beta = st["beta"].double()
+    if case["kind"] == "tape_fwd":
+        us, means, invs = [], [], []
+        for z in st["z"].double().split(n):
+            mu = z.sum(0) / n
+            d = z - mu
+            r = ((d * d).sum(0) / n + EPS) ** -0.5
+            us.append(torch.addcmul(beta.expand_as(d), d, r.expand_as(d)))
+            means.append(mu)
+            invs.append(r)
+        u = torch.cat(us)
+        tape = torch.empty_like(u)
+        for c0 in range(0, C, BLOCK):
+            ub = u[:, c0:c0 + BLOCK]
+            step = ub.abs().max(dim=1, keepdim=True).values / 128
+            m = torch.trunc(ub / torch.where(step > 0, step, torch.ones_like(step))).clamp(-127, 127)
+            tape[:, c0:c0 + BLOCK] = torch.where(ub > 0, m + 0.5, m - 0.5) * step
+        return dict(y=torch.relu(u), mean=torch.stack(means), invstd=torch.stack(invs), tape=tape)
+    step = torch.cat([st["scales"].double()[:, b:b + 1].expand(M, min(BLOCK, C - BLOCK * b))
+                      for b in range(st["scales"].shape[1])], dim=1)
+    u = (st["codes"].double() + 0.5) * step
+    on = (u > 0).double() if bool((step > 0).all()) else (st["codes"] >= 0).double()
+    dy = st["dy"].double()[:, case["co"]:case["co"] + C] * on
+    dzs, db = [], torch.zeros(C, dtype=torch.float64, device="cuda")
+    for i in range(G):
+        gr, xh = dy[i * n:(i + 1) * n], u[i * n:(i + 1) * n] - beta
+        s0, s1 = gr.sum(0), (gr * xh).sum(0)
+        dzs.append((gr - s0 / n - xh * (s1 / n)) * st["invstd"][i].double())
+        db += s0
+    return dict(dz=torch.cat(dzs), dbeta=db)
+
+
+def _exact_conv(case, st):
+    """The sum over taps and channels as one float64 product per image (rows of a patch matrix)."""
+    N, H, W, C, K, k, s = (case[n] for n in ("N", "H", "W", "C", "K", "k", "s"))
+    x = st["x"].double()
+    top = x.abs().max(dim=3, keepdim=True).values
+    step = top / 127
+    xv = torch.round(x / torch.where(top > 0, top, torch.ones_like(top)) * 127) * step
+    w = st["w"].double()
+    if case["deconv"]:
+        w = w.permute(0, 1, 3, 2)
+    wtop = w.abs().reshape(-1, K).max(dim=0).values
+    wv = (torch.round(w / torch.where(wtop > 0, wtop, torch.ones_like(wtop)) * 127) * (wtop / 127)).reshape(-1, K)
+    OH, OW, pt, pl = _geometry(case)
+    oh = torch.arange(OH, device="cuda").view(OH, 1)
+    ow = torch.arange(OW, device="cuda").view(OW, 1)
+    t = torch.arange(k, device="cuda").view(1, k)
+    if case["deconv"]:
+        ih, iw = oh + pt - t, ow + pl - t
+        okh, okw = ih % s == 0, iw % s == 0
+        ih, iw = torch.div(ih, s, rounding_mode="floor"), torch.div(iw, s, rounding_mode="floor")
+    else:
+        ih, iw = oh * s + t - pt, ow * s + t - pl
+        okh, okw = torch.ones_like(ih, dtype=torch.bool), torch.ones_like(iw, dtype=torch.bool)
+    okh, okw = okh & (ih >= 0) & (ih < H), okw & (iw >= 0) & (iw < W)
+    ih, iw = torch.where(okh, ih, H), torch.where(okw, iw, W)          # row / column of zeros
+    out = torch.empty(N, OH, OW, K, dtype=torch.float64, device="cuda")
+    rows = max(1, int(2e8 // (OW * k * k * C)))
+    for i in range(N):
+        pad = torch.zeros(H + 1, W + 1, C, dtype=torch.float64, device="cuda")
+        pad[:H, :W] = xv[i]
+        for r in range(0, OH, rows):
+            patch = pad[ih[r:r + rows].view(-1, 1, k, 1), iw.view(1, OW, 1, k)]      # [rows, OW, k, k, C]
+            out[i, r:r + rows] = (patch.reshape(-1, k * k * C) @ wv).view(-1, OW, K)
+    out += st["b"].double()
+    return out.clamp(min=0) if case["relu"] else out
