@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define TDE_ABI_VERSION 10
+#define TDE_ABI_VERSION 11
 
 /* An operand bound (tde_conv_desc_t.*_absmax, tde_bn_bwd dz_absmax) is an array of this many floats whose
  * maximum is the bound: producers raise one slot per workgroup (atomic max), consumers read all. */
@@ -276,6 +276,80 @@ int tde_bn_bwd_from_sums(int M, int C, int groups, long M_total, const float* z,
                          const float* save_invstd, const float* beta, const float* dy, int dy_cstride, int dy_coff,
                          const double* global_sums, const double* local_sums, float* dz, float* dbeta,
                          int accumulate_dbeta, int relu, float* dz_absmax, void* stream);
+
+/* ---------------------------------------------------------------- 8-bit activations (ABI 11)
+ * Two uses of activations held as 8-bit codes with fp32 scales.  Neither has a counterpart in the reference, whose
+ * path is fp32 throughout; both are opt-in (Predictor(int8=True), Trainer.enable_tape8).
+ *
+ * (1) Integer product, a pixel being a token.  A row (pixel) of C channels becomes codes q = rne(127 x / a),
+ * a = max |x| over its channels, with ONE scale a / 127 (a = 0: codes and scale 0; a row that holds a NaN or an
+ * infinity: codes 0, scale NaN, so every output that reads the pixel is NaN).  rne is exact (ties to even on the
+ * real quotient), so codes do not depend on how the quotient is computed.
+ *   codes  [rows + 1][Cp] int8, Cp = tde_q8_row_bytes(C) (C rounded up to 32, above 32 to 64; padding codes are 0),
+ *   scales [rows + 1] float;  row `rows` is all zero: the pixel outside the image that 'SAME' padding reads.
+ * C <= 4096 (an integer sum over C * 127 * 127 stays far below 2^31).  x: any channel view; pixel stride and offset
+ * need no alignment. */
+int tde_q8_row_bytes(int C);
+int tde_q8_rows(int rows, int C, const float* x, int x_cstride, int x_coff, int8_t* codes, float* scales, void* stream);
+/* Weights: the same rule per OUTPUT channel over all taps and input channels.  layout 0: conv [taps][cin][K], 1:
+ * conv2d_transpose [taps][K][cin] (as tde_bn_fold).  codes [taps][Kp][Cp], Cp = tde_q8_row_bytes(cin), scales [Kp],
+ * Kp = K rounded up to 16 (padding zero); tde_q8_weights_size is the bytes of the codes. */
+size_t tde_q8_weights_size(int taps, int cin, int K);
+int tde_q8_weights(int taps, int cin, int K, int layout, const float* w, int8_t* codes, float* scales, void* stream);
+/* y = relu?( w_scale[k] * sum_tap x_scale[pixel(tap)] * (sum_c x_code * w_code) + bias[k] ): the inner sum in exact
+ * 32-bit integers on the matrix cores, the outer sum over taps in fp32; a 1x1 conv is the plain product of tokens and
+ * weights.  NaN outputs stay NaN under relu.  `d` as for tde_conv2d_fwd_bias_act / tde_deconv2d_fwd_bias_act, except
+ * that the input is the codes of tde_q8_rows on the layer's input pixels, so its view fields are not read (conv:
+ * w_cin channels; deconv: K), and that K (conv) / C (deconv) and the output view need no alignment.  bias may be
+ * NULL. */
+int tde_q8_conv2d_bias_act(const tde_conv_desc_t* d, const int8_t* x_codes, const float* x_scales,
+                           const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y,
+                           void* stream);
+int tde_q8_deconv2d_bias_act(const tde_conv_desc_t* d, const int8_t* x_codes, const float* x_scales,
+                             const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y_big,
+                             void* stream);
+
+/* (2) The 8-bit tape of training BatchNorm + ReLU: what the backward pass needs of a layer -- its pre-BN output z, the
+ * ReLU mask and its output y -- as ONE 8-bit code per element instead of two fp32 tensors.  The pre-activation
+ * u = (z - mean) * invstd + beta (evaluated in fp64) is coded per row in blocks of TDE_TAPE8_BLOCK channels:
+ *   s = (float)max|u| / 128,  code = min(floor(|u| / s), 127) for u > 0,  -1 - min(floor(|u| / s), 127) for u <= 0,
+ * a mid-rise code of value (code + 1/2) s: off by at most s / 2 (and the rounding of s, 2^-17 s, at the block's
+ * maximum), and code >= 0 IS u > 0, so the mask is exact.
+ * A block that holds a NaN or an infinity has scale NaN (its restored values are NaN).
+ *   codes [M][C] int8, scales [M][ceil(C / TDE_TAPE8_BLOCK)] float; both 16-byte aligned.
+ * M rows are `groups` equal row groups, each its own BatchNorm batch (tde_bn_fwd_train).  C % 4 == 0, C <= 1024.
+ * Sums are fp64 in a fixed order: results do not change from run to run. */
+#define TDE_TAPE8_BLOCK 64
+size_t tde_tape8_workspace_size(int M, int C);
+/* z dense [M][C] -> y = relu(u) into its channel view, save_mean / save_invstd [groups][C], moving averages (both NULL:
+ * no update) and the tape; semantics of tde_bn_fwd_train with relu = 1. */
+int tde_tape8_bn_fwd(int M, int C, int groups, const float* z, const float* beta, float eps, float decay, int bessel,
+                     float* moving_mean, float* moving_var, float* save_mean, float* save_invstd, float* y,
+                     int y_cstride, int y_coff, int8_t* codes, float* scales, void* ws, size_t ws_bytes, void* stream);
+/* The same from the (all-reduced) sums of tde_bn_sums(mode 0) / tde_bn_train_t.sums over M_total rows per group. */
+int tde_tape8_bn_fwd_from_sums(int M, int C, int groups, long M_total, const float* z, const double* sums,
+                               const float* beta, float eps, float decay, int bessel, float* moving_mean,
+                               float* moving_var, float* save_mean, float* save_invstd, float* y, int y_cstride,
+                               int y_coff, int8_t* codes, float* scales, void* stream);
+/* The tape's values into a channel view: relu 1: max((code + 1/2) s, 0), the layer's output as its consumers' filter
+ * gradients read it; relu 0: the coded pre-activation. */
+int tde_tape8_restore(int M, int C, const int8_t* codes, const float* scales, int relu, float* y, int y_cstride,
+                      int y_coff, void* stream);
+/* Backward from the tape: g = dy where code >= 0 else 0, xhat = (code + 1/2) s - beta,
+ * dz = invstd (g - mean g - xhat mean(g xhat)) (means over a group's rows), dbeta (+)= sum g; dz_absmax as tde_bn_bwd.
+ * beta is the one of the forward. */
+int tde_tape8_bn_bwd(int M, int C, int groups, const int8_t* codes, const float* scales, const float* save_invstd,
+                     const float* beta, const float* dy, int dy_cstride, int dy_coff, float* dz, float* dbeta,
+                     int accumulate_dbeta, float* dz_absmax, void* ws, size_t ws_bytes, void* stream);
+/* In two phases around the caller's all-reduce (SyncBN): sums [groups][2][C] = (sum g, sum g xhat), then dz from the
+ * global sums over M_total rows per group and dbeta from the local ones, as tde_bn_sums / tde_bn_bwd_from_sums. */
+int tde_tape8_bn_bwd_sums(int M, int C, int groups, const int8_t* codes, const float* scales, const float* beta,
+                          const float* dy, int dy_cstride, int dy_coff, double* sums, double* sums_copy, void* ws,
+                          size_t ws_bytes, void* stream);
+int tde_tape8_bn_bwd_from_sums(int M, int C, int groups, long M_total, const int8_t* codes, const float* scales,
+                               const float* save_invstd, const float* beta, const float* dy, int dy_cstride,
+                               int dy_coff, const double* global_sums, const double* local_sums, float* dz,
+                               float* dbeta, int accumulate_dbeta, float* dz_absmax, void* stream);
 
 /* ---------------------------------------------------------------- legacy resizes
  * resize_like -> tf.image.resize_nearest_neighbor (nets_optflow_depth.py:11-16),

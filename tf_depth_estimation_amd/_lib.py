@@ -13,7 +13,7 @@ import torch  # noqa: F401  (must be imported first, see module docstring)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libtde.so")
-ABI_VERSION = 10
+ABI_VERSION = 11
 BOUND_SLOTS = 16   # TDE_BOUND_SLOTS: an operand bound is the max of this many device floats
 # tde_set_conv_math modes (include/tde.h): exact fp32 MFMA, bf16x3 (~2^-16 per product), and the
 # fp32-accurate three-way bf16 split ("bf16x6": staged in LDS / split in registers)
@@ -150,6 +150,22 @@ _SIGS = {
                                      P, P, c_int, c_int, c_int, P]),
     "tde_bn_bwd_from_sums": (c_int, [c_int, c_int, c_int, ctypes.c_long, P, P, P, P, P, c_int, c_int, P, P, P, P,
                                      c_int, c_int, P, P]),
+    "tde_q8_row_bytes": (c_int, [c_int]),
+    "tde_q8_rows": (c_int, [c_int, c_int, P, c_int, c_int, P, P, P]),
+    "tde_q8_weights_size": (c_size_t, [c_int, c_int, c_int]),
+    "tde_q8_weights": (c_int, [c_int, c_int, c_int, c_int, P, P, P, P]),
+    "tde_q8_conv2d_bias_act": (c_int, [P, P, P, P, P, P, c_int, P, P]),
+    "tde_q8_deconv2d_bias_act": (c_int, [P, P, P, P, P, P, c_int, P, P]),
+    "tde_tape8_workspace_size": (c_size_t, [c_int, c_int]),
+    "tde_tape8_bn_fwd": (c_int, [c_int, c_int, c_int, P, P, c_float, c_float, c_int, P, P, P, P, P, c_int, c_int, P, P,
+                                 P, c_size_t, P]),
+    "tde_tape8_bn_fwd_from_sums": (c_int, [c_int, c_int, c_int, ctypes.c_long, P, P, P, c_float, c_float, c_int, P, P,
+                                           P, P, P, c_int, c_int, P, P, P]),
+    "tde_tape8_restore": (c_int, [c_int, c_int, P, P, c_int, P, c_int, c_int, P]),
+    "tde_tape8_bn_bwd": (c_int, [c_int, c_int, c_int, P, P, P, P, P, c_int, c_int, P, P, c_int, P, P, c_size_t, P]),
+    "tde_tape8_bn_bwd_sums": (c_int, [c_int, c_int, c_int, P, P, P, P, c_int, c_int, P, P, P, c_size_t, P]),
+    "tde_tape8_bn_bwd_from_sums": (c_int, [c_int, c_int, c_int, ctypes.c_long, P, P, P, P, P, c_int, c_int, P, P, P, P,
+                                           c_int, P, P]),
     "tde_resize_nearest_fwd": (c_int, [c_int] * 4 + [P, c_int, c_int, c_int, c_int, P, c_int, c_int, P]),
     "tde_resize_nearest_bwd": (c_int, [c_int] * 4 + [P, c_int, c_int, c_int, c_int, c_int, P, c_int, c_int, P]),
     "tde_resize_bilinear_fwd": (c_int, [c_int] * 4 + [P, c_int, c_int, c_int, c_int, P, c_int, c_int, P]),

@@ -313,23 +313,6 @@ __global__ void __launch_bounds__(256) bn_apply_kernel(int M, int C, const float
   }
 }
 
-// max|dz| of a block's values into one of the TDE_BOUND_SLOTS slots of amax (slot = block % slots, so that
-// at most blocks / 16 atomics contend for an address; a bound is the max of its slots): the fp16x3 conv
-// math's operand bound of the gradient (tde_conv_desc_t.y_absmax).  uint order = float order for
-// non-negative floats; fmaxf from 0 keeps NaN out of the bound.  Every thread of the block must call it.
-__device__ __forceinline__ void block_absmax_to(float m, float* amax) {
-  __shared__ float wmx[4];
-  if (amax == nullptr) return;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  if ((threadIdx.x & 63) == 0) wmx[threadIdx.x >> 6] = m;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    m = fmaxf(fmaxf(wmx[0], wmx[1]), fmaxf(wmx[2], wmx[3]));
-    if (m > 0.f) atomicMax(reinterpret_cast<unsigned*>(amax + (blockIdx.x & (TDE_BOUND_SLOTS - 1))), __float_as_uint(m));
-  }
-}
-
 // coef = (mean g, mean g*xhat) of row group g: from the finalize's coef, or (SUMS) from the all-reduced sums over
 // P.Mt rows (fp64 quotient, one fp32 rounding)
 template <bool SUMS>

@@ -1,0 +1,322 @@
+"""Activations held as 8-bit codes with fp32 scales: an integer conv for prediction and an 8-bit tape for training.
+
+The reference computes and keeps everything in fp32 (nets_optflow_depth.py:76-147 has no reduced form); both uses are
+opt-in here.
+
+  * `Conv8` -- a conv / transposed conv + bias + ReLU as a product of 8-bit integers with one scale per input pixel
+    (token) and one per output channel; a 1x1 conv on [M, C] rows is the plain product of tokens and weights.
+    `batch_prediction.Predictor(int8=True)` runs every folded conv layer this way.
+  * `bn_relu_forward` / `bn_relu_backward` / `Tape8` -- training BatchNorm + ReLU whose backward needs one byte per
+    element (the coded pre-activation: its sign is the ReLU mask, its value both the normalised input and, through
+    `Tape8.restore`, the layer's output).  `program.NetRun(tape8=True)`, `train.Trainer.enable_tape8` and `tape8()` use
+    it for whole networks.
+
+Like the rest of the package these are calls on the current stream of the current device without a CPU fallback;
+none of them records an autograd graph (an input that requires a gradient is refused while gradients are enabled).
+The formulas stand in include/tde.h, "8-bit activations".
+"""
+import contextlib
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import ConvDesc, ptr
+from .program import same_pad
+
+BLOCK = 64            # TDE_TAPE8_BLOCK: channels of a row that share a tape scale
+MAX_CHANNELS = 4096   # of a Conv8 input
+
+
+def _check(t, name, dtype=torch.float32):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda:
+        raise ValueError(f"{name} must be a {str(dtype).split('.')[-1]} tensor on the GPU")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, not on the current device (cuda:{torch.cuda.current_device()})")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: 8-bit operators record none (detach it, or use torch.no_grad())")
+
+
+def _rows(t, name):
+    """(rows, C, pixel stride) of a [..., C] channel view: consecutive pixels a fixed stride apart."""
+    if t.dim() < 2:
+        raise ValueError(f"{name} must have at least two dimensions, got {tuple(t.shape)}")
+    C = t.shape[-1]
+    rows, cs = 1, None
+    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n != 1:
+            if cs is None:
+                cs = s
+            elif s != rows * cs:
+                raise ValueError(f"{name} must be a pixel-major channel view (strides {t.stride()})")
+        rows *= n
+    cs = C if cs is None else cs
+    if rows and (C == 0 or (C > 1 and t.stride(-1) != 1) or cs < C):
+        raise ValueError(f"{name} must be a pixel-major channel view of at least one channel (strides {t.stride()})")
+    return rows, C, cs
+
+
+def _out(out, shape, like, name="out"):
+    if out is None:
+        return torch.empty(shape, dtype=torch.float32, device=like.device)
+    _check(out, name)
+    if tuple(out.shape) != tuple(shape):
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(out.shape)}")
+    return out
+
+
+# ---------------------------------------------------------------- integer product
+class Rows8:
+    """Pixels as 8-bit codes [rows + 1, row_bytes(C)] with a scale each [rows + 1] (the last row is all zero: the
+    pixel outside the image); `shape` is the fp32 tensor's."""
+
+    def __init__(self, codes, scales, shape):
+        self.codes, self.scales, self.shape = codes, scales, tuple(shape)
+
+
+def row_bytes(C):
+    n = _lib.load().tde_q8_row_bytes(C)
+    if n <= 0:
+        raise ValueError(f"{C} channels: 1 to {MAX_CHANNELS} are supported")
+    return n
+
+
+def quantize_rows(x, out=None):
+    """fp32 [..., C] channel view -> Rows8.  out: a Rows8 to write into (a captured step's own buffers)."""
+    _check(x, "x")
+    rows, C, cs = _rows(x, "x")
+    cp = row_bytes(C)
+    if out is None:
+        out = Rows8(torch.empty((rows + 1, cp), dtype=torch.int8, device=x.device),
+                    torch.empty(rows + 1, dtype=torch.float32, device=x.device), x.shape)
+    else:
+        if tuple(out.codes.shape) != (rows + 1, cp) or tuple(out.scales.shape) != (rows + 1,):
+            raise ValueError(f"out holds {tuple(out.codes.shape)} codes, x needs {(rows + 1, cp)}")
+        out.shape = tuple(x.shape)
+    if rows:
+        lib = _lib.load()
+        _lib.check(lib.tde_q8_rows(rows, C, ptr(x), cs, 0, ptr(out.codes), ptr(out.scales), _lib.stream_ptr()),
+                   "quantize_rows")
+    return out
+
+
+class Conv8:
+    """One conv layer in 8-bit integers: y = relu?(conv(x, weights) + bias), TF 'SAME' padding.
+
+    weights: conv [KH, KW, Cin, Cout], or with deconv=True conv2d_transpose [KH, KW, Cout, Cin] (the TF checkpoint
+    layouts), fp32.  They are quantised once (per output channel) by __init__ / load; later changes of the tensor are not
+    seen, as with NetProgram.fold_bn."""
+
+    def __init__(self, weights, bias=None, stride=1, relu=True, deconv=False):
+        if not isinstance(stride, int) or not 1 <= stride <= 64:
+            raise ValueError(f"stride {stride!r}: an integer from 1 to 64 is expected")
+        self.stride, self.relu, self.deconv = stride, bool(relu), bool(deconv)
+        self.load(weights, bias)
+
+    def load(self, weights, bias=None):
+        _check(weights, "weights")
+        if weights.dim() != 4 or 0 in weights.shape:
+            raise ValueError(f"weights must be [KH, KW, Cin, Cout] or [KH, KW, Cout, Cin], got {tuple(weights.shape)}")
+        kh, kw, a, b = weights.shape
+        cin, K = (b, a) if self.deconv else (a, b)
+        if max(kh, kw) > 64 or K > 65535:
+            raise ValueError(f"weights {tuple(weights.shape)}: at most 64x64 taps and 65535 output channels")
+        row_bytes(cin)
+        if bias is not None:
+            _check(bias, "bias")
+            if tuple(bias.shape) != (K,):
+                raise ValueError(f"bias must be ({K},), got {tuple(bias.shape)}")
+        lib = _lib.load()
+        w = weights.contiguous()
+        self.kh, self.kw, self.cin, self.K = kh, kw, cin, K
+        self.codes = torch.empty(lib.tde_q8_weights_size(kh * kw, cin, K), dtype=torch.int8, device=w.device)
+        self.scales = torch.empty((K + 15) // 16 * 16, dtype=torch.float32, device=w.device)
+        self.bias = None if bias is None else bias.detach().clone().contiguous()
+        _lib.check(lib.tde_q8_weights(kh * kw, cin, K, 1 if self.deconv else 0, ptr(w), ptr(self.codes),
+                                      ptr(self.scales), _lib.stream_ptr()), "Conv8 weights")
+        return self
+
+    def out_size(self, H, W):
+        if self.deconv:
+            return H * self.stride, W * self.stride
+        return same_pad(H, self.kh, self.stride)[0], same_pad(W, self.kw, self.stride)[0]
+
+    def desc(self, N, H, W, ocs):
+        """The conv descriptor of a batch (a transposed conv's is that of its virtual forward conv)."""
+        OH, OW = self.out_size(H, W)
+        d = ConvDesc()
+        big, small = ((OH, OW), (H, W)) if self.deconv else ((H, W), (OH, OW))
+        d.N, (d.H, d.W), (d.OH, d.OW) = N, big, small
+        d.C, d.K = (self.K, self.cin) if self.deconv else (self.cin, self.K)
+        d.w_cin = d.C
+        d.KH, d.KW, d.stride = self.kh, self.kw, self.stride
+        d.pad_top, d.pad_left = same_pad(d.H, self.kh, self.stride)[1], same_pad(d.W, self.kw, self.stride)[1]
+        d.x_cstride = d.C
+        d.y_cstride = d.K
+        if self.deconv:
+            d.x_cstride = ocs
+        else:
+            d.y_cstride = ocs
+        return d
+
+    def __call__(self, x, out=None):
+        """x: fp32 [N, H, W, Cin] channel view (or its Rows8), or [M, Cin] rows for a 1x1 stride-1 conv.  Returns
+        [N, OH, OW, Cout] ([M, Cout]), written into the channel view `out` if given."""
+        x8 = x if isinstance(x, Rows8) else quantize_rows(x)
+        shape = x8.shape
+        if shape[-1] != self.cin:
+            raise ValueError(f"x has {shape[-1]} channels, the weights {self.cin}")
+        if len(shape) == 2 and (self.kh, self.kw, self.stride) == (1, 1, 1):
+            N, H, W = 1, 1, shape[0]
+        elif len(shape) == 4:
+            N, H, W = shape[:3]
+        else:
+            raise ValueError(f"x must be [N, H, W, C], or [M, C] for a 1x1 stride-1 conv, got {shape}")
+        OH, OW = self.out_size(H, W)
+        oshape = (W, self.K) if len(shape) == 2 else (N, OH, OW, self.K)
+        y = _out(out, oshape, x8.codes)
+        rows, _, ocs = _rows(y, "out")
+        if rows:
+            lib = _lib.load()
+            fn = lib.tde_q8_deconv2d_bias_act if self.deconv else lib.tde_q8_conv2d_bias_act
+            _lib.check(fn(ctypes.byref(self.desc(N, H, W, ocs)), ptr(x8.codes), ptr(x8.scales), ptr(self.codes),
+                          ptr(self.scales), ptr(self.bias), int(self.relu), ptr(y), _lib.stream_ptr()), "Conv8")
+        return y
+
+
+# ---------------------------------------------------------------- 8-bit tape
+class Tape8:
+    """What the backward of one BatchNorm + ReLU keeps: codes [..., C] (int8), scales [..., ceil(C / 64)], the inverse
+    standard deviations [groups, C] (and the means, when the forward made it)."""
+
+    def __init__(self, codes, scales, invstd, mean=None):
+        _check(codes, "codes", torch.int8)
+        _check(scales, "scales")
+        _check(invstd, "invstd")
+        C = codes.shape[-1] if codes.dim() >= 2 else 0
+        if C == 0 or C % 4 or C > 1024:
+            raise ValueError(f"codes must be [..., C] with C a multiple of 4 up to 1024, got {tuple(codes.shape)}")
+        if tuple(scales.shape) != tuple(codes.shape[:-1]) + ((C + BLOCK - 1) // BLOCK,):
+            raise ValueError(f"scales {tuple(scales.shape)} do not fit codes {tuple(codes.shape)}")
+        if invstd.dim() != 2 or invstd.shape[1] != C:
+            raise ValueError(f"invstd must be [groups, {C}], got {tuple(invstd.shape)}")
+        if not (codes.is_contiguous() and scales.is_contiguous() and invstd.is_contiguous()):
+            raise ValueError("codes, scales and invstd must be contiguous")
+        self.codes, self.scales, self.invstd, self.mean = codes, scales, invstd, mean
+        self.C, self.rows, self.groups = C, codes.numel() // C, invstd.shape[0]
+        _check_groups(self.rows, self.groups)
+
+    def restore(self, relu=True, out=None):
+        """The tape's values [..., C]: relu=True the layer's output as the consumers' filter gradients read it, relu=False
+        the coded pre-activation."""
+        y = _out(out, self.codes.shape, self.codes)
+        rows, _, cs = _rows(y, "out")
+        _check_view(y, cs, "out")
+        if rows:
+            _lib.check(_lib.load().tde_tape8_restore(rows, self.C, ptr(self.codes), ptr(self.scales), int(bool(relu)),
+                                                     ptr(y), cs, 0, _lib.stream_ptr()), "Tape8.restore")
+        return y
+
+
+def _check_groups(rows, groups):
+    if not 1 <= groups <= 8 or rows % groups:
+        raise ValueError(f"{rows} rows are not {groups} equal groups (1 to 8)")
+
+
+def _check_view(t, cs, name):
+    if t.data_ptr() % 16 or cs % 4:
+        raise ValueError(f"{name}: the channel view must start on 16 bytes with a pixel stride of a multiple of 4")
+
+
+def _channels(z, beta):
+    C = z.shape[-1]
+    if C == 0 or C % 4 or C > 1024:
+        raise ValueError(f"{C} channels: a multiple of 4 up to 1024 is expected")
+    _check(beta, "beta")
+    if tuple(beta.shape) != (C,) or not beta.is_contiguous() or beta.data_ptr() % 16:
+        raise ValueError(f"beta must be a contiguous ({C},) tensor that starts on 16 bytes")
+    return C
+
+
+def _workspace(rows, C, device):
+    nb = _lib.load().tde_tape8_workspace_size(rows, C)
+    return torch.empty(nb, dtype=torch.uint8, device=device), nb
+
+
+def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel=True, out=None):
+    """Training BatchNorm (scale=False) + ReLU of z [..., C] (contiguous) that keeps an 8-bit tape: returns (y, Tape8).
+
+    The rows are `groups` equal consecutive groups, each normalised over its own rows.  moving: (moving_mean,
+    moving_variance), updated in place in group order.  out: a channel view for y (16-byte aligned)."""
+    _check(z, "z")
+    C = _channels(z, beta)
+    if z.dim() < 2 or not z.is_contiguous() or z.data_ptr() % 16:
+        raise ValueError("z must be a contiguous [..., C] tensor that starts on 16 bytes")
+    rows = z.numel() // C
+    if rows == 0:
+        raise ValueError("BatchNorm over no rows has no statistics")
+    _check_groups(rows, groups)
+    mm = mv = None
+    if moving is not None:
+        mm, mv = moving
+        for t in (mm, mv):
+            _check(t, "moving")
+            if tuple(t.shape) != (C,) or not t.is_contiguous():
+                raise ValueError(f"moving statistics must be contiguous ({C},) tensors")
+    y = _out(out, z.shape, z)
+    _, _, cs = _rows(y, "out")
+    _check_view(y, cs, "out")
+    codes = torch.empty(z.shape, dtype=torch.int8, device=z.device)
+    scales = torch.empty(tuple(z.shape[:-1]) + ((C + BLOCK - 1) // BLOCK,), dtype=torch.float32, device=z.device)
+    stats = torch.empty((2, groups, C), dtype=torch.float32, device=z.device)
+    ws, nb = _workspace(rows, C, z.device)
+    _lib.check(_lib.load().tde_tape8_bn_fwd(rows, C, groups, ptr(z), ptr(beta), eps, decay, int(bool(bessel)), ptr(mm),
+                                            ptr(mv), ptr(stats[0]), ptr(stats[1]), ptr(y), cs, 0, ptr(codes),
+                                            ptr(scales), ptr(ws), nb, _lib.stream_ptr()), "bn_relu_forward")
+    return y, Tape8(codes, scales, stats[1], stats[0])
+
+
+def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
+    """(dz, dbeta) of the layer whose forward made `tape`, from the gradient dy [..., C] (channel view) of its output;
+    beta as in that forward.  dz: a contiguous tensor to write; dbeta: a tensor to ADD to (a fresh one is written)."""
+    if not isinstance(tape, Tape8):
+        raise ValueError("tape must be a Tape8")
+    _check(dy, "dy")
+    C = _channels(dy, beta)
+    if tuple(dy.shape) != tuple(tape.codes.shape):
+        raise ValueError(f"dy must be {tuple(tape.codes.shape)}, got {tuple(dy.shape)}")
+    rows, _, cs = _rows(dy, "dy")
+    if rows == 0:
+        raise ValueError("BatchNorm over no rows has no gradient")
+    _check_view(dy, cs, "dy")
+    dz = _out(dz, dy.shape, dy, "dz")
+    if not dz.is_contiguous() or dz.data_ptr() % 16:
+        raise ValueError("dz must be contiguous and start on 16 bytes")
+    acc = dbeta is not None
+    dbeta = _out(dbeta, (C,), dy, "dbeta")
+    if not dbeta.is_contiguous():
+        raise ValueError("dbeta must be contiguous")
+    ws, nb = _workspace(rows, C, dy.device)
+    _lib.check(_lib.load().tde_tape8_bn_bwd(rows, C, tape.groups, ptr(tape.codes), ptr(tape.scales), ptr(tape.invstd),
+                                            ptr(beta), ptr(dy), cs, 0, ptr(dz), ptr(dbeta), int(acc), None, ptr(ws), nb,
+                                            _lib.stream_ptr()), "bn_relu_backward")
+    return dz, dbeta
+
+
+# ---------------------------------------------------------------- whole networks
+_TAPE8 = [False]
+
+
+@contextlib.contextmanager
+def tape8(on=True):
+    """`with int8.tape8(): outs = disp_net(images)`: the reference-named network functions called inside keep their
+    training tape in 8 bits (program.NetRun(tape8=True)); the backward may run outside."""
+    was, _TAPE8[0] = _TAPE8[0], bool(on)
+    try:
+        yield
+    finally:
+        _TAPE8[0] = was
+
+
+def tape8_active():
+    return _TAPE8[0]
