@@ -7,7 +7,7 @@ into the ParamChunk's flat gradient buffer (read them with `chunk.grad_view(name
 """
 import torch
 
-from . import variables
+from . import int8, variables
 from .program import NetProgram, NetRun
 
 _PROGRAMS = {}
@@ -34,8 +34,8 @@ def clear_programs():
 
 class _NetFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, anchor, x, prog, is_training):
-        run = NetRun(prog, x.shape[0])
+    def forward(ctx, anchor, x, prog, is_training, tape8):
+        run = NetRun(prog, x.shape[0], tape8=tape8)
         outs = prog.forward(run, x.detach(), is_training)
         ctx.run, ctx.prog = run, prog
         return tuple(outs)
@@ -44,7 +44,7 @@ class _NetFunction(torch.autograd.Function):
     def backward(ctx, *grads):
         need_x = ctx.needs_input_grad[1]
         dx = ctx.prog.backward(ctx.run, list(grads), need_input_grad=need_x)
-        return None, (dx.contiguous() if dx is not None else None), None, None
+        return None, (dx.contiguous() if dx is not None else None), None, None, None
 
 
 def run_net(net_scope, builder, x, is_training=True, **kw):
@@ -54,5 +54,5 @@ def run_net(net_scope, builder, x, is_training=True, **kw):
         raise ValueError("inputs must be float32 tensors on the GPU (the HIP path has no CPU fallback)")
     N, H, W, C = x.shape
     prog = get_program(net_scope, builder, H, W, C, **kw)
-    outs = _NetFunction.apply(prog.chunk.anchor, x, prog, is_training)
+    outs = _NetFunction.apply(prog.chunk.anchor, x, prog, is_training, bool(is_training) and int8.tape8_active())
     return list(outs), prog

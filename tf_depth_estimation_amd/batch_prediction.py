@@ -23,8 +23,8 @@ import ctypes
 
 import torch
 
-from . import _api, _lib, _netlib, checkpoint, pose_ops, variables
-from .program import NetRun
+from . import _api, _lib, _netlib, checkpoint, int8 as int8_ops, pose_ops, variables
+from .program import ConvBN, NetRun
 
 # net name -> (variable scope of the net, spec builder, input channels, builder kwargs, reference)
 NETS = {
@@ -110,9 +110,17 @@ class Predictor:
     overwrites (clone to keep).  Variables come from the process variable store under `scope`, so a
     network trained in this process predicts directly; `restore()` loads a checkpoint instead."""
 
-    def __init__(self, net="disp_net", H=224, W=224, batch=1, scope="model", fold_bn=True, graph=True, cin=None):
+    def __init__(self, net="disp_net", H=224, W=224, batch=1, scope="model", fold_bn=True, graph=True, cin=None,
+                 int8=False):
         """cin: input channels when not the net's usual count -- batch_prediction_optflow.py:43 feeds depth_net an
-        11-channel [I, I1, flow, I_warp] stack at 240x720."""
+        11-channel [I, I1, flow, I_warp] stack at 240x720.
+
+        int8: run every folded conv / deconv layer as a product of 8-bit integers (int8.Conv8: a scale per pixel and
+        per output channel; heads, resizes and activations between layers stay fp32).  Opt-in: outputs differ from the
+        fp32 network's by the 8-bit rounding of weights and activations."""
+        if int8 and not fold_bn:
+            raise ValueError("int8 prediction runs on the folded weights: fold_bn=True")
+        self.int8, self.conv8 = bool(int8), None
         if net not in NETS:
             raise ValueError(f"unknown net {net!r}: one of {sorted(NETS)}")
         net_scope, builder, cin0, kw, _ = NETS[net]
@@ -127,7 +135,7 @@ class Predictor:
         self.refresh()
 
     def _forward(self):
-        outs = self.prog.forward(self.run, self.x, is_training=False, fold_bn=self.fold)
+        outs = self.prog.forward(self.run, self.x, is_training=False, fold_bn=self.fold, conv8=self.conv8)
         if self.net == "depth_net":
             disps, pose_pred, masks = outs[:2], outs[2], outs[3:]
             outs = disps + [pose_ops.reduce_mean_hw(pose_pred).reshape(-1, 1, 6)] + masks   # :183-186
@@ -138,6 +146,8 @@ class Predictor:
         self.graph = None
         if self.fold:
             self.prog.fold_bn()
+        if self.int8:
+            self.conv8 = self._quantize_layers()
         s = _lib.owned_stream(self, "warmup")
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):               # warm-up: allocates every lazily created buffer
@@ -149,6 +159,18 @@ class Predictor:
                                                         capture_error_mode="thread_local"):
                 self.outs = self._forward()
             self.graph = g
+
+    def _quantize_layers(self):
+        """layer -> int8.Conv8 on the folded weights (a snapshot, as fold_bn)."""
+        out = {}
+        for op in self.prog.spec.ops:
+            if isinstance(op, ConvBN):
+                if op.bn:
+                    w, b, _ = self.prog._folded[op.layer]
+                else:
+                    w, b = self.prog.P(f"{op.layer}/weights"), self.prog.P(f"{op.layer}/biases")
+                out[op.layer] = int8_ops.Conv8(w, b, stride=op.s, relu=True, deconv=op.deconv)
+        return out
 
     def restore(self, save_path):
         """saver.restore(sess, checkpoint) (batch_prediction.py:55), then re-fold / re-capture."""

@@ -159,6 +159,10 @@ class Conv8:
             d.y_cstride = ocs
         return d
 
+    def rows(self, x):
+        """The Rows8 of an input (quantize_rows), for several layers that read it."""
+        return quantize_rows(x)
+
     def __call__(self, x, out=None):
         """x: fp32 [N, H, W, Cin] channel view (or its Rows8), or [M, Cin] rows for a 1x1 stride-1 conv.  Returns
         [N, OH, OW, Cout] ([M, Cout]), written into the channel view `out` if given."""

@@ -235,10 +235,16 @@ class NetRun:
     groups), and one backward call yields the sum of the calls' parameter gradients -- what TF computes for the
     shared variables."""
 
-    def __init__(self, prog, N, device="cuda", groups=1):
+    def __init__(self, prog, N, device="cuda", groups=1, tape8=False):
         if groups < 1 or N % groups:
             raise ValueError(f"batch {N} is not {groups} equal groups")
         self.prog, self.N, self.device, self.groups = prog, N, device, groups
+        self.tape8 = False
+        self.tape = {}          # op index -> (codes, scales) of an 8-bit tape (enable_tape8)
+        self.tape_ready = False
+        if tape8:
+            self._alloc_tape8()
+            return
         self.act = {}
         for b in prog.spec.bufs:
             shape = (N, b.H, b.W, b.cs)
@@ -251,10 +257,85 @@ class NetRun:
                 self.stats[i] = torch.empty((2, groups * op.K), device=device, dtype=torch.float32)
             elif isinstance(op, ConvBN):
                 self.z[i] = None
+        self._alloc_absmax()
+        self.grad = None
+
+    def _alloc_absmax(self):
         # per-op bound max|dz| of the BN backward's output (tde_bn_bwd dz_absmax), the gradient operand bound
         # of the conv backward in fp16x3 conv math (tde_conv_desc_t); zeroed at the start of every backward
-        self.absmax = torch.zeros((max(len(prog.spec.ops), 1), _lib.BOUND_SLOTS), device=device, dtype=torch.float32)
+        self.absmax = torch.zeros((max(len(self.prog.spec.ops), 1), _lib.BOUND_SLOTS), device=self.device,
+                                  dtype=torch.float32)
+
+    # ---- 8-bit tape (include/tde.h, "8-bit activations" (2))
+    def _alloc_tape8(self):
+        """Buffers of a run that keeps its training tape in 8 bits: its own input, outputs and head results in fp32, every
+        conv + BatchNorm + ReLU layer as codes + scales, the statistics; everything else -- pre-BN outputs, activations
+        and their gradients -- lies in ONE set per (program, batch) that all its 8-bit runs use in turn
+        (NetProgram.shared_tape8): the forward leaves nothing there that the backward needs, it restores the
+        activations from the tape first.  The runs of a program must therefore follow one another on one stream, as
+        calls that share its workspace do."""
+        spec, N = self.prog.spec, self.N
+        for op in spec.ops:
+            if isinstance(op, ConvBN) and (not op.bn or op.K % 4 or op.K > 1024):
+                raise ValueError(f"8-bit tape: layer {op.layer} needs BatchNorm over a multiple of 4 channels, at most "
+                                 "1024 (BN-free networks keep the fp32 tape)")
+        shared = self.prog.shared_tape8(N, self.device)
+        own = self.prog.own_buffers()
+        kept = getattr(self, "act", None) or {}
+        self.act = {}
+        for b in spec.bufs:
+            if b.name not in own:
+                self.act[b.name] = shared["act"][b.name]
+            elif b.name in kept:
+                self.act[b.name] = kept[b.name]
+            else:
+                make = torch.zeros if b.zero else torch.empty
+                self.act[b.name] = make((N, b.H, b.W, b.cs), device=self.device, dtype=torch.float32)
+        self.z, self.stats, self.tape = {}, {}, {}
+        for i, op in enumerate(spec.ops):
+            if isinstance(op, ConvBN):
+                shape = op.zshape(N)
+                self.z[i] = shared["z"][:int(np.prod(shape))].view(shape)
+                self.stats[i] = torch.empty((2, self.groups * op.K), device=self.device, dtype=torch.float32)
+                self.tape[i] = (torch.empty(shape, device=self.device, dtype=torch.int8),
+                                torch.empty(shape[:3] + ((op.K + 63) // 64,), device=self.device, dtype=torch.float32))
+        if not hasattr(self, "absmax"):
+            self._alloc_absmax()
+        grad = getattr(self, "grad", None)
         self.grad = None
+        if grad is not None:
+            self.ensure_tape8_grad(grad)
+        self.tape8, self.tape_ready = True, False
+
+    def enable_tape8(self):
+        """Keep this run's training tape in 8 bits from the next forward on; its input, output and output gradient
+        buffers stay where they are."""
+        if not self.tape8:
+            self._alloc_tape8()
+        return self
+
+    def ensure_tape8_grad(self, kept):
+        shared = self.prog.shared_tape8(self.N, self.device)
+        out = {v.buf.name for v in self.prog.spec.outputs}
+        self.grad = {}
+        for b in self.prog.spec.bufs:
+            if b.name not in out:
+                self.grad[b.name] = shared["grad"][b.name]
+            elif b.name in kept:
+                self.grad[b.name] = kept[b.name]
+            else:
+                self.grad[b.name] = torch.empty((self.N, b.H, b.W, b.cs), device=self.device, dtype=torch.float32)
+
+    def held_bytes(self):
+        """Bytes this run holds for itself between its forward and its backward (an 8-bit run's shared set is the
+        program's, not counted)."""
+        shared = set()
+        if self.tape8:
+            sh = self.prog.shared_tape8(self.N, self.device)
+            shared = {t.data_ptr() for k in ("act", "grad") for t in sh[k].values()} | {sh["z"].data_ptr()}
+        ts = list(self.act.values()) + [t for t in self.z.values() if t is not None] + list(self.stats.values())
+        ts += [t for pair in self.tape.values() for t in pair] + list((self.grad or {}).values()) + [self.absmax]
+        return sum(t.numel() * t.element_size() for t in ts if t.data_ptr() not in shared)
 
     def vptr(self, v, grad=False):
         t = (self.grad if grad else self.act)[v.buf.name]
@@ -268,7 +349,9 @@ class NetRun:
         return t[..., v.coff:v.coff + v.C]
 
     def ensure_grad(self):
-        if self.grad is None:
+        if self.grad is None and self.tape8:
+            self.ensure_tape8_grad({})
+        elif self.grad is None:
             self.grad = {b.name: torch.empty((self.N, b.H, b.W, b.cs), device=self.device, dtype=torch.float32)
                          for b in self.prog.spec.bufs}
         return self.grad
@@ -310,6 +393,7 @@ class NetProgram:
         self.bn_sync, self.bn_world = None, 1
         self._bn_sums = {}
         self._folded = None     # layer -> (weights with BN folded in, bias); see fold_bn()
+        self._tape8 = {}        # batch -> buffers shared by the runs with an 8-bit tape (shared_tape8)
         # filter-gradient overlap (enable_wgrad_overlap): side stream, its workspace per batch, dz ring
         # (every conv layer but the first of forward sends its filter gradient to the side stream, each behind one event,
         # and the heads' filter gradients join it; measured and removed in round 5: groups of 2-3 layers per wait,
@@ -326,6 +410,51 @@ class NetProgram:
         self.params_ready = None
         self.pre_backward = None    # called first thing in backward (before any gradient is written)
         self.timeline = None        # StepTimeline (diagnostic): a device stamp after every op, under capture only
+
+    def own_buffers(self):
+        """Names of the buffers a run with an 8-bit tape keeps to itself: its input, its outputs, the heads' results."""
+        return ({self.spec.input.name} | {v.buf.name for v in self.spec.outputs} |
+                {op.dst.buf.name for op in self.spec.ops if isinstance(op, Head)})
+
+    def shared_tape8(self, N, device="cuda"):
+        """The buffers all 8-bit-tape runs of this program at batch N work in: activations and gradients by buffer name,
+        and one pre-BN output of the largest layer."""
+        sh = self._tape8.get(N)
+        if sh is None:
+            own, out = self.own_buffers(), {v.buf.name for v in self.spec.outputs}
+
+            def new(b, zero=False):
+                return (torch.zeros if zero else torch.empty)((N, b.H, b.W, b.cs), device=device, dtype=torch.float32)
+            zn = max([int(np.prod(op.zshape(N))) for op in self.spec.ops if isinstance(op, ConvBN)] or [4])
+            sh = self._tape8[N] = {"act": {b.name: new(b, b.zero) for b in self.spec.bufs if b.name not in own},
+                                   "grad": {b.name: new(b) for b in self.spec.bufs if b.name not in out},
+                                   "z": torch.empty(zn, device=device, dtype=torch.float32)}
+        return sh
+
+    def _restore_tape8(self, run):
+        """The activations of run's forward into the shared buffers, in forward order: layer outputs from the tape,
+        resizes and copies from what is restored (or kept: head results) before them."""
+        lib, st, N = _lib.load(), _lib.stream_ptr(), run.N
+        for i, op in enumerate(self.spec.ops):
+            if isinstance(op, ConvBN):
+                codes, scales = run.tape[i]
+                _lib.check(lib.tde_tape8_restore(N * op.dst.H * op.dst.W, op.K, ptr(codes), ptr(scales), 1,
+                                                 run.vptr(op.dst), op.dst.buf.cs, op.dst.coff, st),
+                           op.layer + " tape restore")
+            elif isinstance(op, (Resize, Copy)):
+                self._place(run, op, st)
+
+    def _place(self, run, op, st):
+        """Forward of a Resize or Copy op."""
+        lib, N, s, t = _lib.load(), run.N, op.src, op.dst
+        if isinstance(op, Resize):
+            fn = lib.tde_resize_nearest_fwd if op.kind == "nearest" else lib.tde_resize_bilinear_fwd
+            with self._span("resize"):
+                _lib.check(fn(N, s.H, s.W, s.C, run.vptr(s), s.buf.cs, s.coff, t.H, t.W, run.vptr(t), t.buf.cs,
+                              t.coff, st), op.kind)
+        else:
+            _lib.check(lib.tde_copy_view(N * s.H * s.W, s.C, run.vptr(s), s.buf.cs, s.coff, run.vptr(t), t.buf.cs,
+                                         t.coff, 0, st), "copy")
 
     def _split_plan(self, N):
         """The convs whose forward or data-gradient call takes the halo-tiled path (their weights are kept as
@@ -516,7 +645,7 @@ class NetProgram:
                     ws = max(ws, qb(ctypes_ref(d)))
                     ws = max(ws, q(ctypes_ref(op.folded_desc(N)), 1 if op.deconv else 0))
                     M = N * op.dst.H * op.dst.W
-                    ws = max(ws, lib.tde_bn_workspace_size(M, op.K))
+                    ws = max(ws, lib.tde_bn_workspace_size(M, op.K), lib.tde_tape8_workspace_size(M, op.K))
                     dz = max(dz, M * op.K)
                 elif isinstance(op, Head):
                     ws = max(ws, lib.tde_head_workspace_size(ctypes_ref(op.desc(N))))
@@ -526,18 +655,23 @@ class NetProgram:
         return w.get(ws, dz, "cuda")
 
     # ---------------------------------------------------------------- forward
-    def forward(self, run, x, is_training=True, fold_bn=False):
+    def forward(self, run, x, is_training=True, fold_bn=False, conv8=None):
         """x: [N,H,W,cin] fp32 on the device.  Returns the output view tensors.  fold_bn (inference only):
-        run each conv/deconv + BN + ReLU as ONE bias+ReLU conv on the weights of fold_bn()."""
+        run each conv/deconv + BN + ReLU as ONE bias+ReLU conv on the weights of fold_bn().  conv8 (with fold_bn): a dict
+        layer -> int8.Conv8 that runs those layers in 8-bit integers instead."""
         main = torch.cuda.current_stream()
         try:
-            return self._forward(run, x, is_training, fold_bn)
+            return self._forward(run, x, is_training, fold_bn, conv8)
         finally:
             torch.cuda.set_stream(main)
 
-    def _forward(self, run, x, is_training, fold_bn):
+    def _forward(self, run, x, is_training, fold_bn, conv8):
         if fold_bn and (is_training or self._folded is None):
             raise ValueError("fold_bn needs is_training=False and weights folded by fold_bn()")
+        if conv8 is not None and not fold_bn:
+            raise ValueError("conv8 needs fold_bn")
+        run.tape_ready = False
+        rows8 = {}          # view -> its 8-bit rows: a view is complete before its first reader (static schedule)
         N = run.N
         lib = _lib.load()
         st = _lib.stream_ptr()
@@ -566,7 +700,14 @@ class NetProgram:
                 self.timer.tag = getattr(op, "layer", type(op).__name__)
             if self.pre_op is not None and isinstance(op, (ConvBN, Head)):
                 self.pre_op(self, i)
-            if isinstance(op, ConvBN):
+            if isinstance(op, ConvBN) and conv8 is not None:
+                key = (op.src.buf.name, op.src.coff, op.src.creal)
+                layer = conv8[op.layer]
+                if key not in rows8:
+                    rows8[key] = layer.rows(run.view_tensor(op.src)[..., :op.src.creal])
+                with self._span("conv_fwd", conv_flops(op, N), conv_bytes(op, N)):
+                    layer(rows8[key], out=run.view_tensor(op.dst))
+            elif isinstance(op, ConvBN):
                 if i in split_todo:
                     # one split launch for every pending layer whose weights are final by now (all of them
                     # unless an optimizer step is still running on a side stream)
@@ -600,6 +741,28 @@ class NetProgram:
                     with self._span("conv_fwd", conv_flops(op, N), conv_bytes(op, N)):
                         _lib.check(fn(ctypes_ref(fd), run.vptr(op.src), ptr(wf), ptr(bf), 1, run.vptr(op.dst), ptr(ws),
                                       wsb, st), op.layer)
+                elif is_training and run.tape8:
+                    # 8-bit tape: the conv leaves (sum z, sum z^2) per row group and z in the shared buffer, one apply
+                    # launch writes y, the statistics and the tape (with SyncBN: after the all-reduce of the sums)
+                    G = run.groups
+                    sums = self._sums(i, op.K, 0, G)
+                    bn = _lib.BnTrain(ptr(beta), 1e-3, op.decay, int(self.bessel), ptr(mm), ptr(mv), ptr(sm[0]),
+                                      ptr(sm[1]), run.vptr(op.dst), op.dst.buf.cs, op.dst.coff, 1, G, ptr(sums))
+                    fn = lib.tde_deconv2d_fwd_bn if op.deconv else lib.tde_conv2d_fwd_bn
+                    with self._span("conv_fwd", conv_flops(op, N), conv_bytes(op, N)):
+                        _lib.check(fn(ctypes_ref(d), run.vptr(op.src), ptr(w), ptr(z), ctypes_ref(bn), ptr(ws), wsb,
+                                      st), op.layer + " bn sums")
+                    world = 1
+                    if self.bn_sync is not None:
+                        self.bn_sync(sums)
+                        world = self.bn_world
+                    codes, scales = run.tape[i]
+                    with self._span("bn_fwd"):
+                        _lib.check(lib.tde_tape8_bn_fwd_from_sums(M, op.K, G, M // G * world, ptr(z), ptr(sums),
+                                                                  ptr(beta), 1e-3, op.decay, int(self.bessel), ptr(mm),
+                                                                  ptr(mv), ptr(sm[0]), ptr(sm[1]), run.vptr(op.dst),
+                                                                  op.dst.buf.cs, op.dst.coff, ptr(codes), ptr(scales),
+                                                                  st), op.layer + " bn tape")
                 elif is_training and self.bn_sync is not None:
                     # SyncBN: the conv writes its local (sum z, sum z^2) per row group from its own statistics
                     # partials, ONE all-reduce of all groups' sums, then one apply launch normalises each group over its
@@ -651,18 +814,11 @@ class NetProgram:
                     _lib.check(lib.tde_head_fwd(ctypes_ref(d), run.vptr(op.src), ptr(self.P(f"{op.layer}/weights")),
                                                 ptr(self.P(f"{op.layer}/biases")), run.vptr(op.dst), op.act, op.scale,
                                                 op.offset, st), op.layer)
-            elif isinstance(op, Resize):
-                s, t = op.src, op.dst
-                fn = lib.tde_resize_nearest_fwd if op.kind == "nearest" else lib.tde_resize_bilinear_fwd
-                with self._span("resize"):
-                    _lib.check(fn(N, s.H, s.W, s.C, run.vptr(s), s.buf.cs, s.coff, t.H, t.W, run.vptr(t), t.buf.cs,
-                                  t.coff, st), op.kind)
-            elif isinstance(op, Copy):
-                s, t = op.src, op.dst
-                _lib.check(lib.tde_copy_view(N * s.H * s.W, s.C, run.vptr(s), s.buf.cs, s.coff, run.vptr(t),
-                                             t.buf.cs, t.coff, 0, st), "copy")
+            elif isinstance(op, (Resize, Copy)):
+                self._place(run, op, st)
         if tl is not None and spec.ops:
             tl.mark(self.prefix, "F", spec.ops[-1])
+        run.tape_ready = run.tape8 and is_training
         return [run.view_tensor(v) for v in spec.outputs]
 
     # ---------------------------------------------------------------- backward
@@ -680,6 +836,8 @@ class NetProgram:
             torch.cuda.set_stream(main)
 
     def _backward(self, run, grad_outputs, need_input_grad, on_grads, grad_accumulate):
+        if run.tape8 and not run.tape_ready:
+            raise ValueError("8-bit tape: backward needs this run's training forward first")
         pacc = 1 if grad_accumulate else 0
         N = run.N
         if self.pre_backward is not None:
@@ -715,6 +873,8 @@ class NetProgram:
         ws, dz = self._scratch(N)
         wsb = ws.numel() * 4
         iv = spec.input_view
+        if run.tape8:
+            self._restore_tape8(run)
         _lib.check(lib.tde_zero_bytes(run.absmax.numel() * 4, ptr(run.absmax), st), "zero dz bounds")
         side = self.wgrad_stream if self._production() else None
         if side is SERIAL:
@@ -754,6 +914,29 @@ class NetProgram:
                                                          run.vptr(op.dst, True), op.dst.buf.cs, op.dst.coff, 1, ptr(dz),
                                                          ptr(self.G(f"{op.layer}/biases")), pacc, run.absmax_ptr(i),
                                                          ptr(ws), wsb, st), op.layer + " bias_relu_bwd")
+                elif run.tape8:
+                    beta = self.P(f"{op.layer}/BatchNorm/beta")
+                    gbeta = self.G(f"{op.layer}/BatchNorm/beta")
+                    codes, scales = run.tape[i]
+                    dy = run.vptr(op.dst, True)
+                    with self._span("bn_bwd"):
+                        if self.bn_sync is None:
+                            _lib.check(lib.tde_tape8_bn_bwd(M, op.K, run.groups, ptr(codes), ptr(scales), ptr(sm[1]),
+                                                            ptr(beta), dy, op.dst.buf.cs, op.dst.coff, ptr(dz),
+                                                            ptr(gbeta), pacc, run.absmax_ptr(i), ptr(ws), wsb, st),
+                                       op.layer + " tape bwd")
+                        else:
+                            G = run.groups
+                            ls, gs = self._sums(i, op.K, 1, G), self._sums(i, op.K, 2, G)
+                            _lib.check(lib.tde_tape8_bn_bwd_sums(M, op.K, G, ptr(codes), ptr(scales), ptr(beta), dy,
+                                                                 op.dst.buf.cs, op.dst.coff, ptr(gs), ptr(ls), ptr(ws),
+                                                                 wsb, st), op.layer + " tape sums")
+                            self.bn_sync(gs)
+                            _lib.check(lib.tde_tape8_bn_bwd_from_sums(M, op.K, G, M // G * self.bn_world, ptr(codes),
+                                                                      ptr(scales), ptr(sm[1]), ptr(beta), dy,
+                                                                      op.dst.buf.cs, op.dst.coff, ptr(gs), ptr(ls),
+                                                                      ptr(dz), ptr(gbeta), pacc, run.absmax_ptr(i), st),
+                                       op.layer + " tape syncbn bwd")
                 elif self.bn_sync is not None:
                     # SyncBN backward: local (sum g, sum g*xhat) per row group (one launch writes the copy to be
                     # all-reduced and the local one) -> all-reduce -> dz from the global means in one launch; dbeta

@@ -297,6 +297,18 @@ class Trainer:
         self.det_ws = Ls.det_workspace(self.N, self.H, self.W) if on else None
         return self
 
+    def enable_tape8(self):
+        """Keep the training tape in 8 bits (NetRun.enable_tape8, include/tde.h "8-bit activations"): each conv +
+        BatchNorm + ReLU layer leaves one byte per element for its backward instead of two fp32 tensors, and every run
+        of a program works in one shared set of activation and gradient buffers.  Losses and outputs are those of the
+        fp32 forward; gradients are the formulas' at the coded activations (each off by at most 1/256 of the largest of
+        its 64 channels).  Call before capture()."""
+        if self.graphs is not None or getattr(self, "ov_seq", None) is not None:
+            raise ValueError("enable_tape8 before capture(): the captured step holds the fp32 tape's buffers")
+        for run in getattr(self, "runs", {"": getattr(self, "run", None)}).values():
+            run.enable_tape8()
+        return self
+
     def enable_net_overlap(self, on=True):
         """Run the calls of one network program concurrently with those of the other on a second stream
         (config 4: `depth_net` on both pairs beside `disp_net` on both images, forward and backward; under capture
