@@ -25,8 +25,9 @@ __device__ __forceinline__ float q8_scale(unsigned amax_bits) {
   return amax_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(amax_bits) / 127.f;
 }
 
-// rne(127 x / a), exact: an fp32 quotient is off by at most one; the fp64 remainder 254 x - 2 q a (exact: 24-bit
-// factors) says which way, and breaks a tie to even.  a: finite maximum, |x| <= a.
+// rne(127 x / a), exact.  The fp32 estimate t = x * (127 / a) is off by less than 4e-5 (three roundings of at most 127),
+// so unless t lies that close to a half-integer its rounding is the quotient's.  Near one (1 element in 10^4) the fp64
+// remainder 254 x - 2 q a (exact: 24-bit factors) decides, and breaks a tie to even.  a: finite maximum, |x| <= a.
 struct Q8Div {
   double a;
   float inv;
@@ -41,14 +42,34 @@ __device__ __forceinline__ Q8Div q8_div(unsigned amax_bits) {
   if (d.mode == 1) d.inv = 127.f * __builtin_amdgcn_rcpf(a);
   return d;
 }
-__device__ __forceinline__ int q8_code(float x, const Q8Div& d) {
-  if (d.mode == 0) return 0;
+__device__ __noinline__ int q8_code_exact(float x, double a) {
   const double xd = 127.0 * (double)x;
-  int q = d.mode == 1 ? (int)rintf(x * d.inv) : (int)rint(xd / d.a);
-  const double r = 2.0 * fma(-(double)q, d.a, xd);
-  if (r > d.a || (r == d.a && (q & 1))) ++q;
-  if (r < -d.a || (r == -d.a && (q & 1))) --q;
+  int q = (int)rint(xd / a);
+  const double r = 2.0 * fma(-(double)q, a, xd);
+  if (r > a || (r == a && (q & 1))) ++q;
+  if (r < -a || (r == -a && (q & 1))) --q;
   return q;
+}
+// codes of four channels, packed
+__device__ __forceinline__ int q8_code4(const f4& x, const Q8Div& d) {
+  f4 q;
+  bool near = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float t = x[j] * d.inv;
+    q[j] = rintf(t);
+    near |= fabsf(fabsf(t - q[j]) - 0.5f) < 5e-5f;
+  }
+  int p = 0;
+  if (d.mode == 2 || (near && d.mode == 1)) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p |= (q8_code_exact(x[j], d.a) & 0xff) << (8 * j);
+    return p;
+  }
+  if (d.mode == 0) return 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) p |= ((int)q[j] & 0xff) << (8 * j);
+  return p;
 }
 
 // ---- rows: L lanes per row (a power of two <= 64), QPL quads of channels per lane held in registers; VEC: 16-byte loads
@@ -86,12 +107,7 @@ __global__ void __launch_bounds__(256) q8_rows_kernel(long rows, int C, int Cp, 
 #pragma unroll
   for (int i = 0; i < QPL; ++i) {
     const int c = 4 * (l + i * L);
-    if (c < Cp) {
-      int q = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) q |= (q8_code(v[i][j], d) & 0xff) << (8 * j);
-      *reinterpret_cast<int*>(codes + row * Cp + c) = q;
-    }
+    if (c < Cp) *reinterpret_cast<int*>(codes + row * Cp + c) = q8_code4(v[i], d);
   }
   if (l == 0) scales[row] = q8_scale(am);      // (row `rows`: no channel was read, scale 0)
 }
@@ -114,11 +130,14 @@ __global__ void __launch_bounds__(256) q8_weights_kernel(int taps, int cin, int 
   __syncthreads();
   am = max(max(sh[0], sh[1]), max(sh[2], sh[3]));
   const Q8Div d = q8_div(am);
-  for (int i = threadIdx.x; i < taps * Cp; i += 256) {
-    const int t = i / Cp, c = i - t * Cp;
-    float v = 0.f;
-    if (k < K && c < cin) v = layout == 0 ? w[((long)t * cin + c) * K + k] : w[((long)t * K + k) * cin + c];
-    codes[((long)t * Kp + k) * Cp + c] = (int8_t)q8_code(v, d);
+  for (int i = threadIdx.x; i < taps * Cp / 4; i += 256) {
+    const int t = 4 * i / Cp, c = 4 * i - t * Cp;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (k < K && c + j < cin)
+        v[j] = layout == 0 ? w[((long)t * cin + c + j) * K + k] : w[((long)t * K + k) * cin + c + j];
+    *reinterpret_cast<int*>(codes + ((long)t * Kp + k) * Cp + c) = q8_code4(v, d);
   }
   if (threadIdx.x == 0) scales[k] = q8_scale(am);
 }

@@ -6,8 +6,7 @@
 // Backward: g = dy [q >= 0], xhat = (q + 1/2) s - beta, dz = invstd (g - mean g - xhat mean(g xhat)).
 //
 // u is evaluated in fp64 because a code next to a step's border flips with the last bits of u: with fp64 the codes are
-// those of the definition.  The floor itself is exact too: an fp32 quotient is off by at most one, and
-// fma(-q, s, |u|) in fp64 tells which way.  fp64 FMAs run at the fp32 rate here, so the passes stay bound by memory.
+// those of the definition (tape_code4).  fp64 FMAs run at the fp32 rate here, so the passes stay bound by memory.
 //
 // Lanes: a row's block of 64 channels is one 16-lane DPP row, four channels per lane (narrower layers use 1-8 lanes per
 // row), so max|u| is four DPP moves, a row's z / dy is one 16-byte and its codes one 4-byte access per lane.
@@ -37,19 +36,37 @@ __device__ __forceinline__ unsigned group_umax(unsigned v) {
   return v;
 }
 
-// code of u under scale s (inv ~ 1 / s): the exact floor(|u| / s) clamped to 127, sign folded in
-__device__ __forceinline__ int tape_code(double u, float s, float inv) {
+// codes of four u under scale s, packed: the exact floor(|u| / s) clamped to 127, sign folded in.  The fp32 estimate
+// t = |u| / s is off by less than 4e-5 (three roundings of at most 128), so unless t lies that close to an integer its floor
+// is the quotient's; near one (1 element in 10^4; values past 127.5 are clamped anyway) the fp64 remainder decides.
+__device__ __noinline__ int tape_code_exact(double u, float s) {
   const double au = fabs(u);
-  int q = 0;
-  if (s >= 0x1p-100f) {
-    q = (int)fminf((float)au * inv, 127.f);
-    const double r = fma(-(double)q, (double)s, au);
-    q += r < 0.0 ? -1 : (r >= (double)s ? 1 : 0);
-    q = min(q, 127);
-  } else if (s > 0.f) {                      // 1 / s may not be an fp32 number
-    q = (int)fmin(floor(au / (double)s), 127.0);
-  }
+  int q = (int)fmin(floor(au / (double)s), 127.0);
+  const double r = fma(-(double)q, (double)s, au);
+  if (r < 0.0) --q;
+  if (r >= (double)s && q < 127) ++q;
   return u > 0.0 ? q : -1 - q;
+}
+__device__ __forceinline__ int tape_code4(const d4& u, const f4& uf, float s) {
+  const bool est = s >= 0x1p-100f, any = s > 0.f;      // (s NaN or 0: codes 0 / -1; below 2^-100 1 / s may overflow)
+  const float inv = est ? __builtin_amdgcn_rcpf(s) : 0.f;
+  int q[4], p = 0;
+  bool near = any && !est;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float t = fabsf(uf[j]) * inv;
+    const float fl = floorf(fminf(t, 127.f));
+    q[j] = est ? (int)fl : 0;
+    near |= est && t > 0.5f && t < 127.5f && fabsf(t - rintf(t)) < 5e-5f;
+  }
+  if (near) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) p |= (tape_code_exact(u[j], s) & 0xff) << (8 * j);
+    return p;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) p |= ((u[j] > 0.0 ? q[j] : -1 - q[j]) & 0xff) << (8 * j);
+  return p;
 }
 
 // scale of a block from the bits of max|u| (NaN and infinity order above every finite value)
@@ -66,16 +83,15 @@ __device__ __forceinline__ float tape_value(int packed, int j, float s) {
 template <int L>
 __device__ __forceinline__ void tape_row(const d4& u, f4& y, int& packed, float& s) {
   unsigned am = 0;
+  f4 uf;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    y[j] = (float)(u[j] < 0.0 ? 0.0 : u[j]);
-    am = max(am, __float_as_uint((float)u[j]) & 0x7fffffffu);
+    uf[j] = (float)u[j];
+    y[j] = uf[j] < 0.f ? 0.f : uf[j];
+    am = max(am, __float_as_uint(uf[j]) & 0x7fffffffu);
   }
   s = tape_scale(group_umax<L>(am));
-  const float inv = s >= 0x1p-100f ? __builtin_amdgcn_rcpf(s) : 0.f;
-  packed = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) packed |= (tape_code(u[j], s, inv) & 0xff) << (8 * j);
+  packed = tape_code4(u, uf, s);
 }
 
 struct TapeFwd {
@@ -272,14 +288,15 @@ __global__ void __launch_bounds__(256) tape_fwd_apply_kernel(const TapeFwd p, co
   }
 }
 
-constexpr int SMALL_RB = 8;        // rows a lane of the one-launch kernels holds
+constexpr int SMALL_NT = 512;      // threads of the one-launch kernels (1024 with 8 rows a lane spill: 18 us against 5)
+constexpr int SMALL_RB = 8;        // most rows a lane of theirs holds
 
-// Few rows (Mg <= SMALL_RB * 1024 / L): one block per 64-channel block keeps its columns of z in registers, so statistics,
+// Few rows (Mg <= SMALL_RB * SMALL_NT / L): one block per 64-channel block keeps its columns of z in registers, so statistics,
 // y and the tape are one launch and z is read once.
-template <int L>
-__global__ void __launch_bounds__(1024) tape_fwd_small_kernel(const TapeFwd p) {
-  constexpr int R = 1024 / L;
-  __shared__ double sh[16][L][8];
+template <int L, int RB>
+__global__ void __launch_bounds__(SMALL_NT) tape_fwd_small_kernel(const TapeFwd p) {
+  constexpr int R = SMALL_NT / L, NW = SMALL_NT / 64;
+  __shared__ double sh[NW][L][8];
   __shared__ double tot[L][8];
   const int tid = threadIdx.x, l = tid % L, rl = tid / L, b = blockIdx.x, lane = tid & 63, wv = tid >> 6;
   const int c = 64 * b + 4 * l;
@@ -294,15 +311,15 @@ __global__ void __launch_bounds__(1024) tape_fwd_small_kernel(const TapeFwd p) {
     }
   for (int g = 0; g < p.G; ++g) {
     const long base = (long)g * p.Mg;
-    f4 v[SMALL_RB];
+    f4 v[RB];
     d4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < SMALL_RB; ++i) {
+    for (int i = 0; i < RB; ++i) {
       const int r = rl + i * R;
       v[i] = on && r < p.Mg ? *reinterpret_cast<const f4*>(p.z + (base + r) * p.C + c) : f4{0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
-    for (int i = 0; i < SMALL_RB; ++i)
+    for (int i = 0; i < RB; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const double zd = (double)v[i][j];
@@ -323,7 +340,7 @@ __global__ void __launch_bounds__(1024) tape_fwd_small_kernel(const TapeFwd p) {
     if (tid < 8 * L) {
       double s = 0;
 #pragma unroll
-      for (int w = 0; w < 16; ++w) s += sh[w][tid >> 3][tid & 7];
+      for (int w = 0; w < NW; ++w) s += sh[w][tid >> 3][tid & 7];
       tot[tid >> 3][tid & 7] = s;
     }
     __syncthreads();
@@ -343,7 +360,7 @@ __global__ void __launch_bounds__(1024) tape_fwd_small_kernel(const TapeFwd p) {
         }
       }
 #pragma unroll
-    for (int i = 0; i < SMALL_RB; ++i) {
+    for (int i = 0; i < RB; ++i) {
       const int r = rl + i * R;
       if (r >= p.Mg) break;
       const long row = base + r;
@@ -469,10 +486,10 @@ __global__ void __launch_bounds__(256) tape_bwd_apply_kernel(const TapeBwd p, co
   block_absmax_to(mx, p.absmax);
 }
 
-template <int L>
-__global__ void __launch_bounds__(1024) tape_bwd_small_kernel(const TapeBwd p) {
-  constexpr int R = 1024 / L;
-  __shared__ double sh[16][L][8];
+template <int L, int RB>
+__global__ void __launch_bounds__(SMALL_NT) tape_bwd_small_kernel(const TapeBwd p) {
+  constexpr int R = SMALL_NT / L, NW = SMALL_NT / 64;
+  __shared__ double sh[NW][L][8];
   __shared__ double tot[L][8];
   const int tid = threadIdx.x, l = tid % L, rl = tid / L, b = blockIdx.x, lane = tid & 63, wv = tid >> 6;
   const int c = 64 * b + 4 * l;
@@ -487,12 +504,12 @@ __global__ void __launch_bounds__(1024) tape_bwd_small_kernel(const TapeBwd p) {
   }
   for (int g = 0; g < p.G; ++g) {
     const long base = (long)g * p.Mg;
-    f4 v[SMALL_RB];
-    int cd[SMALL_RB];
-    float sc[SMALL_RB];
+    f4 v[RB];
+    int cd[RB];
+    float sc[RB];
     d4 s0 = {0, 0, 0, 0}, s1 = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < SMALL_RB; ++i) {
+    for (int i = 0; i < RB; ++i) {
       const int r = rl + i * R;
       const long row = base + r;
       const bool ok = on && r < p.Mg;
@@ -501,7 +518,7 @@ __global__ void __launch_bounds__(1024) tape_bwd_small_kernel(const TapeBwd p) {
       sc[i] = ok ? p.scales[row * p.NB + b] : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < SMALL_RB; ++i) {
+    for (int i = 0; i < RB; ++i) {
       if (!on || rl + i * R >= p.Mg) break;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -525,7 +542,7 @@ __global__ void __launch_bounds__(1024) tape_bwd_small_kernel(const TapeBwd p) {
     if (tid < 8 * L) {
       double s = 0;
 #pragma unroll
-      for (int w = 0; w < 16; ++w) s += sh[w][tid >> 3][tid & 7];
+      for (int w = 0; w < NW; ++w) s += sh[w][tid >> 3][tid & 7];
       tot[tid >> 3][tid & 7] = s;
     }
     __syncthreads();
@@ -539,7 +556,7 @@ __global__ void __launch_bounds__(1024) tape_bwd_small_kernel(const TapeBwd p) {
       }
       const f4 is = *reinterpret_cast<const f4*>(p.save_invstd + (long)g * p.C + c);
 #pragma unroll
-      for (int i = 0; i < SMALL_RB; ++i) {
+      for (int i = 0; i < RB; ++i) {
         const int r = rl + i * R;
         if (r >= p.Mg) break;
         f4 o;
@@ -576,7 +593,7 @@ int tape_apply_rows(int M, int C, const TapePlan& t) {
   const long want = ((long)M + 2047) / 2048;
   return (int)(want > 8 * R ? want : 8 * R);
 }
-bool tape_small(int Mg, int L) { return Mg <= SMALL_RB * 1024 / L; }
+bool tape_small(int Mg, int L) { return Mg <= SMALL_RB * SMALL_NT / L; }
 
 #define TAPE_L(L, F)                 \
   switch (L) {                       \
@@ -651,7 +668,11 @@ int tde_tape8_bn_fwd(int M, int C, int groups, const float* z, const float* beta
   const TapeFwd p{M / groups, C, t.NB, groups, z, beta, (double)(M / groups), eps, decay, bessel, moving_mean, moving_var,
                   save_mean, save_invstd, y, y_cstride, y_coff, codes, scales};
   if (tape_small(p.Mg, t.L)) {
-#define F(LL) hipLaunchKernelGGL(tape_fwd_small_kernel<LL>, dim3(t.NB), dim3(1024), 0, st, p)
+#define F(LL)                                                                                                       \
+  if (p.Mg <= 2 * SMALL_NT / LL)                                                                                    \
+    hipLaunchKernelGGL((tape_fwd_small_kernel<LL, 2>), dim3(t.NB), dim3(SMALL_NT), 0, st, p);                       \
+  else                                                                                                              \
+    hipLaunchKernelGGL((tape_fwd_small_kernel<LL, SMALL_RB>), dim3(t.NB), dim3(SMALL_NT), 0, st, p)
     TAPE_L(t.L, F)
 #undef F
     return tde_launch_status();
@@ -738,7 +759,11 @@ int tde_tape8_bn_bwd(int M, int C, int groups, const int8_t* codes, const float*
   const TapeBwd p{M / groups, C, t.NB, groups, codes, scales, save_invstd, beta, dy, dy_cstride, dy_coff,
                   (double)(M / groups), dz, dbeta, dz_absmax, accumulate_dbeta};
   if (tape_small(p.Mg, t.L)) {
-#define F(LL) hipLaunchKernelGGL(tape_bwd_small_kernel<LL>, dim3(t.NB), dim3(1024), 0, st, p)
+#define F(LL)                                                                                                       \
+  if (p.Mg <= 2 * SMALL_NT / LL)                                                                                    \
+    hipLaunchKernelGGL((tape_bwd_small_kernel<LL, 2>), dim3(t.NB), dim3(SMALL_NT), 0, st, p);                       \
+  else                                                                                                              \
+    hipLaunchKernelGGL((tape_bwd_small_kernel<LL, SMALL_RB>), dim3(t.NB), dim3(SMALL_NT), 0, st, p)
     TAPE_L(t.L, F)
 #undef F
     return tde_launch_status();

@@ -17,11 +17,12 @@ The formulas stand in include/tde.h, "8-bit activations".
 """
 import contextlib
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
-from ._lib import ConvDesc, ptr
+from ._lib import ConvDesc
 from .program import same_pad
 
 BLOCK = 64            # TDE_TAPE8_BLOCK: channels of a row that share a tape scale
@@ -29,7 +30,7 @@ MAX_CHANNELS = 4096   # of a Conv8 input
 
 
 def _check(t, name, dtype=torch.float32):
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda:
         raise ValueError(f"{name} must be a {str(dtype).split('.')[-1]} tensor on the GPU")
     if t.device.index != torch.cuda.current_device():
         raise ValueError(f"{name} is on {t.device}, not on the current device (cuda:{torch.cuda.current_device()})")
@@ -39,11 +40,14 @@ def _check(t, name, dtype=torch.float32):
 
 def _rows(t, name):
     """(rows, C, pixel stride) of a [..., C] channel view: consecutive pixels a fixed stride apart."""
-    if t.dim() < 2:
-        raise ValueError(f"{name} must have at least two dimensions, got {tuple(t.shape)}")
-    C = t.shape[-1]
+    shape = t.shape
+    if len(shape) < 2:
+        raise ValueError(f"{name} must have at least two dimensions, got {tuple(shape)}")
+    C = shape[-1]
+    if C and t.is_contiguous():
+        return t.numel() // C, C, C
     rows, cs = 1, None
-    for n, s in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    for n, s in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
         if n != 1:
             if cs is None:
                 cs = s
@@ -56,24 +60,21 @@ def _rows(t, name):
     return rows, C, cs
 
 
-def _out(out, shape, like, name="out"):
+def _out(out, shape, device, name="out"):
     if out is None:
-        return torch.empty(shape, dtype=torch.float32, device=like.device)
+        return torch.empty(shape, dtype=torch.float32, device=device)
     _check(out, name)
-    if tuple(out.shape) != tuple(shape):
+    if out.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(out.shape)}")
     return out
 
 
+def _stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
 # ---------------------------------------------------------------- integer product
-class Rows8:
-    """Pixels as 8-bit codes [rows + 1, row_bytes(C)] with a scale each [rows + 1] (the last row is all zero: the
-    pixel outside the image); `shape` is the fp32 tensor's."""
-
-    def __init__(self, codes, scales, shape):
-        self.codes, self.scales, self.shape = codes, scales, tuple(shape)
-
-
+@functools.lru_cache(maxsize=None)
 def row_bytes(C):
     n = _lib.load().tde_q8_row_bytes(C)
     if n <= 0:
@@ -81,22 +82,46 @@ def row_bytes(C):
     return n
 
 
+class Rows8:
+    """Pixels as 8-bit codes with a scale each; `shape` is that of the fp32 tensor [..., C].  One row more than pixels:
+    the last is all zero (the pixel outside the image).  `codes` is [rows + 1, row_bytes(C)], `scales` [rows + 1]."""
+
+    def __init__(self, shape, device="cuda"):
+        self.C, self.rows = shape[-1], 1
+        for n in shape[:-1]:
+            self.rows *= n
+        self.row_bytes = row_bytes(self.C)
+        self._scales_at = (self.rows + 1) * self.row_bytes       # one buffer: scales behind the codes
+        self.buffer = torch.empty(self._scales_at + 4 * (self.rows + 1), dtype=torch.int8, device=device)
+        self.shape = tuple(shape)
+
+    @property
+    def codes(self):
+        return self.buffer[:self._scales_at].view(self.rows + 1, self.row_bytes)
+
+    @property
+    def scales(self):
+        return self.buffer[self._scales_at:].view(torch.float32)
+
+    def pointers(self):
+        p = self.buffer.data_ptr()
+        return p, p + self._scales_at
+
+
 def quantize_rows(x, out=None):
-    """fp32 [..., C] channel view -> Rows8.  out: a Rows8 to write into (a captured step's own buffers)."""
+    """fp32 [..., C] channel view -> Rows8.  out: a Rows8 of the same rows and channels to write into."""
     _check(x, "x")
     rows, C, cs = _rows(x, "x")
-    cp = row_bytes(C)
     if out is None:
-        out = Rows8(torch.empty((rows + 1, cp), dtype=torch.int8, device=x.device),
-                    torch.empty(rows + 1, dtype=torch.float32, device=x.device), x.shape)
+        out = Rows8(x.shape, x.device)
+    elif not isinstance(out, Rows8) or (out.rows, out.C) != (rows, C):
+        raise ValueError(f"out must be the Rows8 of {rows} rows of {C} channels")
     else:
-        if tuple(out.codes.shape) != (rows + 1, cp) or tuple(out.scales.shape) != (rows + 1,):
-            raise ValueError(f"out holds {tuple(out.codes.shape)} codes, x needs {(rows + 1, cp)}")
+        _check(out.buffer, "out", torch.int8)
         out.shape = tuple(x.shape)
     if rows:
-        lib = _lib.load()
-        _lib.check(lib.tde_q8_rows(rows, C, ptr(x), cs, 0, ptr(out.codes), ptr(out.scales), _lib.stream_ptr()),
-                   "quantize_rows")
+        codes, scales = out.pointers()
+        _lib.check(_lib.load().tde_q8_rows(rows, C, x.data_ptr(), cs, 0, codes, scales, _stream()), "quantize_rows")
     return out
 
 
@@ -132,8 +157,10 @@ class Conv8:
         self.codes = torch.empty(lib.tde_q8_weights_size(kh * kw, cin, K), dtype=torch.int8, device=w.device)
         self.scales = torch.empty((K + 15) // 16 * 16, dtype=torch.float32, device=w.device)
         self.bias = None if bias is None else bias.detach().clone().contiguous()
-        _lib.check(lib.tde_q8_weights(kh * kw, cin, K, 1 if self.deconv else 0, ptr(w), ptr(self.codes),
-                                      ptr(self.scales), _lib.stream_ptr()), "Conv8 weights")
+        self._geometry = functools.lru_cache(maxsize=64)(self._make_geometry)
+        self._desc = functools.lru_cache(maxsize=64)(self._make_desc)
+        _lib.check(lib.tde_q8_weights(kh * kw, cin, K, 1 if self.deconv else 0, w.data_ptr(), self.codes.data_ptr(),
+                                      self.scales.data_ptr(), _stream()), "Conv8 weights")
         return self
 
     def out_size(self, H, W):
@@ -141,8 +168,20 @@ class Conv8:
             return H * self.stride, W * self.stride
         return same_pad(H, self.kh, self.stride)[0], same_pad(W, self.kw, self.stride)[0]
 
-    def desc(self, N, H, W, ocs):
-        """The conv descriptor of a batch (a transposed conv's is that of its virtual forward conv)."""
+    def _make_geometry(self, shape):
+        """(N, H, W, output shape) of an input shape."""
+        if shape[-1] != self.cin:
+            raise ValueError(f"x has {shape[-1]} channels, the weights {self.cin}")
+        if len(shape) == 2 and (self.kh, self.kw, self.stride) == (1, 1, 1):
+            return 1, 1, shape[0], torch.Size((shape[0], self.K))
+        if len(shape) != 4:
+            raise ValueError(f"x must be [N, H, W, C], or [M, C] for a 1x1 stride-1 conv, got {shape}")
+        N, H, W = shape[:3]
+        return N, H, W, torch.Size((N,) + self.out_size(H, W) + (self.K,))
+
+    def _make_desc(self, N, H, W, ocs):
+        """The conv descriptor of a batch whose output has pixel stride ocs (a transposed conv's is that of its virtual
+        forward conv)."""
         OH, OW = self.out_size(H, W)
         d = ConvDesc()
         big, small = ((OH, OW), (H, W)) if self.deconv else ((H, W), (OH, OW))
@@ -151,40 +190,30 @@ class Conv8:
         d.w_cin = d.C
         d.KH, d.KW, d.stride = self.kh, self.kw, self.stride
         d.pad_top, d.pad_left = same_pad(d.H, self.kh, self.stride)[1], same_pad(d.W, self.kw, self.stride)[1]
-        d.x_cstride = d.C
-        d.y_cstride = d.K
-        if self.deconv:
-            d.x_cstride = ocs
-        else:
-            d.y_cstride = ocs
+        d.x_cstride, d.y_cstride = (ocs, d.K) if self.deconv else (d.C, ocs)
         return d
 
-    def rows(self, x):
-        """The Rows8 of an input (quantize_rows), for several layers that read it."""
-        return quantize_rows(x)
+    quantize = staticmethod(quantize_rows)      # the Rows8 of an input, for several layers that read it
 
     def __call__(self, x, out=None):
         """x: fp32 [N, H, W, Cin] channel view (or its Rows8), or [M, Cin] rows for a 1x1 stride-1 conv.  Returns
         [N, OH, OW, Cout] ([M, Cout]), written into the channel view `out` if given."""
-        x8 = x if isinstance(x, Rows8) else quantize_rows(x)
-        shape = x8.shape
-        if shape[-1] != self.cin:
-            raise ValueError(f"x has {shape[-1]} channels, the weights {self.cin}")
-        if len(shape) == 2 and (self.kh, self.kw, self.stride) == (1, 1, 1):
-            N, H, W = 1, 1, shape[0]
-        elif len(shape) == 4:
-            N, H, W = shape[:3]
+        if isinstance(x, Rows8):
+            N, H, W, oshape = self._geometry(x.shape)
+            _check(x.buffer, "x", torch.int8)
+            x8 = x
         else:
-            raise ValueError(f"x must be [N, H, W, C], or [M, C] for a 1x1 stride-1 conv, got {shape}")
-        OH, OW = self.out_size(H, W)
-        oshape = (W, self.K) if len(shape) == 2 else (N, OH, OW, self.K)
-        y = _out(out, oshape, x8.codes)
+            N, H, W, oshape = self._geometry(tuple(getattr(x, "shape", (0,))))
+            x8 = quantize_rows(x)
+        y = _out(out, oshape, x8.buffer.device)
         rows, _, ocs = _rows(y, "out")
         if rows:
+            xc, xs = x8.pointers()
             lib = _lib.load()
             fn = lib.tde_q8_deconv2d_bias_act if self.deconv else lib.tde_q8_conv2d_bias_act
-            _lib.check(fn(ctypes.byref(self.desc(N, H, W, ocs)), ptr(x8.codes), ptr(x8.scales), ptr(self.codes),
-                          ptr(self.scales), ptr(self.bias), int(self.relu), ptr(y), _lib.stream_ptr()), "Conv8")
+            _lib.check(fn(ctypes.byref(self._desc(N, H, W, ocs)), xc, xs, self.codes.data_ptr(), self.scales.data_ptr(),
+                          None if self.bias is None else self.bias.data_ptr(), self.relu, y.data_ptr(), _stream()),
+                       "Conv8")
         return y
 
 
@@ -206,19 +235,25 @@ class Tape8:
             raise ValueError(f"invstd must be [groups, {C}], got {tuple(invstd.shape)}")
         if not (codes.is_contiguous() and scales.is_contiguous() and invstd.is_contiguous()):
             raise ValueError("codes, scales and invstd must be contiguous")
-        self.codes, self.scales, self.invstd, self.mean = codes, scales, invstd, mean
-        self.C, self.rows, self.groups = C, codes.numel() // C, invstd.shape[0]
+        self._set(codes, scales, invstd, mean)
         _check_groups(self.rows, self.groups)
+
+    def _set(self, codes, scales, invstd, mean):
+        self.codes, self.scales, self.invstd, self.mean = codes, scales, invstd, mean
+        self.C = codes.shape[-1]
+        self.rows, self.groups = codes.numel() // self.C, invstd.shape[0]
+        return self
 
     def restore(self, relu=True, out=None):
         """The tape's values [..., C]: relu=True the layer's output as the consumers' filter gradients read it, relu=False
         the coded pre-activation."""
-        y = _out(out, self.codes.shape, self.codes)
+        _check(self.codes, "codes", torch.int8)
+        y = _out(out, self.codes.shape, self.codes.device)
         rows, _, cs = _rows(y, "out")
         _check_view(y, cs, "out")
         if rows:
-            _lib.check(_lib.load().tde_tape8_restore(rows, self.C, ptr(self.codes), ptr(self.scales), int(bool(relu)),
-                                                     ptr(y), cs, 0, _lib.stream_ptr()), "Tape8.restore")
+            _lib.check(_lib.load().tde_tape8_restore(rows, self.C, self.codes.data_ptr(), self.scales.data_ptr(),
+                                                     bool(relu), y.data_ptr(), cs, 0, _stream()), "Tape8.restore")
         return y
 
 
@@ -232,19 +267,17 @@ def _check_view(t, cs, name):
         raise ValueError(f"{name}: the channel view must start on 16 bytes with a pixel stride of a multiple of 4")
 
 
-def _channels(z, beta):
-    C = z.shape[-1]
+def _check_beta(C, beta):
     if C == 0 or C % 4 or C > 1024:
         raise ValueError(f"{C} channels: a multiple of 4 up to 1024 is expected")
     _check(beta, "beta")
-    if tuple(beta.shape) != (C,) or not beta.is_contiguous() or beta.data_ptr() % 16:
+    if beta.shape != (C,) or not beta.is_contiguous() or beta.data_ptr() % 16:
         raise ValueError(f"beta must be a contiguous ({C},) tensor that starts on 16 bytes")
-    return C
 
 
-def _workspace(rows, C, device):
-    nb = _lib.load().tde_tape8_workspace_size(rows, C)
-    return torch.empty(nb, dtype=torch.uint8, device=device), nb
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows, C):
+    return _lib.load().tde_tape8_workspace_size(rows, C)
 
 
 def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel=True, out=None):
@@ -253,8 +286,10 @@ def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel
     The rows are `groups` equal consecutive groups, each normalised over its own rows.  moving: (moving_mean,
     moving_variance), updated in place in group order.  out: a channel view for y (16-byte aligned)."""
     _check(z, "z")
-    C = _channels(z, beta)
-    if z.dim() < 2 or not z.is_contiguous() or z.data_ptr() % 16:
+    shape, dev = z.shape, z.device
+    C = shape[-1] if len(shape) >= 2 else 0
+    _check_beta(C, beta)
+    if not z.is_contiguous() or z.data_ptr() % 16:
         raise ValueError("z must be a contiguous [..., C] tensor that starts on 16 bytes")
     rows = z.numel() // C
     if rows == 0:
@@ -262,22 +297,24 @@ def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel
     _check_groups(rows, groups)
     mm = mv = None
     if moving is not None:
-        mm, mv = moving
-        for t in (mm, mv):
+        for t in moving:
             _check(t, "moving")
-            if tuple(t.shape) != (C,) or not t.is_contiguous():
+            if t.shape != (C,) or not t.is_contiguous():
                 raise ValueError(f"moving statistics must be contiguous ({C},) tensors")
-    y = _out(out, z.shape, z)
+        mm, mv = (t.data_ptr() for t in moving)
+    y = _out(out, shape, dev)
     _, _, cs = _rows(y, "out")
     _check_view(y, cs, "out")
-    codes = torch.empty(z.shape, dtype=torch.int8, device=z.device)
-    scales = torch.empty(tuple(z.shape[:-1]) + ((C + BLOCK - 1) // BLOCK,), dtype=torch.float32, device=z.device)
-    stats = torch.empty((2, groups, C), dtype=torch.float32, device=z.device)
-    ws, nb = _workspace(rows, C, z.device)
-    _lib.check(_lib.load().tde_tape8_bn_fwd(rows, C, groups, ptr(z), ptr(beta), eps, decay, int(bool(bessel)), ptr(mm),
-                                            ptr(mv), ptr(stats[0]), ptr(stats[1]), ptr(y), cs, 0, ptr(codes),
-                                            ptr(scales), ptr(ws), nb, _lib.stream_ptr()), "bn_relu_forward")
-    return y, Tape8(codes, scales, stats[1], stats[0])
+    codes = torch.empty(shape, dtype=torch.int8, device=dev)
+    scales = torch.empty(shape[:-1] + ((C + BLOCK - 1) // BLOCK,), dtype=torch.float32, device=dev)
+    mean, invstd = torch.empty((2, groups, C), dtype=torch.float32, device=dev).unbind()
+    nb = _workspace_bytes(rows, C)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    _lib.check(_lib.load().tde_tape8_bn_fwd(rows, C, groups, z.data_ptr(), beta.data_ptr(), eps, decay, bool(bessel), mm,
+                                            mv, mean.data_ptr(), invstd.data_ptr(), y.data_ptr(), cs, 0,
+                                            codes.data_ptr(), scales.data_ptr(), ws.data_ptr(), nb, _stream()),
+               "bn_relu_forward")
+    return y, Tape8.__new__(Tape8)._set(codes, scales, invstd, mean)
 
 
 def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
@@ -286,24 +323,28 @@ def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
     if not isinstance(tape, Tape8):
         raise ValueError("tape must be a Tape8")
     _check(dy, "dy")
-    C = _channels(dy, beta)
-    if tuple(dy.shape) != tuple(tape.codes.shape):
-        raise ValueError(f"dy must be {tuple(tape.codes.shape)}, got {tuple(dy.shape)}")
+    _check(tape.codes, "codes", torch.int8)
+    shape, dev, C = tape.codes.shape, dy.device, tape.C
+    _check_beta(C, beta)
+    if dy.shape != shape:
+        raise ValueError(f"dy must be {tuple(shape)}, got {tuple(dy.shape)}")
     rows, _, cs = _rows(dy, "dy")
     if rows == 0:
         raise ValueError("BatchNorm over no rows has no gradient")
     _check_view(dy, cs, "dy")
-    dz = _out(dz, dy.shape, dy, "dz")
+    dz = _out(dz, shape, dev, "dz")
     if not dz.is_contiguous() or dz.data_ptr() % 16:
         raise ValueError("dz must be contiguous and start on 16 bytes")
     acc = dbeta is not None
-    dbeta = _out(dbeta, (C,), dy, "dbeta")
+    dbeta = _out(dbeta, (C,), dev, "dbeta")
     if not dbeta.is_contiguous():
         raise ValueError("dbeta must be contiguous")
-    ws, nb = _workspace(rows, C, dy.device)
-    _lib.check(_lib.load().tde_tape8_bn_bwd(rows, C, tape.groups, ptr(tape.codes), ptr(tape.scales), ptr(tape.invstd),
-                                            ptr(beta), ptr(dy), cs, 0, ptr(dz), ptr(dbeta), int(acc), None, ptr(ws), nb,
-                                            _lib.stream_ptr()), "bn_relu_backward")
+    nb = _workspace_bytes(rows, C)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    _lib.check(_lib.load().tde_tape8_bn_bwd(rows, C, tape.groups, tape.codes.data_ptr(), tape.scales.data_ptr(),
+                                            tape.invstd.data_ptr(), beta.data_ptr(), dy.data_ptr(), cs, 0,
+                                            dz.data_ptr(), dbeta.data_ptr(), acc, None, ws.data_ptr(), nb, _stream()),
+               "bn_relu_backward")
     return dz, dbeta
 
 

@@ -704,7 +704,7 @@ class NetProgram:
                 key = (op.src.buf.name, op.src.coff, op.src.creal)
                 layer = conv8[op.layer]
                 if key not in rows8:
-                    rows8[key] = layer.rows(run.view_tensor(op.src)[..., :op.src.creal])
+                    rows8[key] = layer.quantize(run.view_tensor(op.src)[..., :op.src.creal])
                 with self._span("conv_fwd", conv_flops(op, N), conv_bytes(op, N)):
                     layer(rows8[key], out=run.view_tensor(op.dst))
             elif isinstance(op, ConvBN):
