@@ -301,7 +301,7 @@ int tde_q8_weights(int taps, int cin, int K, int layout, const float* w, int8_t*
  * weights.  NaN outputs stay NaN under relu.  `d` as for tde_conv2d_fwd_bias_act / tde_deconv2d_fwd_bias_act, except
  * that the input is the codes of tde_q8_rows on the layer's input pixels, so its view fields are not read (conv:
  * w_cin channels; deconv: K), and that K (conv) / C (deconv) and the output view need no alignment.  bias may be
- * NULL. */
+ * NULL.  At most 2^26 input and output pixels. */
 int tde_q8_conv2d_bias_act(const tde_conv_desc_t* d, const int8_t* x_codes, const float* x_scales,
                            const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y,
                            void* stream);
@@ -321,6 +321,8 @@ int tde_q8_deconv2d_bias_act(const tde_conv_desc_t* d, const int8_t* x_codes, co
  * Sums are fp64 in a fixed order: results do not change from run to run. */
 #define TDE_TAPE8_BLOCK 64
 size_t tde_tape8_workspace_size(int M, int C);
+/* 1: tde_tape8_bn_fwd / tde_tape8_bn_bwd on this shape are one launch that needs no workspace (ws may be NULL). */
+int tde_tape8_one_launch(int M, int C, int groups);
 /* z dense [M][C] -> y = relu(u) into its channel view, save_mean / save_invstd [groups][C], moving averages (both NULL:
  * no update) and the tape; semantics of tde_bn_fwd_train with relu = 1. */
 int tde_tape8_bn_fwd(int M, int C, int groups, const float* z, const float* beta, float eps, float decay, int bessel,

@@ -85,6 +85,18 @@ CONVS = [
     (1, 4, 5, 16, 8, 3, 3, True, True),
     (16, 40, 48, 32, 24, 3, 1, False, True),
     (16, 32, 48, 16, 130, 3, 1, False, True),
+    (1, 32, 48, 1024, 40, 7, 1, False, True),     # a patch filled in several channel chunks
+    (1, 33, 41, 600, 20, 5, 2, False, True),
+    (2, 20, 24, 320, 200, 3, 1, False, False),
+    (1, 16, 20, 700, 64, 7, 2, True, True),
+    (1, 200, 5, 64, 33, 3, 1, False, True),       # narrow maps: 8 and 4 pixel wide tiles
+    (3, 100, 3, 32, 40, 3, 1, False, True),
+    (64, 6, 6, 64, 64, 3, 1, False, True),
+    (300, 3, 4, 64, 48, 3, 1, False, True),       # many maps too small for a tile
+    (1, 1, 2100, 192, 300, 1, 1, False, True),    # the plain product, small and large tiles
+    (1, 1, 8200, 64, 1600, 1, 1, False, False),
+    (2, 50, 60, 128, 96, 1, 1, False, True),
+    (2, 50, 60, 128, 96, 1, 2, False, True),
 ]
 
 

@@ -114,7 +114,10 @@ def test_tape_arguments(p):
                dict(beta=None), dict(mm=p), dict(sm=None), dict(si=None), dict(y=None), dict(y=odd), dict(cs=6),
                dict(co=4), dict(co=-4), dict(codes=None), dict(codes=odd), dict(scales=None)):
         assert fwd(**kw) == -1, kw
-    assert fwd(nb=16) == -2 and fwd(ws=None) == -2 and fwd(ws=odd) == -2
+    # (few rows run as one launch that needs no workspace)
+    assert lib.tde_tape8_one_launch(8, 4, 1) == 1 and lib.tde_tape8_one_launch(1 << 20, 4, 2) == 0
+    assert lib.tde_tape8_one_launch(8, 4, 3) == 0
+    assert fwd(M=1 << 20, nb=16) == -2 and fwd(M=1 << 20, ws=None) == -2 and fwd(M=1 << 20, ws=odd) == -2
 
     def bwd(M=8, C=4, G=1, codes=p, scales=p, si=p, beta=p, dy=p, cs=4, co=0, dz=p, ws=p, nb=big):
         return lib.tde_tape8_bn_bwd(M, C, G, codes, scales, si, beta, dy, cs, co, dz, None, 0, None, ws, nb, None)
@@ -123,7 +126,7 @@ def test_tape_arguments(p):
                dict(beta=None), dict(beta=odd), dict(dy=None), dict(dy=odd), dict(cs=5), dict(co=8), dict(dz=None),
                dict(dz=odd)):
         assert bwd(**kw) == -1, kw
-    assert bwd(nb=16) == -2
+    assert bwd(M=1 << 20, nb=16) == -2
     assert lib.tde_tape8_restore(8, 4, p, p, 2, p, 4, 0, None) == -1
     assert lib.tde_tape8_restore(8, 4, p, p, 1, p, 4, 4, None) == -1
     assert lib.tde_tape8_bn_fwd_from_sums(8, 4, 2, 3, p, p, p, 1e-3, 0.99, 1, None, None, p, p, p, 4, 0, p, p, None) == -1

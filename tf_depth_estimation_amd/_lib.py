@@ -157,6 +157,7 @@ _SIGS = {
     "tde_q8_conv2d_bias_act": (c_int, [P, P, P, P, P, P, c_int, P, P]),
     "tde_q8_deconv2d_bias_act": (c_int, [P, P, P, P, P, P, c_int, P, P]),
     "tde_tape8_workspace_size": (c_size_t, [c_int, c_int]),
+    "tde_tape8_one_launch": (c_int, [c_int, c_int, c_int]),
     "tde_tape8_bn_fwd": (c_int, [c_int, c_int, c_int, P, P, c_float, c_float, c_int, P, P, P, P, P, c_int, c_int, P, P,
                                  P, c_size_t, P]),
     "tde_tape8_bn_fwd_from_sums": (c_int, [c_int, c_int, c_int, ctypes.c_long, P, P, P, c_float, c_float, c_int, P, P,
@@ -230,6 +231,12 @@ def ptr(t):
 
 def stream_ptr():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def raw_stream(device_index):
+    """Handle of the device's current stream as an integer (stream_ptr() without its Stream object: 0.1 us instead of 2.8
+    per call, where a call is a few microseconds)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 _hip = None

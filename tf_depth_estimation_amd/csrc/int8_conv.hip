@@ -10,8 +10,6 @@
 // tile, loaded by the lane that needs it, and the result leaves as one 16-byte store.
 #include "tde_common.h"
 
-#include <type_traits>
-
 namespace {
 
 typedef int i4 __attribute__((ext_vector_type(4)));
@@ -20,6 +18,7 @@ typedef int i4 __attribute__((ext_vector_type(4)));
 inline int q8_row(int C) { return C <= 32 ? 32 : (C + 63) / 64 * 64; }
 inline int q8_cols(int K) { return (K + 15) / 16 * 16; }
 constexpr int Q8_MAXC = 4096;
+constexpr long Q8_MAXPIX = 1 << 26;      // pixels of an input or output: a grid's threads stay below 2^32
 
 __device__ __forceinline__ float q8_scale(unsigned amax_bits) {
   return amax_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(amax_bits) / 127.f;
@@ -77,39 +76,39 @@ template <int L, int QPL, bool VEC>
 __global__ void __launch_bounds__(256) q8_rows_kernel(long rows, int C, int Cp, const float* x, long cs, int co,
                                                       int8_t* codes, float* scales) {
   const int l = threadIdx.x % L;
-  const long row = (long)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (row > rows) return;
-  const float* px = x + row * cs + co;
-  f4 v[QPL];
-  unsigned am = 0;
+  for (long row = (long)blockIdx.x * (256 / L) + threadIdx.x / L; row <= rows; row += (long)gridDim.x * (256 / L)) {
+    const float* px = x + row * cs + co;
+    f4 v[QPL];
+    unsigned am = 0;
 #pragma unroll
-  for (int i = 0; i < QPL; ++i) {
-    const int c = 4 * (l + i * L);
-    v[i] = f4{0.f, 0.f, 0.f, 0.f};
-    if (row < rows && c < C) {
-      if (VEC) {
-        v[i] = *reinterpret_cast<const f4*>(px + c);
+    for (int i = 0; i < QPL; ++i) {
+      const int c = 4 * (l + i * L);
+      v[i] = f4{0.f, 0.f, 0.f, 0.f};
+      if (row < rows && c < C) {
+        if (VEC) {
+          v[i] = *reinterpret_cast<const f4*>(px + c);
 #pragma unroll
-        for (int j = 1; j < 4; ++j)
-          if (c + j >= C) v[i][j] = 0.f;
-      } else {
+          for (int j = 1; j < 4; ++j)
+            if (c + j >= C) v[i][j] = 0.f;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (c + j < C) v[i][j] = px[c + j];
+          for (int j = 0; j < 4; ++j)
+            if (c + j < C) v[i][j] = px[c + j];
+        }
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) am = max(am, __float_as_uint(v[i][j]) & 0x7fffffffu);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) am = max(am, __float_as_uint(v[i][j]) & 0x7fffffffu);
-  }
+    for (int o = 1; o < L; o <<= 1) am = max(am, (unsigned)__shfl_xor((int)am, o, 64));
+    const Q8Div d = q8_div(am);
 #pragma unroll
-  for (int o = 1; o < L; o <<= 1) am = max(am, (unsigned)__shfl_xor((int)am, o, 64));
-  const Q8Div d = q8_div(am);
-#pragma unroll
-  for (int i = 0; i < QPL; ++i) {
-    const int c = 4 * (l + i * L);
-    if (c < Cp) *reinterpret_cast<int*>(codes + row * Cp + c) = q8_code4(v[i], d);
+    for (int i = 0; i < QPL; ++i) {
+      const int c = 4 * (l + i * L);
+      if (c < Cp) *reinterpret_cast<int*>(codes + row * Cp + c) = q8_code4(v[i], d);
+    }
+    if (l == 0) scales[row] = q8_scale(am);      // (row `rows`: no channel was read, scale 0)
   }
-  if (l == 0) scales[row] = q8_scale(am);      // (row `rows`: no channel was read, scale 0)
 }
 
 // ---- weights: one block per output channel (padding channels write zeros)
@@ -192,17 +191,39 @@ struct Q8Frag<32> {
   static __device__ __forceinline__ i4 mfma(T a, T b, i4 c) { return __builtin_amdgcn_mfma_i32_16x16x32_i8(a, b, c, 0, 0, 0); }
 };
 
-// WK waves split the (tap, channel chunk) steps of a tile of 16 TM channels x 16 TN pixels and add their fp32 sums through
-// LDS in wave order; WP groups of WK waves take neighbouring pixel tiles.  Fragments come straight from the caches:
-// a lane's 16 (8) bytes are its row's k-quarter, so a fragment is 16 segments of 64 (32) contiguous bytes.
-template <int TM, int TN, int KC, int WK, int WP>
-__global__ void __launch_bounds__(64 * WK * WP) q8_conv_kernel(const Q8Conv p) {
+// bias, scale, ReLU and store of one tile: four channels k.. of the pixel at py
+__device__ __forceinline__ void q8_store(const Q8Conv& p, float* py, int k, const f4& acc) {
+  if (k >= p.K) return;
+  const f4 ws = *reinterpret_cast<const f4*>(p.ws + k);       // (scales are padded to Kp)
+  f4 o;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float v = fmaf(acc[e], ws[e], p.bias && k + e < p.K ? p.bias[k + e] : 0.f);
+    o[e] = p.relu && v < 0.f ? 0.f : v;
+  }
+  if (p.vec && k + 3 < p.K) {
+    tde_st(reinterpret_cast<f4*>(py + k), o);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (k + e < p.K) py[k + e] = o[e];
+  }
+}
+__device__ __forceinline__ float* q8_out(const Q8Conv& p, const Q8Class& cl, int n, int i, int j) {
+  return p.y + (((long)n * p.OH + i * p.os + cl.py) * p.OW + j * p.os + cl.px) * p.ycs + p.yco;
+}
+
+// ---- few pixels: WK waves take turns at the (tap, channel chunk) steps of a tile of 16 TM channels x 16 TN pixels and
+// add their fp32 sums through LDS in wave order.  The time is the latency of the weights, so a wave has the fragments of U
+// steps in flight, straight from the caches (a lane's 16 / 8 bytes are its row's k-quarter), and every step is scaled by
+// itself.  (4x4x512 -> 512, one image: 7.2 us with one step in flight.)
+template <int TM, int TN, int KC, int WK, int U>
+__global__ void __launch_bounds__(64 * WK) q8_split_kernel(const Q8Conv p) {
   using F = typename Q8Frag<KC>::T;
-  __shared__ f4 red[WK > 1 ? WP * (WK - 1) * TM * TN * 64 : 1];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wk = wv % WK, wp = wv / WK;
-  const int r16 = lane & 15, kq = lane >> 4;
+  __shared__ f4 red[(WK - 1) * TM * TN * 64];
+  const int lane = threadIdx.x & 63, wk = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
   const Q8Class cl = q8_class(p, blockIdx.z);
-  const int m0 = (blockIdx.x * WP + wp) * 16 * TN, n0 = blockIdx.y * 16 * TM;
+  const int m0 = blockIdx.x * 16 * TN, n0 = blockIdx.y * 16 * TM;
   const long zero_row = (long)p.N * p.H * p.W;
 
   int iy[TN], ix[TN];
@@ -229,111 +250,356 @@ __global__ void __launch_bounds__(64 * WK * WP) q8_conv_kernel(const Q8Conv p) {
     for (int b = 0; b < TN; ++b) acc[a][b] = f4{0.f, 0.f, 0.f, 0.f};
 
   const int nch = p.Cp / KC, steps = cl.nty * cl.ntx * nch;
-  int s = (int)((long)steps * wk / WK);
-  const int s1 = (int)((long)steps * (wk + 1) / WK);
-  while (s < s1) {
-    const int t = s / nch, ch0 = s - t * nch, ch1 = min(nch, ch0 + s1 - s);
-    const int ty = t / cl.ntx, tx = t - ty * cl.ntx;
-    const long wtap = ((long)(cl.ky0 + p.kst * ty) * p.KW + cl.kx0 + p.kst * tx) * p.Kp * p.Cp;
-    const int8_t* xr[TN];
-    float xs[TN];
+  for (int s0 = wk; s0 < steps; s0 += WK * U) {
+    F fa[U][TM], fb[U][TN];
+    float xs[U][TN];
 #pragma unroll
-    for (int b = 0; b < TN; ++b) {
-      const int yy = iy[b] + p.dir * ty, xx = ix[b] + p.dir * tx;
-      const bool in = (unsigned)yy < (unsigned)p.H && (unsigned)xx < (unsigned)p.W;
-      const long pix = in ? pb[b] + (long)yy * p.W + xx : zero_row;
-      xr[b] = p.x + pix * p.Cp + kq * (KC / 4);
-      xs[b] = p.xs[pix];
+    for (int u = 0; u < U; ++u) {
+      const int sr = s0 + u * WK, s = min(sr, steps - 1);      // (a step past the end: a valid load, scale 0)
+      const int t = s / nch, ch = s - t * nch, ty = t / cl.ntx, tx = t - ty * cl.ntx;
+      const long wtap = ((long)(cl.ky0 + p.kst * ty) * p.KW + cl.kx0 + p.kst * tx) * p.Kp * p.Cp + ch * KC;
+#pragma unroll
+      for (int a = 0; a < TM; ++a) fa[u][a] = *reinterpret_cast<const F*>(wrow[a] + wtap);
+#pragma unroll
+      for (int b = 0; b < TN; ++b) {
+        const int yy = iy[b] + p.dir * ty, xx = ix[b] + p.dir * tx;
+        const bool in = (unsigned)yy < (unsigned)p.H && (unsigned)xx < (unsigned)p.W && sr < steps;
+        const long pix = in ? pb[b] + (long)yy * p.W + xx : zero_row;
+        fb[u][b] = *reinterpret_cast<const F*>(p.x + pix * p.Cp + kq * (KC / 4) + ch * KC);
+        xs[u][b] = p.xs[pix];
+      }
     }
-    i4 ia[TM][TN];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TN; ++b) {
+          const i4 ia = Q8Frag<KC>::mfma(fa[u][a], fb[u][b], i4{0, 0, 0, 0});
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[a][b][j] = fmaf((float)ia[j], xs[u][b], acc[a][b][j]);
+        }
+  }
+
+  if (wk > 0)
 #pragma unroll
     for (int a = 0; a < TM; ++a)
 #pragma unroll
-      for (int b = 0; b < TN; ++b) ia[a][b] = i4{0, 0, 0, 0};
-    for (int ch = ch0; ch < ch1; ++ch) {
-      F fa[TM], fb[TN];
-#pragma unroll
-      for (int a = 0; a < TM; ++a) fa[a] = *reinterpret_cast<const F*>(wrow[a] + wtap + ch * KC);
-#pragma unroll
-      for (int b = 0; b < TN; ++b) fb[b] = *reinterpret_cast<const F*>(xr[b] + ch * KC);
-#pragma unroll
-      for (int a = 0; a < TM; ++a)
-#pragma unroll
-        for (int b = 0; b < TN; ++b) ia[a][b] = Q8Frag<KC>::mfma(fa[a], fb[b], ia[a][b]);
-    }
+      for (int b = 0; b < TN; ++b) red[((wk - 1) * TM * TN + a * TN + b) * 64 + lane] = acc[a][b];
+  __syncthreads();
+  if (wk > 0) return;
+  for (int w = 0; w < WK - 1; ++w)
 #pragma unroll
     for (int a = 0; a < TM; ++a)
 #pragma unroll
-      for (int b = 0; b < TN; ++b)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[a][b][j] = fmaf((float)ia[a][b][j], xs[b], acc[a][b][j]);
-    s += ch1 - ch0;
-  }
-
-  if (WK > 1) {
-    f4* mine = red + wp * (WK - 1) * TM * TN * 64;
-    if (wk > 0)
-#pragma unroll
-      for (int a = 0; a < TM; ++a)
-#pragma unroll
-        for (int b = 0; b < TN; ++b) mine[((wk - 1) * TM * TN + a * TN + b) * 64 + lane] = acc[a][b];
-    __syncthreads();
-    if (wk > 0) return;
-    for (int w = 0; w < WK - 1; ++w)
-#pragma unroll
-      for (int a = 0; a < TM; ++a)
-#pragma unroll
-        for (int b = 0; b < TN; ++b) acc[a][b] += mine[(w * TM * TN + a * TN + b) * 64 + lane];
-  }
-
+      for (int b = 0; b < TN; ++b) acc[a][b] += red[(w * TM * TN + a * TN + b) * 64 + lane];
 #pragma unroll
   for (int b = 0; b < TN; ++b) {
     const int m = m0 + 16 * b + r16;
     if (m >= cl.M) continue;
     const int hw = cl.GH * cl.GW, n = m / hw, r = m - n * hw, i = r / cl.GW, j = r - i * cl.GW;
-    float* py = p.y + (((long)n * p.OH + i * p.os + cl.py) * p.OW + j * p.os + cl.px) * p.ycs + p.yco;
+    float* py = q8_out(p, cl, n, i, j);
+#pragma unroll
+    for (int a = 0; a < TM; ++a) q8_store(p, py, n0 + 16 * a + 4 * kq, acc[a][b]);
+  }
+}
+
+// ---- maps: a block computes 16 TM WC channels of a TH x TW tile of pixels (16 TN WP of them) of one image and class.  The
+// input pixels its taps reach lie in LDS as a patch of codes (`cb` bytes of channels at a time) and scales, zero outside
+// the image, so a tap is one uniform offset into it and needs no address or bounds arithmetic; the weights come from the
+// caches, one step ahead.  Rows are padded by a quarter fragment: 16 (8) bytes, so 8 (16) neighbouring pixels' fragments
+// lie in different banks.  What bounds it: a tap's conversion is 8 VALU instructions per 16x16 tile, 32 cycles, against 16
+// (8) cycles of the matrix unit per 64 (32) channels.
+struct Q8Tile {
+  int TW, tx, ty, cb;        // tile width, tiles per row and column of the class grid, channel bytes per patch fill
+};
+
+template <int TM, int TN, int KC, int WC, int WP>
+__global__ void __launch_bounds__(64 * WC * WP) q8_halo_kernel(const Q8Conv p, const Q8Tile tl) {
+  using F = typename Q8Frag<KC>::T;
+  constexpr int NT = 64 * WC * WP, BP = 16 * TN * WP, PADB = KC / 4;
+  extern __shared__ __attribute__((aligned(16))) char q8_lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, wc = wv % WC, wp = wv / WC;
+  const int r16 = lane & 15, kq = lane >> 4;
+  const Q8Class cl = q8_class(p, blockIdx.z);
+  const int per = tl.tx * tl.ty;
+  const int n = blockIdx.x / per, rem = blockIdx.x - n * per, tyi = rem / tl.tx, txi = rem - tyi * tl.tx;
+  const int TH = BP / tl.TW, i0 = tyi * TH, j0 = txi * tl.TW;
+  if (i0 >= cl.GH || j0 >= cl.GW) return;                   // (tiles are counted for the largest class)
+  const int n0 = (blockIdx.y * WC + wc) * 16 * TM;
+  const int PH = (TH - 1) * p.is + cl.nty, PW = (tl.TW - 1) * p.is + cl.ntx, NP = PH * PW;
+  const int back = p.dir < 0;
+  const int oy = i0 * p.is + cl.iy0 - (back ? cl.nty - 1 : 0), ox = j0 * p.is + cl.ix0 - (back ? cl.ntx - 1 : 0);
+  const int RB = tl.cb + PADB;                              // patch row bytes
+  float* const psc = reinterpret_cast<float*>(q8_lds);      // scales [NP], then codes
+  char* const pcd = q8_lds + ((NP * 4 + 15) & ~15);
+
+  int px[TN];                                               // this lane's pixels in the patch, at tap offset 0
+#pragma unroll
+  for (int b = 0; b < TN; ++b) {
+    const int q = 16 * (wp * TN + b) + r16, i = q / tl.TW, j = q - i * tl.TW;
+    px[b] = (i * PW + j) * p.is;
+  }
+  const int8_t* wrow[TM];
+#pragma unroll
+  for (int a = 0; a < TM; ++a) wrow[a] = p.w + (long)min(n0 + 16 * a + r16, p.Kp - 1) * p.Cp + kq * (KC / 4);
+
+  f4 acc[TM][TN];
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b) acc[a][b] = f4{0.f, 0.f, 0.f, 0.f};
+
+  const int taps = cl.nty * cl.ntx;
+  for (int c0 = 0; c0 < p.Cp && taps > 0; c0 += tl.cb) {
+    const int cbytes = min(tl.cb, p.Cp - c0), nq = cbytes / 16, total = NP * nq;
+    if (c0 > 0) __syncthreads();                            // the last fill's fragments have been read
+    for (int base = tid; base < total; base += 4 * NT) {
+      i4 v[4];
+      int dst[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int idx = base + u * NT;
+        v[u] = i4{0, 0, 0, 0};
+        dst[u] = -1;
+        if (idx < total) {
+          const int pp = idx / nq, c = idx - pp * nq, y = pp / PW, x = pp - y * PW, iy = oy + y, ix = ox + x;
+          dst[u] = pp * RB + 16 * c;
+          if ((unsigned)iy < (unsigned)p.H && (unsigned)ix < (unsigned)p.W) {
+            const long pix = ((long)n * p.H + iy) * p.W + ix;
+            v[u] = *reinterpret_cast<const i4*>(p.x + pix * p.Cp + c0 + 16 * c);
+            if (c0 == 0 && c == 0) psc[pp] = p.xs[pix];
+          } else if (c0 == 0 && c == 0) {
+            psc[pp] = 0.f;
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (dst[u] >= 0) {
+          if (KC == 64) {
+            *reinterpret_cast<i4*>(pcd + dst[u]) = v[u];
+          } else {                                          // (rows of 40 bytes: 8-byte aligned)
+            int2* d = reinterpret_cast<int2*>(pcd + dst[u]);
+            d[0] = int2{v[u][0], v[u][1]};
+            d[1] = int2{v[u][2], v[u][3]};
+          }
+        }
+    }
+    __syncthreads();
+
+    // steps (tap, chunk); the weights of the next step are loaded before this one's products
+    const int nch = cbytes / KC;
+    auto wofs = [&](int ty, int tx, int ch) __attribute__((always_inline)) {
+      return ((long)(cl.ky0 + p.kst * ty) * p.KW + cl.kx0 + p.kst * tx) * p.Kp * p.Cp + c0 + ch * KC;
+    };
+    F fa[TM], fn[TM];
+    {
+      const long o = wofs(0, 0, 0);
+#pragma unroll
+      for (int a = 0; a < TM; ++a) fa[a] = *reinterpret_cast<const F*>(wrow[a] + o);
+    }
+    for (int ty = 0; ty < cl.nty; ++ty)
+      for (int tx = 0; tx < cl.ntx; ++tx) {
+        const int toff = back ? (cl.nty - 1 - ty) * PW + (cl.ntx - 1 - tx) : ty * PW + tx;
+        float xs[TN];
+        i4 ia[TM][TN];
+#pragma unroll
+        for (int b = 0; b < TN; ++b) xs[b] = psc[px[b] + toff];
+#pragma unroll
+        for (int a = 0; a < TM; ++a)
+#pragma unroll
+          for (int b = 0; b < TN; ++b) ia[a][b] = i4{0, 0, 0, 0};
+        for (int ch = 0; ch < nch; ++ch) {
+          const bool lc = ch + 1 < nch, lx = tx + 1 < cl.ntx, ly = ty + 1 < cl.nty;
+          const long o = lc ? wofs(ty, tx, ch + 1) : (lx ? wofs(ty, tx + 1, 0) : wofs(ly ? ty + 1 : ty, 0, 0));
+#pragma unroll
+          for (int a = 0; a < TM; ++a) fn[a] = *reinterpret_cast<const F*>(wrow[a] + o);
+          F fb[TN];
+#pragma unroll
+          for (int b = 0; b < TN; ++b)
+            fb[b] = *reinterpret_cast<const F*>(pcd + (px[b] + toff) * RB + ch * KC + kq * (KC / 4));
+#pragma unroll
+          for (int a = 0; a < TM; ++a)
+#pragma unroll
+            for (int b = 0; b < TN; ++b) ia[a][b] = Q8Frag<KC>::mfma(fa[a], fb[b], ia[a][b]);
+#pragma unroll
+          for (int a = 0; a < TM; ++a) fa[a] = fn[a];
+        }
+#pragma unroll
+        for (int a = 0; a < TM; ++a)
+#pragma unroll
+          for (int b = 0; b < TN; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[a][b][j] = fmaf((float)ia[a][b][j], xs[b], acc[a][b][j]);
+      }
+  }
+
+#pragma unroll
+  for (int b = 0; b < TN; ++b) {
+    const int q = 16 * (wp * TN + b) + r16, i = i0 + q / tl.TW, j = j0 + q % tl.TW;
+    if (i >= cl.GH || j >= cl.GW) continue;
+    float* py = q8_out(p, cl, n, i, j);
+#pragma unroll
+    for (int a = 0; a < TM; ++a) q8_store(p, py, n0 + 16 * a + 4 * kq, acc[a][b]);
+  }
+}
+
+// ---- one tap, stride 1: the plain product of M tokens and K weight rows.  Both operands reach LDS by DMA
+// (global_load_lds_dwordx4: a wave instruction copies 16 rows of 64 bytes) into a ring of three slots, two steps in
+// flight across the barriers; the 16-byte quarters of a row are exchanged by (row >> 1) & 3 on the way, so that the
+// fragment reads of 8 neighbouring rows hit different banks.  All sums stay integers until the end.
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef __attribute__((address_space(1))) void* gbl_ptr_t;
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+template <int TM, int TN, int WC, int WP>
+__global__ void __launch_bounds__(64 * WC * WP) q8_gemm_kernel(const Q8Conv p, int M, int nct) {
+  constexpr int NW = WC * WP, BC = 16 * TM * WC, BP = 16 * TN * WP, NI = (BC + BP) / 16, DI = NI / NW;
+  static_assert(NI % NW == 0, "whole DMA instructions per wave");
+  constexpr int SLOT = (BC + BP) * 64;
+  extern __shared__ __attribute__((aligned(16))) char q8_lds[];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, wc = wv % WC, wp = wv / WC;
+  const int r16 = lane & 15, kq = lane >> 4;
+  const int lb = tde_xcd_block(blockIdx.x, gridDim.x), pt = lb / nct, ct = lb - pt * nct;
+  const int m0 = pt * BP, n0 = ct * BC;
+
+  const int8_t* src[DI];
+#pragma unroll
+  for (int j = 0; j < DI; ++j) {
+    const int row = (wv * DI + j) * 16 + (lane >> 2);
+    const int q = ((lane & 3) ^ ((row >> 1) & 3)) * 16;
+    src[j] = row < BC ? p.w + (long)min(n0 + row, p.Kp - 1) * p.Cp + q
+                      : p.x + (long)min(m0 + row - BC, M) * p.Cp + q;       // (row M of the codes is zero)
+  }
+  auto dma = [&](int s, int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < DI; ++j)
+      __builtin_amdgcn_global_load_lds((gbl_ptr_t)(src[j] + s * 64),
+                                       (lds_ptr_t)(q8_lds + slot * SLOT + (wv * DI + j) * 1024), 16, 0, 0);
+  };
+  i4 acc[TM][TN];
+#pragma unroll
+  for (int a = 0; a < TM; ++a)
+#pragma unroll
+    for (int b = 0; b < TN; ++b) acc[a][b] = i4{0, 0, 0, 0};
+
+  const int lofs = r16 * 64 + ((kq ^ ((r16 >> 1) & 3)) << 4);
+  const int steps = p.Cp / 64, last = steps - 1;
+  dma(0, 0);
+  dma(min(1, last), 1);
+  int slot = 0;
+  for (int s = 0; s < steps; ++s) {
+    vm_wait<DI>();        // this wave's part of step s has landed (step s + 1 may still fly)
+    lds_barrier();        // everybody's has, and everybody is done with the slot of step s - 1
+    dma(min(s + 2, last), slot == 0 ? 2 : slot - 1);
+    const char* base = q8_lds + slot * SLOT + lofs;
+    i4 fa[TM], fb[TN];
+#pragma unroll
+    for (int a = 0; a < TM; ++a) fa[a] = *reinterpret_cast<const i4*>(base + (wc * TM + a) * 1024);
+#pragma unroll
+    for (int b = 0; b < TN; ++b) fb[b] = *reinterpret_cast<const i4*>(base + BC * 64 + (wp * TN + b) * 1024);
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+      for (int b = 0; b < TN; ++b) acc[a][b] = Q8Frag<64>::mfma(fa[a], fb[b], acc[a][b]);
+    slot = slot == 2 ? 0 : slot + 1;
+  }
+  vm_wait<0>();           // no DMA may outlive the block's LDS
+
+#pragma unroll
+  for (int b = 0; b < TN; ++b) {
+    const int m = m0 + (wp * TN + b) * 16 + r16;
+    if (m >= M) continue;
+    const float xs = p.xs[m];
+    float* py = p.y + (long)m * p.ycs + p.yco;
 #pragma unroll
     for (int a = 0; a < TM; ++a) {
-      const int k = n0 + 16 * a + 4 * kq;
-      if (k >= p.K) continue;
-      const f4 ws = *reinterpret_cast<const f4*>(p.ws + k);       // (scales are padded to Kp)
-      f4 o;
+      f4 v;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = fmaf(acc[a][b][e], ws[e], p.bias && k + e < p.K ? p.bias[k + e] : 0.f);
-        o[e] = p.relu && v < 0.f ? 0.f : v;
-      }
-      if (p.vec && k + 3 < p.K) {
-        tde_st(reinterpret_cast<f4*>(py + k), o);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (k + e < p.K) py[k + e] = o[e];
-      }
+      for (int j = 0; j < 4; ++j) v[j] = (float)acc[a][b][j] * xs;
+      q8_store(p, py, n0 + (wc * TM + a) * 16 + 4 * kq, v);
     }
   }
 }
 
-template <int TM, int TN, int WK, int WP>
-void q8_launch(const Q8Conv& p, long Mmax, int classes, hipStream_t st) {
-  const dim3 grid(tde_cdiv(Mmax, 16 * TN * WP), tde_cdiv(p.K, 16 * TM), classes);
+// ---- launches
+template <int TM, int TN, int WK, int U>
+void q8_split_launch(const Q8Conv& p, long Mmax, int classes, hipStream_t st) {
+  const dim3 grid(tde_cdiv(Mmax, 16 * TN), tde_cdiv(p.K, 16 * TM), classes);
   if (p.Cp % 64 == 0)
-    hipLaunchKernelGGL((q8_conv_kernel<TM, TN, 64, WK, WP>), grid, dim3(64 * WK * WP), 0, st, p);
+    hipLaunchKernelGGL((q8_split_kernel<TM, TN, 64, WK, U>), grid, dim3(64 * WK), 0, st, p);
   else
-    hipLaunchKernelGGL((q8_conv_kernel<TM, TN, 32, WK, WP>), grid, dim3(64 * WK * WP), 0, st, p);
+    hipLaunchKernelGGL((q8_split_kernel<TM, TN, 32, WK, U>), grid, dim3(64 * WK), 0, st, p);
+}
+
+constexpr int Q8_LDS = 64 * 1024;      // patch bytes of a halo block: two blocks fit a CU's 160 KB
+
+// patch pixels of a TH x TW tile (the class with the most taps)
+inline int q8_patch(const Q8Conv& p, int TH, int TW) {
+  const int nty = p.deconv ? (p.KH + p.os - 1) / p.os : p.KH, ntx = p.deconv ? (p.KW + p.os - 1) / p.os : p.KW;
+  return ((TH - 1) * p.is + nty) * ((TW - 1) * p.is + ntx);
+}
+
+template <int TM, int TN, int WC, int WP>
+bool q8_halo_launch(const Q8Conv& p, int GH, int GW, int classes, hipStream_t st) {
+  constexpr int BP = 16 * TN * WP, BC = 16 * TM * WC;
+  Q8Tile t;
+  t.TW = GW > 8 ? 16 : (GW > 4 ? 8 : 4);
+  if (BP / t.TW < 1) return false;
+  const int TH = BP / t.TW, NP = q8_patch(p, TH, t.TW), kc = p.Cp % 64 == 0 ? 64 : 32;
+  t.tx = tde_cdiv(GW, t.TW); t.ty = tde_cdiv(GH, TH);
+  t.cb = (Q8_LDS - 4 * NP - 16) / NP - kc / 4;
+  t.cb = t.cb >= p.Cp ? p.Cp : t.cb / kc * kc;
+  if (t.cb < kc) return false;
+  const int lds = ((4 * NP + 15) & ~15) + NP * (t.cb + kc / 4);
+  const long blocks = (long)p.N * t.tx * t.ty;
+  if (blocks > 0x7fffffffL) return false;
+  const dim3 grid((unsigned)blocks, tde_cdiv(p.K, BC), classes);
+  if (kc == 64)
+    hipLaunchKernelGGL((q8_halo_kernel<TM, TN, 64, WC, WP>), grid, dim3(64 * WC * WP), lds, st, p, t);
+  else
+    hipLaunchKernelGGL((q8_halo_kernel<TM, TN, 32, WC, WP>), grid, dim3(64 * WC * WP), lds, st, p, t);
+  return true;
+}
+
+template <int TM, int TN, int WC, int WP>
+void q8_gemm_launch(const Q8Conv& p, int M, hipStream_t st) {
+  constexpr int BP = 16 * TN * WP, BC = 16 * TM * WC, LDS = 3 * (BC + BP) * 64;
+  if (LDS > 64 * 1024)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&q8_gemm_kernel<TM, TN, WC, WP>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  const int nct = tde_cdiv(p.K, BC);
+  hipLaunchKernelGGL((q8_gemm_kernel<TM, TN, WC, WP>), dim3((unsigned)((long)tde_cdiv(M, BP) * nct)), dim3(64 * WC * WP),
+                     LDS, st, p, M, nct);
 }
 
 int q8_conv(Q8Conv p, hipStream_t st) {
-  const int s = p.deconv ? p.os : 1;
-  const long Mmax = (long)p.N * ((p.OH + s - 1) / s) * ((p.OW + s - 1) / s);
-  if (Mmax > (1 << 30)) return TDE_ERR_UNSUPPORTED;
-  const int classes = s * s;
+  const int s = p.deconv ? p.os : 1, classes = s * s;
+  const int GH = (p.OH + s - 1) / s, GW = (p.OW + s - 1) / s;
+  const long Mmax = (long)p.N * GH * GW;
   const long tiles = ((Mmax + 15) / 16) * ((p.K + 15) / 16) * classes;      // 16 x 16 tiles
-  if (tiles <= 2048) q8_launch<1, 1, 16, 1>(p, Mmax, classes, st);
-  else if (tiles <= 16384) q8_launch<2, 2, 4, 1>(p, Mmax, classes, st);
-  else if (p.K <= 16) q8_launch<1, 4, 1, 4>(p, Mmax, classes, st);
-  else if (p.K <= 32) q8_launch<2, 4, 1, 4>(p, Mmax, classes, st);
-  else q8_launch<4, 4, 1, 4>(p, Mmax, classes, st);
+  if (p.KH == 1 && p.KW == 1 && p.is == 1 && p.os == 1 && p.OH == p.H && p.OW == p.W && p.Cp % 64 == 0 && tiles > 2048) {
+    const long big = (long)tde_cdiv(Mmax, 256) * tde_cdiv(p.K, 256);
+    if (big >= 192) q8_gemm_launch<8, 4, 2, 4>(p, (int)Mmax, st);
+    else q8_gemm_launch<4, 4, 2, 2>(p, (int)Mmax, st);
+    return tde_launch_status();
+  }
+  bool done = false;
+  if (GH * GW >= 32 && tiles > 1024) {
+    // pixels per block: 256 (128, 64 with more channels), halved while that leaves CUs without a block
+    const bool few = Mmax * classes * ((p.K + 127) / 128) < 256L * 256;
+    if (p.K <= 16) done = few ? q8_halo_launch<1, 2, 1, 4>(p, GH, GW, classes, st) : q8_halo_launch<1, 4, 1, 4>(p, GH, GW, classes, st);
+    else if (p.K <= 32) done = few ? q8_halo_launch<2, 2, 1, 4>(p, GH, GW, classes, st) : q8_halo_launch<2, 4, 1, 4>(p, GH, GW, classes, st);
+    else if (p.K <= 64) done = few ? q8_halo_launch<2, 2, 2, 2>(p, GH, GW, classes, st) : q8_halo_launch<2, 4, 2, 2>(p, GH, GW, classes, st);
+    else done = few ? q8_halo_launch<2, 2, 4, 1>(p, GH, GW, classes, st) : q8_halo_launch<2, 4, 4, 1>(p, GH, GW, classes, st);
+  }
+  if (!done) {
+    if (tiles <= 4096) q8_split_launch<1, 1, 16, 4>(p, Mmax, classes, st);
+    else q8_split_launch<2, 2, 4, 2>(p, Mmax, classes, st);
+  }
   return tde_launch_status();
 }
 
@@ -345,7 +611,7 @@ bool q8_args_ok(const tde_conv_desc_t* d, const int8_t* xc, const float* xs, con
       d->pad_top < 0 || d->pad_left < 0 || d->pad_top >= d->KH || d->pad_left >= d->KW)
     return false;
   if (cin <= 0 || cin > Q8_MAXC || cout <= 0 || cout > 65535 || d->KH > 64 || d->KW > 64 || d->stride > 64) return false;
-  if ((long)d->N * d->H * d->W > (1 << 30) || (long)d->N * d->OH * d->OW > (1 << 30)) return false;
+  if ((long)d->N * d->H * d->W > Q8_MAXPIX || (long)d->N * d->OH * d->OW > Q8_MAXPIX) return false;
   if (ocs <= 0 || oco < 0 || oco + cout > ocs) return false;
   return (relu == 0 || relu == 1) && tde_aligned16(xc) && tde_aligned16(wc) && tde_aligned16(ws) &&
          (reinterpret_cast<uintptr_t>(xs) & 3u) == 0 && (reinterpret_cast<uintptr_t>(y) & 3u) == 0;
@@ -366,7 +632,7 @@ int tde_q8_rows(int rows, int C, const float* x, int x_cstride, int x_coff, int8
   hipStream_t st = static_cast<hipStream_t>(stream);
 #define R(LL, QQ)                                                                                                     \
   do {                                                                                                                \
-    const dim3 grid(tde_cdiv((long)rows + 1, 256 / LL));                                                              \
+    const dim3 grid((unsigned)(tde_cdiv((long)rows + 1, 256 / LL) < (1 << 20) ? tde_cdiv((long)rows + 1, 256 / LL) : 1 << 20)); \
     if (vec)                                                                                                          \
       hipLaunchKernelGGL((q8_rows_kernel<LL, QQ, true>), grid, dim3(256), 0, st, (long)rows, C, Cp, x, (long)x_cstride, \
                          x_coff, codes, scales);                                                                      \

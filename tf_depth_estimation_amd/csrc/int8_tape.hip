@@ -655,6 +655,10 @@ size_t tde_tape8_workspace_size(int M, int C) {
   return tape_part_bytes(M, C) + (size_t)BN_MAX_GROUPS * 2 * C * sizeof(double);
 }
 
+int tde_tape8_one_launch(int M, int C, int groups) {
+  return tape_shape_ok(M, C, groups) && tape_small(M / groups, tape_lanes(C)) ? 1 : 0;
+}
+
 int tde_tape8_bn_fwd(int M, int C, int groups, const float* z, const float* beta, float eps, float decay, int bessel,
                      float* moving_mean, float* moving_var, float* save_mean, float* save_invstd, float* y,
                      int y_cstride, int y_coff, int8_t* codes, float* scales, void* ws, size_t ws_bytes, void* stream) {
@@ -662,7 +666,6 @@ int tde_tape8_bn_fwd(int M, int C, int groups, const float* z, const float* beta
   TDE_CHECK_ARG(tape_shape_ok(M, C, groups) && z && tde_aligned16(z) && beta && save_mean && save_invstd &&
                 tape_view_ok(y, C, y_cstride, y_coff) && tape_ok(codes, scales) &&
                 (moving_mean == nullptr) == (moving_var == nullptr));
-  if (ws_bytes < tde_tape8_workspace_size(M, C) || !ws || !tde_aligned16(ws)) return TDE_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const TapePlan t = tape_plan(M, C, groups);
   const TapeFwd p{M / groups, C, t.NB, groups, z, beta, (double)(M / groups), eps, decay, bessel, moving_mean, moving_var,
@@ -677,6 +680,7 @@ int tde_tape8_bn_fwd(int M, int C, int groups, const float* z, const float* beta
 #undef F
     return tde_launch_status();
   }
+  if (ws_bytes < tde_tape8_workspace_size(M, C) || !ws || !tde_aligned16(ws)) return TDE_ERR_WORKSPACE;
   double* part = reinterpret_cast<double*>(tde_ws_body(ws));
   double* sums = reinterpret_cast<double*>(tde_ws_body(ws) + tape_part_bytes(M, C));
   TapeSums s{};
@@ -753,7 +757,6 @@ int tde_tape8_bn_bwd(int M, int C, int groups, const int8_t* codes, const float*
   TDE_CHECK_ARG(tape_shape_ok(M, C, groups) && tape_ok(codes, scales) && save_invstd && beta &&
                 tde_aligned16(save_invstd) && tde_aligned16(beta) && tape_view_ok(dy, C, dy_cstride, dy_coff) && dz &&
                 tde_aligned16(dz));
-  if (ws_bytes < tde_tape8_workspace_size(M, C) || !ws || !tde_aligned16(ws)) return TDE_ERR_WORKSPACE;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const TapePlan t = tape_plan(M, C, groups);
   const TapeBwd p{M / groups, C, t.NB, groups, codes, scales, save_invstd, beta, dy, dy_cstride, dy_coff,
@@ -768,6 +771,7 @@ int tde_tape8_bn_bwd(int M, int C, int groups, const int8_t* codes, const float*
 #undef F
     return tde_launch_status();
   }
+  if (ws_bytes < tde_tape8_workspace_size(M, C) || !ws || !tde_aligned16(ws)) return TDE_ERR_WORKSPACE;
   double* part = reinterpret_cast<double*>(tde_ws_body(ws));
   double* sums = reinterpret_cast<double*>(tde_ws_body(ws) + tape_part_bytes(M, C));
   TapeSums s{};

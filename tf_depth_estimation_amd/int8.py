@@ -69,10 +69,6 @@ def _out(out, shape, device, name="out"):
     return out
 
 
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
-
-
 # ---------------------------------------------------------------- integer product
 @functools.lru_cache(maxsize=None)
 def row_bytes(C):
@@ -121,7 +117,8 @@ def quantize_rows(x, out=None):
         out.shape = tuple(x.shape)
     if rows:
         codes, scales = out.pointers()
-        _lib.check(_lib.load().tde_q8_rows(rows, C, x.data_ptr(), cs, 0, codes, scales, _stream()), "quantize_rows")
+        _lib.check(_lib.load().tde_q8_rows(rows, C, x.data_ptr(), cs, 0, codes, scales,
+                                           _lib.raw_stream(x.get_device())), "quantize_rows")
     return out
 
 
@@ -160,7 +157,7 @@ class Conv8:
         self._geometry = functools.lru_cache(maxsize=64)(self._make_geometry)
         self._desc = functools.lru_cache(maxsize=64)(self._make_desc)
         _lib.check(lib.tde_q8_weights(kh * kw, cin, K, 1 if self.deconv else 0, w.data_ptr(), self.codes.data_ptr(),
-                                      self.scales.data_ptr(), _stream()), "Conv8 weights")
+                                      self.scales.data_ptr(), _lib.raw_stream(w.get_device())), "Conv8 weights")
         return self
 
     def out_size(self, H, W):
@@ -212,8 +209,8 @@ class Conv8:
             lib = _lib.load()
             fn = lib.tde_q8_deconv2d_bias_act if self.deconv else lib.tde_q8_conv2d_bias_act
             _lib.check(fn(ctypes.byref(self._desc(N, H, W, ocs)), xc, xs, self.codes.data_ptr(), self.scales.data_ptr(),
-                          None if self.bias is None else self.bias.data_ptr(), self.relu, y.data_ptr(), _stream()),
-                       "Conv8")
+                          None if self.bias is None else self.bias.data_ptr(), self.relu, y.data_ptr(),
+                          _lib.raw_stream(y.get_device())), "Conv8")
         return y
 
 
@@ -235,25 +232,52 @@ class Tape8:
             raise ValueError(f"invstd must be [groups, {C}], got {tuple(invstd.shape)}")
         if not (codes.is_contiguous() and scales.is_contiguous() and invstd.is_contiguous()):
             raise ValueError("codes, scales and invstd must be contiguous")
-        self._set(codes, scales, invstd, mean)
+        if any(t.data_ptr() % 16 for t in (codes, scales, invstd)):
+            raise ValueError("codes, scales and invstd must start on 16 bytes")
+        self.shape, self.C, self.rows, self.groups = codes.shape, C, codes.numel() // C, invstd.shape[0]
         _check_groups(self.rows, self.groups)
+        self._buffer, self._views = codes, (codes, scales, invstd, mean)
+        self._ptrs = (codes.data_ptr(), scales.data_ptr(), invstd.data_ptr())
 
-    def _set(self, codes, scales, invstd, mean):
-        self.codes, self.scales, self.invstd, self.mean = codes, scales, invstd, mean
-        self.C = codes.shape[-1]
-        self.rows, self.groups = codes.numel() // self.C, invstd.shape[0]
-        return self
+    @classmethod
+    def _empty(cls, shape, C, rows, groups, device):
+        """The tape of a forward, in one buffer: codes, scales, invstd and mean behind one another, 16 bytes aligned."""
+        t = cls.__new__(cls)
+        t.shape, t.C, t.rows, t.groups = shape, C, rows, groups
+        s = (rows * C + 15) // 16 * 16
+        i = s + (rows * ((C + BLOCK - 1) // BLOCK) * 4 + 15) // 16 * 16
+        m = i + 4 * groups * C
+        t._buffer, t._views = torch.empty(m + 4 * groups * C, dtype=torch.int8, device=device), None
+        p = t._buffer.data_ptr()
+        t._ptrs, t._mean_ptr, t._at = (p, p + s, p + i), p + m, (s, i, m)
+        return t
+
+    def _view(self, k):
+        if self._views is None:
+            b, (s, i, m), nb, gc = self._buffer, self._at, (self.C + BLOCK - 1) // BLOCK, 4 * self.groups * self.C
+            self._views = (b[:self.rows * self.C].view(self.shape),
+                           b[s:s + 4 * self.rows * nb].view(torch.float32).view(self.shape[:-1] + (nb,)),
+                           b[i:i + gc].view(torch.float32).view(self.groups, self.C),
+                           b[m:m + gc].view(torch.float32).view(self.groups, self.C))
+        return self._views[k]
+
+    codes = property(lambda self: self._view(0))
+    scales = property(lambda self: self._view(1))
+    invstd = property(lambda self: self._view(2))
+    mean = property(lambda self: self._view(3))
 
     def restore(self, relu=True, out=None):
         """The tape's values [..., C]: relu=True the layer's output as the consumers' filter gradients read it, relu=False
         the coded pre-activation."""
-        _check(self.codes, "codes", torch.int8)
-        y = _out(out, self.codes.shape, self.codes.device)
+        _check(self._buffer, "codes", torch.int8)
+        dev = self._buffer.device
+        y = _out(out, self.shape, dev)
         rows, _, cs = _rows(y, "out")
         _check_view(y, cs, "out")
         if rows:
-            _lib.check(_lib.load().tde_tape8_restore(rows, self.C, self.codes.data_ptr(), self.scales.data_ptr(),
-                                                     bool(relu), y.data_ptr(), cs, 0, _stream()), "Tape8.restore")
+            codes, scales, _ = self._ptrs
+            _lib.check(_lib.load().tde_tape8_restore(rows, self.C, codes, scales, bool(relu), y.data_ptr(), cs, 0,
+                                                     _lib.raw_stream(dev.index)), "Tape8.restore")
         return y
 
 
@@ -276,8 +300,18 @@ def _check_beta(C, beta):
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(rows, C):
-    return _lib.load().tde_tape8_workspace_size(rows, C)
+def _workspace_bytes(rows, C, groups):
+    lib = _lib.load()
+    return 0 if lib.tde_tape8_one_launch(rows, C, groups) else lib.tde_tape8_workspace_size(rows, C)
+
+
+def _workspace(rows, C, groups, device):
+    """(keeper, pointer, bytes) of the call's workspace."""
+    nb = _workspace_bytes(rows, C, groups)
+    if nb == 0:
+        return None, None, 0
+    ws = torch.empty(nb, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), nb
 
 
 def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel=True, out=None):
@@ -305,16 +339,13 @@ def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel
     y = _out(out, shape, dev)
     _, _, cs = _rows(y, "out")
     _check_view(y, cs, "out")
-    codes = torch.empty(shape, dtype=torch.int8, device=dev)
-    scales = torch.empty(shape[:-1] + ((C + BLOCK - 1) // BLOCK,), dtype=torch.float32, device=dev)
-    mean, invstd = torch.empty((2, groups, C), dtype=torch.float32, device=dev).unbind()
-    nb = _workspace_bytes(rows, C)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    tape = Tape8._empty(shape, C, rows, groups, dev)
+    codes, scales, invstd = tape._ptrs
+    keep, ws, nb = _workspace(rows, C, groups, dev)
     _lib.check(_lib.load().tde_tape8_bn_fwd(rows, C, groups, z.data_ptr(), beta.data_ptr(), eps, decay, bool(bessel), mm,
-                                            mv, mean.data_ptr(), invstd.data_ptr(), y.data_ptr(), cs, 0,
-                                            codes.data_ptr(), scales.data_ptr(), ws.data_ptr(), nb, _stream()),
-               "bn_relu_forward")
-    return y, Tape8.__new__(Tape8)._set(codes, scales, invstd, mean)
+                                            mv, tape._mean_ptr, invstd, y.data_ptr(), cs, 0, codes, scales, ws, nb,
+                                            _lib.raw_stream(dev.index)), "bn_relu_forward")
+    return y, tape
 
 
 def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
@@ -323,8 +354,8 @@ def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
     if not isinstance(tape, Tape8):
         raise ValueError("tape must be a Tape8")
     _check(dy, "dy")
-    _check(tape.codes, "codes", torch.int8)
-    shape, dev, C = tape.codes.shape, dy.device, tape.C
+    _check(tape._buffer, "codes", torch.int8)
+    shape, dev, C = tape.shape, dy.device, tape.C
     _check_beta(C, beta)
     if dy.shape != shape:
         raise ValueError(f"dy must be {tuple(shape)}, got {tuple(dy.shape)}")
@@ -339,12 +370,11 @@ def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
     dbeta = _out(dbeta, (C,), dev, "dbeta")
     if not dbeta.is_contiguous():
         raise ValueError("dbeta must be contiguous")
-    nb = _workspace_bytes(rows, C)
-    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-    _lib.check(_lib.load().tde_tape8_bn_bwd(rows, C, tape.groups, tape.codes.data_ptr(), tape.scales.data_ptr(),
-                                            tape.invstd.data_ptr(), beta.data_ptr(), dy.data_ptr(), cs, 0,
-                                            dz.data_ptr(), dbeta.data_ptr(), acc, None, ws.data_ptr(), nb, _stream()),
-               "bn_relu_backward")
+    keep, ws, nb = _workspace(rows, C, tape.groups, dev)
+    codes, scales, invstd = tape._ptrs
+    _lib.check(_lib.load().tde_tape8_bn_bwd(rows, C, tape.groups, codes, scales, invstd, beta.data_ptr(), dy.data_ptr(),
+                                            cs, 0, dz.data_ptr(), dbeta.data_ptr(), acc, None, ws, nb,
+                                            _lib.raw_stream(dev.index)), "bn_relu_backward")
     return dz, dbeta
 
 
