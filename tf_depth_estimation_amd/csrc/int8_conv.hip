@@ -305,21 +305,25 @@ __global__ void __launch_bounds__(64 * WK) q8_split_kernel(const Q8Conv p) {
 }
 
 // ---- maps: a block computes 16 TM WC channels of a TH x TW tile of pixels (16 TN WP of them) of one image and class.  The
-// input pixels its taps reach lie in LDS as a patch of codes (`cb` bytes of channels at a time) and scales, zero outside
-// the image, so a tap is one uniform offset into it and needs no address or bounds arithmetic; the weights come from the
-// caches, one step ahead.  Rows are padded by a quarter fragment: 16 (8) bytes, so 8 (16) neighbouring pixels' fragments
-// lie in different banks.  What bounds it: a tap's conversion is 8 VALU instructions per 16x16 tile, 32 cycles, against 16
-// (8) cycles of the matrix unit per 64 (32) channels.
+// input pixels its taps reach lie in LDS as a patch of rows [scale | codes] (`cb` bytes of channels at a time), zero
+// outside the image, so a tap is one uniform offset into it and needs no address or bounds arithmetic; the weights come
+// from the caches, two steps (tap, channel chunk) ahead.  The scale's 16 (8) bytes also pad the rows, so that the
+// fragments of 8 (16) neighbouring pixels lie in different banks.  WK groups of waves split the steps where there are few
+// tiles, and add their sums through LDS in order.  ONE: a tap is one step (the usual case of few channels), no loop.
+// What bounds it there: a tap's conversion is 8 VALU instructions per 16x16 tile, 32 cycles, against 16 (8) cycles of the
+// matrix unit.  (The second launch bound keeps the products out of the accumulator file: with it, 2 moves per result and
+// step cost more than the products.)
 struct Q8Tile {
   int TW, tx, ty, cb;        // tile width, tiles per row and column of the class grid, channel bytes per patch fill
 };
 
-template <int TM, int TN, int KC, int WC, int WP>
-__global__ void __launch_bounds__(64 * WC * WP) q8_halo_kernel(const Q8Conv p, const Q8Tile tl) {
+template <int TM, int TN, int KC, bool ONE, int WC, int WP, int WK>
+__global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8Conv p, const Q8Tile tl) {
   using F = typename Q8Frag<KC>::T;
-  constexpr int NT = 64 * WC * WP, BP = 16 * TN * WP, PADB = KC / 4;
+  constexpr int NT = 64 * WC * WP * WK, BP = 16 * TN * WP, HEAD = KC / 4;
   extern __shared__ __attribute__((aligned(16))) char q8_lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, wc = wv % WC, wp = wv / WC;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wc = wv % WC, wp = wv / WC % WP, wk = wv / (WC * WP);
   const int r16 = lane & 15, kq = lane >> 4;
   const Q8Class cl = q8_class(p, blockIdx.z);
   const int per = tl.tx * tl.ty;
@@ -330,19 +334,20 @@ __global__ void __launch_bounds__(64 * WC * WP) q8_halo_kernel(const Q8Conv p, c
   const int PH = (TH - 1) * p.is + cl.nty, PW = (tl.TW - 1) * p.is + cl.ntx, NP = PH * PW;
   const int back = p.dir < 0;
   const int oy = i0 * p.is + cl.iy0 - (back ? cl.nty - 1 : 0), ox = j0 * p.is + cl.ix0 - (back ? cl.ntx - 1 : 0);
-  const int RB = tl.cb + PADB;                              // patch row bytes
-  float* const psc = reinterpret_cast<float*>(q8_lds);      // scales [NP], then codes
-  char* const pcd = q8_lds + ((NP * 4 + 15) & ~15);
+  const int RB = tl.cb + HEAD;                              // bytes of a patch row
 
-  int px[TN];                                               // this lane's pixels in the patch, at tap offset 0
+  int prow[TN];                                             // this lane's pixels in the patch (bytes), at tap offset 0
 #pragma unroll
   for (int b = 0; b < TN; ++b) {
     const int q = 16 * (wp * TN + b) + r16, i = q / tl.TW, j = q - i * tl.TW;
-    px[b] = (i * PW + j) * p.is;
+    prow[b] = (i * PW + j) * p.is * RB;
   }
-  const int8_t* wrow[TM];
+  const int kofs = HEAD + kq * (KC / 4);                    // this lane's k-quarter in a row
+  unsigned wrow[TM];                                        // ... and its weight rows in a tap's plane
 #pragma unroll
-  for (int a = 0; a < TM; ++a) wrow[a] = p.w + (long)min(n0 + 16 * a + r16, p.Kp - 1) * p.Cp + kq * (KC / 4);
+  for (int a = 0; a < TM; ++a) wrow[a] = (unsigned)min(n0 + 16 * a + r16, p.Kp - 1) * (unsigned)p.Cp + kq * (KC / 4);
+  const int dy = (back ? -PW : PW) * RB, dx = back ? -RB : RB;
+  const int org = back ? ((cl.nty - 1) * PW + cl.ntx - 1) * RB : 0;      // patch offset of tap (0, 0)
 
   f4 acc[TM][TN];
 #pragma unroll
@@ -357,20 +362,20 @@ __global__ void __launch_bounds__(64 * WC * WP) q8_halo_kernel(const Q8Conv p, c
     for (int base = tid; base < total; base += 4 * NT) {
       i4 v[4];
       int dst[4];
+      float sc[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int idx = base + u * NT;
         v[u] = i4{0, 0, 0, 0};
+        sc[u] = 0.f;
         dst[u] = -1;
         if (idx < total) {
           const int pp = idx / nq, c = idx - pp * nq, y = pp / PW, x = pp - y * PW, iy = oy + y, ix = ox + x;
-          dst[u] = pp * RB + 16 * c;
+          dst[u] = pp * RB + HEAD + 16 * c;
           if ((unsigned)iy < (unsigned)p.H && (unsigned)ix < (unsigned)p.W) {
             const long pix = ((long)n * p.H + iy) * p.W + ix;
             v[u] = *reinterpret_cast<const i4*>(p.x + pix * p.Cp + c0 + 16 * c);
-            if (c0 == 0 && c == 0) psc[pp] = p.xs[pix];
-          } else if (c0 == 0 && c == 0) {
-            psc[pp] = 0.f;
+            if (c == 0) sc[u] = p.xs[pix];
           }
         }
       }
@@ -378,63 +383,114 @@ __global__ void __launch_bounds__(64 * WC * WP) q8_halo_kernel(const Q8Conv p, c
       for (int u = 0; u < 4; ++u)
         if (dst[u] >= 0) {
           if (KC == 64) {
-            *reinterpret_cast<i4*>(pcd + dst[u]) = v[u];
+            *reinterpret_cast<i4*>(q8_lds + dst[u]) = v[u];
           } else {                                          // (rows of 40 bytes: 8-byte aligned)
-            int2* d = reinterpret_cast<int2*>(pcd + dst[u]);
+            int2* d = reinterpret_cast<int2*>(q8_lds + dst[u]);
             d[0] = int2{v[u][0], v[u][1]};
             d[1] = int2{v[u][2], v[u][3]};
           }
+          if ((base + u * NT) % nq == 0) *reinterpret_cast<float*>(q8_lds + dst[u] - HEAD) = sc[u];
         }
     }
     __syncthreads();
 
-    // steps (tap, chunk); the weights of the next step are loaded before this one's products
-    const int nch = cbytes / KC;
-    auto wofs = [&](int ty, int tx, int ch) __attribute__((always_inline)) {
-      return ((long)(cl.ky0 + p.kst * ty) * p.KW + cl.kx0 + p.kst * tx) * p.Kp * p.Cp + c0 + ch * KC;
-    };
-    F fa[TM], fn[TM];
-    {
-      const long o = wofs(0, 0, 0);
+    // this wave group's steps, the weights of the next two in flight
+    const int nch = ONE ? 1 : cbytes / KC, steps = taps * nch;
+    const int s0 = steps * wk / WK, s1 = steps * (wk + 1) / WK;
+    if (s0 < s1) {
+      const int t0 = s0 / nch, ch0 = s0 - t0 * nch, ty0 = t0 / cl.ntx, tx0 = t0 - ty0 * cl.ntx;
+      int lch = ch0, lty = ty0, ltx = tx0;                  // step to load
+      int ch = ch0, ty = ty0, tx = tx0, s = s0;             // step to compute
+      const long plane = (long)p.Kp * p.Cp;
+      const long wx = p.kst * plane, wy = p.kst * p.KW * plane - (cl.ntx - 1) * wx;      // to the next tap, the next row
+      const int8_t* const w0 = p.w + ((long)cl.ky0 * p.KW + cl.kx0) * plane + c0;
+      const int8_t* wt = w0 + ((long)p.kst * ty0 * p.KW + p.kst * tx0) * plane;
+      auto load = [&](F(&f)[TM]) __attribute__((always_inline)) {
+        const int8_t* wl = ONE ? wt : wt + lch * KC;
 #pragma unroll
-      for (int a = 0; a < TM; ++a) fa[a] = *reinterpret_cast<const F*>(wrow[a] + o);
-    }
-    for (int ty = 0; ty < cl.nty; ++ty)
-      for (int tx = 0; tx < cl.ntx; ++tx) {
-        const int toff = back ? (cl.nty - 1 - ty) * PW + (cl.ntx - 1 - tx) : ty * PW + tx;
-        float xs[TN];
-        i4 ia[TM][TN];
-#pragma unroll
-        for (int b = 0; b < TN; ++b) xs[b] = psc[px[b] + toff];
+        for (int a = 0; a < TM; ++a) f[a] = *reinterpret_cast<const F*>(wl + wrow[a]);
+        const bool nt = ONE || lch + 1 == nch, nr = nt && ltx + 1 == cl.ntx, end = nr && lty + 1 == cl.nty;
+        lch = nt ? 0 : lch + 1;
+        ltx = nr ? 0 : (nt ? ltx + 1 : ltx);
+        lty = end ? 0 : (nr ? lty + 1 : lty);               // (past the last step: the first tap again)
+        wt = end ? w0 : wt + (nr ? wy : (nt ? wx : 0));
+      };
+      i4 ia[TM][TN];
+      if (!ONE)
 #pragma unroll
         for (int a = 0; a < TM; ++a)
 #pragma unroll
           for (int b = 0; b < TN; ++b) ia[a][b] = i4{0, 0, 0, 0};
-        for (int ch = 0; ch < nch; ++ch) {
-          const bool lc = ch + 1 < nch, lx = tx + 1 < cl.ntx, ly = ty + 1 < cl.nty;
-          const long o = lc ? wofs(ty, tx, ch + 1) : (lx ? wofs(ty, tx + 1, 0) : wofs(ly ? ty + 1 : ty, 0, 0));
+      auto step = [&](F(&f)[TM], F(&fl)[TM]) __attribute__((always_inline)) {
+        load(fl);
+        const char* pt = q8_lds + (org + ty * dy + tx * dx);
+        F fb[TN];
+        float xs[TN];
 #pragma unroll
-          for (int a = 0; a < TM; ++a) fn[a] = *reinterpret_cast<const F*>(wrow[a] + o);
-          F fb[TN];
+        for (int b = 0; b < TN; ++b) fb[b] = *reinterpret_cast<const F*>(pt + prow[b] + kofs + (ONE ? 0 : ch * KC));
+        if (ONE) {
 #pragma unroll
-          for (int b = 0; b < TN; ++b)
-            fb[b] = *reinterpret_cast<const F*>(pcd + (px[b] + toff) * RB + ch * KC + kq * (KC / 4));
+          for (int b = 0; b < TN; ++b) xs[b] = *reinterpret_cast<const float*>(pt + prow[b]);
 #pragma unroll
           for (int a = 0; a < TM; ++a)
 #pragma unroll
-            for (int b = 0; b < TN; ++b) ia[a][b] = Q8Frag<KC>::mfma(fa[a], fb[b], ia[a][b]);
+            for (int b = 0; b < TN; ++b) ia[a][b] = Q8Frag<KC>::mfma(f[a], fb[b], i4{0, 0, 0, 0});
+        } else {
 #pragma unroll
-          for (int a = 0; a < TM; ++a) fa[a] = fn[a];
+          for (int a = 0; a < TM; ++a)
+#pragma unroll
+            for (int b = 0; b < TN; ++b) ia[a][b] = Q8Frag<KC>::mfma(f[a], fb[b], ia[a][b]);
         }
+        ++s;
+        if (ONE || ch + 1 == nch || s == s1) {
+          if (!ONE)
 #pragma unroll
-        for (int a = 0; a < TM; ++a)
+            for (int b = 0; b < TN; ++b) xs[b] = *reinterpret_cast<const float*>(pt + prow[b]);
 #pragma unroll
-          for (int b = 0; b < TN; ++b)
+          for (int a = 0; a < TM; ++a)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[a][b][j] = fmaf((float)ia[a][b][j], xs[b], acc[a][b][j]);
+            for (int b = 0; b < TN; ++b) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[a][b][j] = fmaf((float)ia[a][b][j], xs[b], acc[a][b][j]);
+              if (!ONE) ia[a][b] = i4{0, 0, 0, 0};
+            }
+        }
+        const bool nt = ONE || ch + 1 == nch, nr = nt && tx + 1 == cl.ntx;
+        ch = nt ? 0 : ch + 1;
+        tx = nr ? 0 : (nt ? tx + 1 : tx);
+        ty = nr ? ty + 1 : ty;
+      };
+      F f0[TM], f1[TM], f2[TM];
+      load(f0);
+      load(f1);
+      while (true) {
+        step(f0, f2);
+        if (s == s1) break;
+        step(f1, f0);
+        if (s == s1) break;
+        step(f2, f1);
+        if (s == s1) break;
       }
+    }
   }
 
+  if (WK > 1) {
+    __syncthreads();                                        // the patch has been read: its LDS takes the partial sums
+    f4* red = reinterpret_cast<f4*>(q8_lds) + (wp * WC + wc) * (WK - 1) * TM * TN * 64;
+    if (wk > 0)
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TN; ++b) red[((wk - 1) * TM * TN + a * TN + b) * 64 + lane] = acc[a][b];
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll
+    for (int w = 0; w < WK - 1; ++w)
+#pragma unroll
+      for (int a = 0; a < TM; ++a)
+#pragma unroll
+        for (int b = 0; b < TN; ++b) acc[a][b] += red[(w * TM * TN + a * TN + b) * 64 + lane];
+  }
 #pragma unroll
   for (int b = 0; b < TN; ++b) {
     const int q = 16 * (wp * TN + b) + r16, i = i0 + q / tl.TW, j = j0 + q % tl.TW;
@@ -543,25 +599,28 @@ inline int q8_patch(const Q8Conv& p, int TH, int TW) {
   return ((TH - 1) * p.is + nty) * ((TW - 1) * p.is + ntx);
 }
 
-template <int TM, int TN, int WC, int WP>
+template <int TM, int TN, int WC, int WP, int WK>
 bool q8_halo_launch(const Q8Conv& p, int GH, int GW, int classes, hipStream_t st) {
-  constexpr int BP = 16 * TN * WP, BC = 16 * TM * WC;
+  constexpr int BP = 16 * TN * WP, BC = 16 * TM * WC, NT = 64 * WC * WP * WK;
+  constexpr int RED = (WK - 1) * WC * WP * TM * TN * 1024;
+  static_assert(RED <= Q8_LDS, "partial sums fit the patch's LDS");
   Q8Tile t;
   t.TW = GW > 8 ? 16 : (GW > 4 ? 8 : 4);
-  if (BP / t.TW < 1) return false;
   const int TH = BP / t.TW, NP = q8_patch(p, TH, t.TW), kc = p.Cp % 64 == 0 ? 64 : 32;
   t.tx = tde_cdiv(GW, t.TW); t.ty = tde_cdiv(GH, TH);
-  t.cb = (Q8_LDS - 4 * NP - 16) / NP - kc / 4;
+  t.cb = Q8_LDS / NP - kc / 4;
   t.cb = t.cb >= p.Cp ? p.Cp : t.cb / kc * kc;
   if (t.cb < kc) return false;
-  const int lds = ((4 * NP + 15) & ~15) + NP * (t.cb + kc / 4);
+  const int patch = NP * (t.cb + kc / 4), lds = patch > RED ? patch : RED;
   const long blocks = (long)p.N * t.tx * t.ty;
-  if (blocks > 0x7fffffffL) return false;
+  if (blocks * NT >= (1L << 32)) return false;
   const dim3 grid((unsigned)blocks, tde_cdiv(p.K, BC), classes);
-  if (kc == 64)
-    hipLaunchKernelGGL((q8_halo_kernel<TM, TN, 64, WC, WP>), grid, dim3(64 * WC * WP), lds, st, p, t);
+  if (kc == 32)
+    hipLaunchKernelGGL((q8_halo_kernel<TM, TN, 32, true, WC, WP, WK>), grid, dim3(NT), lds, st, p, t);
+  else if (p.Cp == 64)
+    hipLaunchKernelGGL((q8_halo_kernel<TM, TN, 64, true, WC, WP, WK>), grid, dim3(NT), lds, st, p, t);
   else
-    hipLaunchKernelGGL((q8_halo_kernel<TM, TN, 32, WC, WP>), grid, dim3(64 * WC * WP), lds, st, p, t);
+    hipLaunchKernelGGL((q8_halo_kernel<TM, TN, 64, false, WC, WP, WK>), grid, dim3(NT), lds, st, p, t);
   return true;
 }
 
@@ -589,12 +648,32 @@ int q8_conv(Q8Conv p, hipStream_t st) {
   }
   bool done = false;
   if (GH * GW >= 32 && tiles > 1024) {
-    // pixels per block: 256 (128, 64 with more channels), halved while that leaves CUs without a block
-    const bool few = Mmax * classes * ((p.K + 127) / 128) < 256L * 256;
-    if (p.K <= 16) done = few ? q8_halo_launch<1, 2, 1, 4>(p, GH, GW, classes, st) : q8_halo_launch<1, 4, 1, 4>(p, GH, GW, classes, st);
-    else if (p.K <= 32) done = few ? q8_halo_launch<2, 2, 1, 4>(p, GH, GW, classes, st) : q8_halo_launch<2, 4, 1, 4>(p, GH, GW, classes, st);
-    else if (p.K <= 64) done = few ? q8_halo_launch<2, 2, 2, 2>(p, GH, GW, classes, st) : q8_halo_launch<2, 4, 2, 2>(p, GH, GW, classes, st);
-    else done = few ? q8_halo_launch<2, 2, 4, 1>(p, GH, GW, classes, st) : q8_halo_launch<2, 4, 4, 1>(p, GH, GW, classes, st);
+    static const int force = std::getenv("TDE_Q8V") ? std::atoi(std::getenv("TDE_Q8V")) : -1;
+    const long px = Mmax * classes;
+    int v;
+    if (p.K <= 16) v = px >= 256L * 512 ? 0 : 4;
+    else if (p.K <= 32) v = px >= 256L * 512 ? 1 : 5;
+    else if (p.K <= 64) v = px >= 128L * 512 ? 2 : 6;
+    else v = px * ((p.K + 127) / 128) >= 64L * 512 ? 3 : 7;
+    if (force >= 0) v = force;
+    switch (v) {
+      case 0: done = q8_halo_launch<1, 4, 1, 4, 1>(p, GH, GW, classes, st); break;
+      case 1: done = q8_halo_launch<2, 4, 1, 4, 1>(p, GH, GW, classes, st); break;
+      case 2: done = q8_halo_launch<2, 4, 2, 2, 1>(p, GH, GW, classes, st); break;
+      case 3: done = q8_halo_launch<2, 4, 4, 1, 1>(p, GH, GW, classes, st); break;
+      case 4: done = q8_halo_launch<1, 2, 1, 2, 2>(p, GH, GW, classes, st); break;
+      case 5: done = q8_halo_launch<2, 2, 1, 2, 2>(p, GH, GW, classes, st); break;
+      case 6: done = q8_halo_launch<2, 2, 2, 1, 4>(p, GH, GW, classes, st); break;
+      case 7: done = q8_halo_launch<2, 4, 2, 1, 4>(p, GH, GW, classes, st); break;
+      case 8: done = q8_halo_launch<2, 2, 1, 4, 2>(p, GH, GW, classes, st); break;
+      case 9: done = q8_halo_launch<2, 4, 2, 2, 2>(p, GH, GW, classes, st); break;
+      case 10: done = q8_halo_launch<2, 2, 2, 2, 4>(p, GH, GW, classes, st); break;
+      case 11: done = q8_halo_launch<2, 4, 1, 2, 2>(p, GH, GW, classes, st); break;
+      case 12: done = q8_halo_launch<1, 4, 1, 2, 2>(p, GH, GW, classes, st); break;
+      case 13: done = q8_halo_launch<4, 4, 2, 2, 1>(p, GH, GW, classes, st); break;
+      case 14: done = q8_halo_launch<4, 2, 2, 1, 4>(p, GH, GW, classes, st); break;
+      case 15: done = q8_halo_launch<2, 2, 1, 4, 1>(p, GH, GW, classes, st); break;
+    }
   }
   if (!done) {
     if (tiles <= 4096) q8_split_launch<1, 1, 16, 4>(p, Mmax, classes, st);
