@@ -505,6 +505,9 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
 // (global_load_lds_dwordx4: a wave instruction copies 16 rows of 64 bytes) into a ring of three slots, two steps in
 // flight across the barriers; the 16-byte quarters of a row are exchanged by (row >> 1) & 3 on the way, so that the
 // fragment reads of 8 neighbouring rows hit different banks.  All sums stay integers until the end.
+// 8192 x 2048 x 2048: 43 us = 1590 TOP/s with 256 x 256 tiles on 8 waves, whose LDS reads (96 bytes a clock) run under the
+// products because the pixel fragments, which every product needs, are read first (55 us the other way round); 128 x 128
+// tiles read 128 bytes a clock for the same products and take 65 us, and serve where the large ones leave CUs idle.
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef __attribute__((address_space(1))) void* gbl_ptr_t;
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -544,6 +547,18 @@ __global__ void __launch_bounds__(64 * WC * WP) q8_gemm_kernel(const Q8Conv p, i
 
   const int lofs = r16 * 64 + ((kq ^ ((r16 >> 1) & 3)) << 4);
   const int steps = p.Cp / 64, last = steps - 1;
+  auto compute = [&](int slot) __attribute__((always_inline)) {
+    const char* base = q8_lds + slot * SLOT + lofs;
+    i4 fa[TM], fb[TN];
+#pragma unroll
+    for (int b = 0; b < TN; ++b) fb[b] = *reinterpret_cast<const i4*>(base + BC * 64 + (wp * TN + b) * 1024);
+#pragma unroll
+    for (int a = 0; a < TM; ++a) fa[a] = *reinterpret_cast<const i4*>(base + (wc * TM + a) * 1024);
+#pragma unroll
+    for (int a = 0; a < TM; ++a)
+#pragma unroll
+      for (int b = 0; b < TN; ++b) acc[a][b] = Q8Frag<64>::mfma(fa[a], fb[b], acc[a][b]);
+  };
   dma(0, 0);
   dma(min(1, last), 1);
   int slot = 0;
@@ -551,16 +566,7 @@ __global__ void __launch_bounds__(64 * WC * WP) q8_gemm_kernel(const Q8Conv p, i
     vm_wait<DI>();        // this wave's part of step s has landed (step s + 1 may still fly)
     lds_barrier();        // everybody's has, and everybody is done with the slot of step s - 1
     dma(min(s + 2, last), slot == 0 ? 2 : slot - 1);
-    const char* base = q8_lds + slot * SLOT + lofs;
-    i4 fa[TM], fb[TN];
-#pragma unroll
-    for (int a = 0; a < TM; ++a) fa[a] = *reinterpret_cast<const i4*>(base + (wc * TM + a) * 1024);
-#pragma unroll
-    for (int b = 0; b < TN; ++b) fb[b] = *reinterpret_cast<const i4*>(base + BC * 64 + (wp * TN + b) * 1024);
-#pragma unroll
-    for (int a = 0; a < TM; ++a)
-#pragma unroll
-      for (int b = 0; b < TN; ++b) acc[a][b] = Q8Frag<64>::mfma(fa[a], fb[b], acc[a][b]);
+    compute(slot);
     slot = slot == 2 ? 0 : slot + 1;
   }
   vm_wait<0>();           // no DMA may outlive the block's LDS
@@ -641,39 +647,29 @@ int q8_conv(Q8Conv p, hipStream_t st) {
   const long Mmax = (long)p.N * GH * GW;
   const long tiles = ((Mmax + 15) / 16) * ((p.K + 15) / 16) * classes;      // 16 x 16 tiles
   if (p.KH == 1 && p.KW == 1 && p.is == 1 && p.os == 1 && p.OH == p.H && p.OW == p.W && p.Cp % 64 == 0 && tiles > 2048) {
-    const long big = (long)tde_cdiv(Mmax, 256) * tde_cdiv(p.K, 256);
+    const long big = (long)tde_cdiv(Mmax, 256) * tde_cdiv(p.K, 256);      // tiles of 256 x 256
     if (big >= 192) q8_gemm_launch<8, 4, 2, 4>(p, (int)Mmax, st);
     else q8_gemm_launch<4, 4, 2, 2>(p, (int)Mmax, st);
     return tde_launch_status();
   }
   bool done = false;
-  if (GH * GW >= 32 && tiles > 1024) {
-    static const int force = std::getenv("TDE_Q8V") ? std::atoi(std::getenv("TDE_Q8V")) : -1;
-    const long px = Mmax * classes;
-    int v;
-    if (p.K <= 16) v = px >= 256L * 512 ? 0 : 4;
-    else if (p.K <= 32) v = px >= 256L * 512 ? 1 : 5;
-    else if (p.K <= 64) v = px >= 128L * 512 ? 2 : 6;
-    else v = px * ((p.K + 127) / 128) >= 64L * 512 ? 3 : 7;
-    if (force >= 0) v = force;
-    switch (v) {
-      case 0: done = q8_halo_launch<1, 4, 1, 4, 1>(p, GH, GW, classes, st); break;
-      case 1: done = q8_halo_launch<2, 4, 1, 4, 1>(p, GH, GW, classes, st); break;
-      case 2: done = q8_halo_launch<2, 4, 2, 2, 1>(p, GH, GW, classes, st); break;
-      case 3: done = q8_halo_launch<2, 4, 4, 1, 1>(p, GH, GW, classes, st); break;
-      case 4: done = q8_halo_launch<1, 2, 1, 2, 2>(p, GH, GW, classes, st); break;
-      case 5: done = q8_halo_launch<2, 2, 1, 2, 2>(p, GH, GW, classes, st); break;
-      case 6: done = q8_halo_launch<2, 2, 2, 1, 4>(p, GH, GW, classes, st); break;
-      case 7: done = q8_halo_launch<2, 4, 2, 1, 4>(p, GH, GW, classes, st); break;
-      case 8: done = q8_halo_launch<2, 2, 1, 4, 2>(p, GH, GW, classes, st); break;
-      case 9: done = q8_halo_launch<2, 4, 2, 2, 2>(p, GH, GW, classes, st); break;
-      case 10: done = q8_halo_launch<2, 2, 2, 2, 4>(p, GH, GW, classes, st); break;
-      case 11: done = q8_halo_launch<2, 4, 1, 2, 2>(p, GH, GW, classes, st); break;
-      case 12: done = q8_halo_launch<1, 4, 1, 2, 2>(p, GH, GW, classes, st); break;
-      case 13: done = q8_halo_launch<4, 4, 2, 2, 1>(p, GH, GW, classes, st); break;
-      case 14: done = q8_halo_launch<4, 2, 2, 1, 4>(p, GH, GW, classes, st); break;
-      case 15: done = q8_halo_launch<2, 2, 1, 4, 1>(p, GH, GW, classes, st); break;
-    }
+  if (GH * GW >= 12 && tiles > 64) {
+    // Blocks of fewer pixels and channels, and more wave groups that split the steps, the fewer tiles there are; timed for
+    // each size on the networks' layers at batch 1, 8 and 32 (us, this choice / the next larger block):
+    // 14x14x512 -> 256 8.3 / 10.4, 28x28x256 -> 128 6.4 / 7.9, 6x8x1024 -> 512 (8) 16.1 / 19.3, 24x32x128 -> 128 (8)
+    // 9.6 / 10.5, 12x16x512 -> 256 (8) 15.3 / 18.0, 48x64x64 -> 64 k5 (8) 11.6 / 13.4, 96x128x32 -> 32 k7 (8) 22.0 / 28.2,
+    // (32) 64.8 / 72.9 with this choice's smaller neighbour, 24x32x256 -> 128 (32) 23.7 / 28.1
+    if (tiles < 512) done = q8_halo_launch<1, 2, 1, 1, 8>(p, GH, GW, classes, st);
+    else if (tiles < 1536) done = q8_halo_launch<2, 2, 1, 1, 8>(p, GH, GW, classes, st);
+    else if (p.K <= 16) done = tiles < 8192 ? q8_halo_launch<1, 4, 1, 2, 2>(p, GH, GW, classes, st)
+                                            : q8_halo_launch<1, 4, 1, 4, 1>(p, GH, GW, classes, st);
+    else if (tiles < 4096) done = p.K > 64 && p.Cp > 128 ? q8_halo_launch<2, 4, 1, 1, 4>(p, GH, GW, classes, st)
+                                                         : q8_halo_launch<2, 2, 1, 1, 4>(p, GH, GW, classes, st);
+    else if (p.K > 64) done = q8_halo_launch<2, 4, 2, 1, 2>(p, GH, GW, classes, st);
+    else if (tiles < 8192) done = q8_halo_launch<2, 2, 1, 2, 2>(p, GH, GW, classes, st);
+    else if (p.K > 32) done = q8_halo_launch<2, 4, 2, 2, 1>(p, GH, GW, classes, st);
+    else if (tiles < 16384) done = q8_halo_launch<2, 4, 1, 2, 2>(p, GH, GW, classes, st);
+    else done = q8_halo_launch<2, 4, 1, 4, 1>(p, GH, GW, classes, st);
   }
   if (!done) {
     if (tiles <= 4096) q8_split_launch<1, 1, 16, 4>(p, Mmax, classes, st);

@@ -97,7 +97,7 @@ __device__ __forceinline__ void tape_row(const d4& u, f4& y, int& packed, float&
 struct TapeFwd {
   int Mg, C, NB, G;          // rows per group, channels, 64-channel blocks, groups
   const float *z, *beta;
-  double Mt;                 // rows per group over all replicas
+  double Mt, invM;           // rows per group over all replicas
   float eps, decay;
   int bessel;
   float *mm, *mv, *save_mean, *save_invstd;
@@ -107,12 +107,18 @@ struct TapeFwd {
   float* scales;
 };
 
-__device__ __forceinline__ void tape_stats(double s0, double s1, double Mt, float eps, double& mean, double& var,
-                                           double& is) {
+// mean (a true quotient: a constant channel's mean is its value, so u = beta there), variance, 1 / sqrt(var + eps): the
+// estimate of v_rsq_f64 and two Newton steps, off by a last bit or two, for a quarter of the instructions of sqrt and divide
+__device__ __forceinline__ void tape_stats(double s0, double s1, double Mt, double invM, float eps, double& mean,
+                                           double& var, double& is) {
   mean = s0 / Mt;
-  var = s1 / Mt - mean * mean;
+  var = s1 * invM - mean * mean;
   if (var < 0) var = 0;
-  is = 1.0 / sqrt(var + (double)eps);
+  const double x = var + (double)eps;
+  double y = __builtin_amdgcn_rsq(x);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) y = fma(0.5 * y, fma(-x * y, y, 1.0), y);
+  is = x > 0.0 && x < 1e300 ? y : 1.0 / sqrt(x);          // (zero, infinity and NaN: as the formula)
 }
 
 // statistics and moving averages of channel c of every group, groups in order
@@ -120,7 +126,7 @@ __device__ __forceinline__ void tape_publish(const TapeFwd& p, const double* sum
   float m0 = p.mm ? p.mm[c] : 0.f, v0 = p.mm ? p.mv[c] : 0.f;
   for (int g = 0; g < p.G; ++g) {
     double mean, var, is;
-    tape_stats(sums[(long)g * 2 * p.C + c], sums[(long)g * 2 * p.C + p.C + c], p.Mt, p.eps, mean, var, is);
+    tape_stats(sums[(long)g * 2 * p.C + c], sums[(long)g * 2 * p.C + p.C + c], p.Mt, p.invM, p.eps, mean, var, is);
     p.save_mean[(long)g * p.C + c] = (float)mean;
     p.save_invstd[(long)g * p.C + c] = (float)is;
     const double vu = (p.bessel && p.Mt > 1) ? var * p.Mt / (p.Mt - 1) : var;
@@ -213,28 +219,34 @@ __global__ void __launch_bounds__(256) tape_sums_kernel(const TapeSums p) {
   }
 }
 
-// part [G * per_g][2C] -> sums [G][2C] (and a copy): block = 16 columns x 64 stripes, grid (columns, group)
+// part [G * per_g][2C] -> sums [G][2C] (and a copy): block = 8 columns x 128 stripes, up to 8 chunks per lane in flight;
+// grid (columns, group)
 __global__ void __launch_bounds__(1024) tape_finalize_kernel(int C2, int per_g, const double* part, double* sums,
                                                              double* copy) {
-  __shared__ double sh[64][16];
-  const int col = threadIdx.x & 15, st = threadIdx.x >> 4, cc = blockIdx.x * 16 + col;
+  __shared__ double sh[128][8];
+  const int col = threadIdx.x & 7, st = threadIdx.x >> 3, cc = blockIdx.x * 8 + col;
   const double* pp = part + (long)blockIdx.y * per_g * C2;
-  double a[4] = {0, 0, 0, 0};
-  if (cc < C2) {
-    int k = st;
-    for (; k + 192 < per_g; k += 256)
+  double a = 0;
+  if (cc < C2)
+    for (int k0 = st; k0 < per_g; k0 += 1024) {
+      double v[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) a[u] += pp[(long)(k + 64 * u) * C2 + cc];
-    for (int u = 0; k < per_g; k += 64, ++u) a[u] += pp[(long)k * C2 + cc];
-  }
-  sh[st][col] = (a[0] + a[1]) + (a[2] + a[3]);
+      for (int u = 0; u < 8; ++u) v[u] = k0 + 128 * u < per_g ? pp[(long)(k0 + 128 * u) * C2 + cc] : 0.0;
+      a += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+    }
+  sh[st][col] = a;
   __syncthreads();
-  if (threadIdx.x < 16 && cc < C2) {
+  if (threadIdx.x < 64) {          // one wave: 8 columns x 8 lanes of 16 stripes
+    const int part8 = threadIdx.x >> 3;
     double s = 0;
 #pragma unroll
-    for (int k = 0; k < 64; ++k) s += sh[k][col];
-    sums[(long)blockIdx.y * C2 + cc] = s;
-    if (copy) copy[(long)blockIdx.y * C2 + cc] = s;
+    for (int k = 0; k < 16; ++k) s += sh[part8 * 16 + k][col];
+#pragma unroll
+    for (int o = 8; o < 64; o <<= 1) s += __shfl_xor(s, o, 64);
+    if (threadIdx.x < 8 && cc < C2) {
+      sums[(long)blockIdx.y * C2 + cc] = s;
+      if (copy) copy[(long)blockIdx.y * C2 + cc] = s;
+    }
   }
 }
 
@@ -253,7 +265,7 @@ __global__ void __launch_bounds__(256) tape_fwd_apply_kernel(const TapeFwd p, co
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       double m, v, i;
-      tape_stats(sums[(long)g * 2 * p.C + c + j], sums[(long)g * 2 * p.C + p.C + c + j], p.Mt, p.eps, m, v, i);
+      tape_stats(sums[(long)g * 2 * p.C + c + j], sums[(long)g * 2 * p.C + p.C + c + j], p.Mt, p.invM, p.eps, m, v, i);
       mu[j] = m; is[j] = i; bt[j] = (double)p.beta[c + j];
       if (blockIdx.x == 0 && g == 0 && rl == 0) tape_publish(p, sums, c + j);
     }
@@ -349,7 +361,7 @@ __global__ void __launch_bounds__(SMALL_NT) tape_fwd_small_kernel(const TapeFwd 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         double m, var, i;
-        tape_stats(tot[l][j], tot[l][4 + j], p.Mt, p.eps, m, var, i);
+        tape_stats(tot[l][j], tot[l][4 + j], p.Mt, p.invM, p.eps, m, var, i);
         mu[j] = m; is[j] = i;
         if (rl == 0) {
           p.save_mean[(long)g * p.C + c + j] = (float)m;
@@ -587,11 +599,11 @@ TapePlan tape_plan(int M, int C, int G) {
   t.per_g = tde_cdiv(Mg, t.rpc);
   return t;
 }
-// rows of an apply block: eight steps of its row lanes, more when that is over 2048 blocks
+// rows of an apply block: four steps of its row lanes, more when that is over 2048 blocks
 int tape_apply_rows(int M, int C, const TapePlan& t) {
   const int R = 256 / (t.NB * t.L);
   const long want = ((long)M + 2047) / 2048;
-  return (int)(want > 8 * R ? want : 8 * R);
+  return (int)(want > 4 * R ? want : 4 * R);
 }
 bool tape_small(int Mg, int L) { return Mg <= SMALL_RB * SMALL_NT / L; }
 
@@ -613,7 +625,7 @@ void tape_sums_launch(int mode, const TapePlan& t, int G, TapeSums p, double* pa
   else hipLaunchKernelGGL((tape_sums_kernel<LL, 1>), grid, dim3(256), 0, st, p)
   TAPE_L(t.L, F)
 #undef F
-  hipLaunchKernelGGL(tape_finalize_kernel, dim3(tde_cdiv(2 * p.C, 16), G), dim3(1024), 0, st, 2 * p.C, t.per_g, part,
+  hipLaunchKernelGGL(tape_finalize_kernel, dim3(tde_cdiv(2 * p.C, 8), G), dim3(1024), 0, st, 2 * p.C, t.per_g, part,
                      sums, copy);
 }
 void tape_fwd_apply_launch(const TapePlan& t, const TapeFwd& p, const double* sums, hipStream_t st) {
@@ -668,12 +680,14 @@ int tde_tape8_bn_fwd(int M, int C, int groups, const float* z, const float* beta
                 (moving_mean == nullptr) == (moving_var == nullptr));
   hipStream_t st = static_cast<hipStream_t>(stream);
   const TapePlan t = tape_plan(M, C, groups);
-  const TapeFwd p{M / groups, C, t.NB, groups, z, beta, (double)(M / groups), eps, decay, bessel, moving_mean, moving_var,
+  const TapeFwd p{M / groups, C, t.NB, groups, z, beta, (double)(M / groups), 1.0 / (M / groups), eps, decay, bessel, moving_mean, moving_var,
                   save_mean, save_invstd, y, y_cstride, y_coff, codes, scales};
   if (tape_small(p.Mg, t.L)) {
 #define F(LL)                                                                                                       \
   if (p.Mg <= 2 * SMALL_NT / LL)                                                                                    \
     hipLaunchKernelGGL((tape_fwd_small_kernel<LL, 2>), dim3(t.NB), dim3(SMALL_NT), 0, st, p);                       \
+  else if (p.Mg <= 4 * SMALL_NT / LL)                                                                               \
+    hipLaunchKernelGGL((tape_fwd_small_kernel<LL, 4>), dim3(t.NB), dim3(SMALL_NT), 0, st, p);                       \
   else                                                                                                              \
     hipLaunchKernelGGL((tape_fwd_small_kernel<LL, SMALL_RB>), dim3(t.NB), dim3(SMALL_NT), 0, st, p)
     TAPE_L(t.L, F)
@@ -699,7 +713,7 @@ int tde_tape8_bn_fwd_from_sums(int M, int C, int groups, long M_total, const flo
                 save_mean && save_invstd && tape_view_ok(y, C, y_cstride, y_coff) && tape_ok(codes, scales) &&
                 (moving_mean == nullptr) == (moving_var == nullptr));
   const TapePlan t = tape_plan(M, C, groups);
-  const TapeFwd p{M / groups, C, t.NB, groups, z, beta, (double)M_total, eps, decay, bessel, moving_mean, moving_var,
+  const TapeFwd p{M / groups, C, t.NB, groups, z, beta, (double)M_total, 1.0 / (double)M_total, eps, decay, bessel, moving_mean, moving_var,
                   save_mean, save_invstd, y, y_cstride, y_coff, codes, scales};
   tape_fwd_apply_launch(t, p, sums, static_cast<hipStream_t>(stream));
   return tde_launch_status();
@@ -765,6 +779,8 @@ int tde_tape8_bn_bwd(int M, int C, int groups, const int8_t* codes, const float*
 #define F(LL)                                                                                                       \
   if (p.Mg <= 2 * SMALL_NT / LL)                                                                                    \
     hipLaunchKernelGGL((tape_bwd_small_kernel<LL, 2>), dim3(t.NB), dim3(SMALL_NT), 0, st, p);                       \
+  else if (p.Mg <= 4 * SMALL_NT / LL)                                                                               \
+    hipLaunchKernelGGL((tape_bwd_small_kernel<LL, 4>), dim3(t.NB), dim3(SMALL_NT), 0, st, p);                       \
   else                                                                                                              \
     hipLaunchKernelGGL((tape_bwd_small_kernel<LL, SMALL_RB>), dim3(t.NB), dim3(SMALL_NT), 0, st, p)
     TAPE_L(t.L, F)

@@ -241,35 +241,47 @@ class Tape8:
 
     @classmethod
     def _empty(cls, shape, C, rows, groups, device):
-        """The tape of a forward, in one buffer: codes, scales, invstd and mean behind one another, 16 bytes aligned."""
+        """The tape of a forward, in one buffer of floats: codes, scales, invstd and mean behind one another, 16 bytes
+        aligned."""
         t = cls.__new__(cls)
         t.shape, t.C, t.rows, t.groups = shape, C, rows, groups
-        s = (rows * C + 15) // 16 * 16
-        i = s + (rows * ((C + BLOCK - 1) // BLOCK) * 4 + 15) // 16 * 16
-        m = i + 4 * groups * C
-        t._buffer, t._views = torch.empty(m + 4 * groups * C, dtype=torch.int8, device=device), None
+        s = (rows * C + 15) // 16 * 4
+        i = s + (rows * ((C + BLOCK - 1) // BLOCK) + 3) // 4 * 4
+        m = i + groups * C
+        t._buffer, t._views, t._at = torch.empty(m + groups * C, dtype=torch.float32, device=device), None, (s, i, m)
         p = t._buffer.data_ptr()
-        t._ptrs, t._mean_ptr, t._at = (p, p + s, p + i), p + m, (s, i, m)
+        t._ptrs, t._mean_ptr = (p, p + 4 * s, p + 4 * i), p + 4 * m
         return t
 
-    def _view(self, k):
-        if self._views is None:
-            b, (s, i, m), nb, gc = self._buffer, self._at, (self.C + BLOCK - 1) // BLOCK, 4 * self.groups * self.C
-            self._views = (b[:self.rows * self.C].view(self.shape),
-                           b[s:s + 4 * self.rows * nb].view(torch.float32).view(self.shape[:-1] + (nb,)),
-                           b[i:i + gc].view(torch.float32).view(self.groups, self.C),
-                           b[m:m + gc].view(torch.float32).view(self.groups, self.C))
-        return self._views[k]
+    @property
+    def codes(self):
+        if self._views is not None:
+            return self._views[0]
+        return self._buffer.view(torch.int8)[:self.rows * self.C].view(self.shape)
 
-    codes = property(lambda self: self._view(0))
-    scales = property(lambda self: self._view(1))
-    invstd = property(lambda self: self._view(2))
-    mean = property(lambda self: self._view(3))
+    @property
+    def scales(self):
+        if self._views is not None:
+            return self._views[1]
+        nb, s = (self.C + BLOCK - 1) // BLOCK, self._at[0]
+        return self._buffer[s:s + self.rows * nb].view(self.shape[:-1] + (nb,))
+
+    @property
+    def invstd(self):
+        if self._views is not None:
+            return self._views[2]
+        return self._buffer.as_strided((self.groups, self.C), (self.C, 1), self._at[1])
+
+    @property
+    def mean(self):
+        if self._views is not None:
+            return self._views[3]
+        return self._buffer.as_strided((self.groups, self.C), (self.C, 1), self._at[2])
 
     def restore(self, relu=True, out=None):
         """The tape's values [..., C]: relu=True the layer's output as the consumers' filter gradients read it, relu=False
         the coded pre-activation."""
-        _check(self._buffer, "codes", torch.int8)
+        _check(self._buffer, "tape", self._buffer.dtype)
         dev = self._buffer.device
         y = _out(out, self.shape, dev)
         rows, _, cs = _rows(y, "out")
@@ -354,7 +366,7 @@ def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
     if not isinstance(tape, Tape8):
         raise ValueError("tape must be a Tape8")
     _check(dy, "dy")
-    _check(tape._buffer, "codes", torch.int8)
+    _check(tape._buffer, "tape", tape._buffer.dtype)
     shape, dev, C = tape.shape, dy.device, tape.C
     _check_beta(C, beta)
     if dy.shape != shape:
