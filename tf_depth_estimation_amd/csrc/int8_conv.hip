@@ -71,43 +71,56 @@ __device__ __forceinline__ int q8_code4(const f4& x, const Q8Div& d) {
   return p;
 }
 
-// ---- rows: L lanes per row (a power of two <= 64), QPL quads of channels per lane held in registers; VEC: 16-byte loads
-template <int L, int QPL, bool VEC>
+// ---- rows: L lanes per row (a power of two <= 64), QPL quads of channels per lane and RT rows held in registers, so that
+// a lane has about four loads in flight; VEC: 16-byte loads
+template <int L, int QPL, int RT, bool VEC>
 __global__ void __launch_bounds__(256) q8_rows_kernel(long rows, int C, int Cp, const float* x, long cs, int co,
                                                       int8_t* codes, float* scales) {
+  constexpr int R = 256 / L;
   const int l = threadIdx.x % L;
-  for (long row = (long)blockIdx.x * (256 / L) + threadIdx.x / L; row <= rows; row += (long)gridDim.x * (256 / L)) {
-    const float* px = x + row * cs + co;
-    f4 v[QPL];
-    unsigned am = 0;
+  for (long r0 = (long)blockIdx.x * (R * RT) + threadIdx.x / L; r0 <= rows; r0 += (long)gridDim.x * (R * RT)) {
+    f4 v[RT][QPL];
 #pragma unroll
-    for (int i = 0; i < QPL; ++i) {
-      const int c = 4 * (l + i * L);
-      v[i] = f4{0.f, 0.f, 0.f, 0.f};
-      if (row < rows && c < C) {
-        if (VEC) {
-          v[i] = *reinterpret_cast<const f4*>(px + c);
+    for (int t = 0; t < RT; ++t) {
+      const long row = r0 + t * R;
+      const float* px = x + row * cs + co;
 #pragma unroll
-          for (int j = 1; j < 4; ++j)
-            if (c + j >= C) v[i][j] = 0.f;
-        } else {
+      for (int i = 0; i < QPL; ++i) {
+        const int c = 4 * (l + i * L);
+        v[t][i] = f4{0.f, 0.f, 0.f, 0.f};
+        if (row < rows && c < C) {
+          if (VEC) {
+            v[t][i] = *reinterpret_cast<const f4*>(px + c);
+          } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (c + j < C) v[i][j] = px[c + j];
+            for (int j = 0; j < 4; ++j)
+              if (c + j < C) v[t][i][j] = px[c + j];
+          }
         }
       }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) am = max(am, __float_as_uint(v[i][j]) & 0x7fffffffu);
     }
 #pragma unroll
-    for (int o = 1; o < L; o <<= 1) am = max(am, (unsigned)__shfl_xor((int)am, o, 64));
-    const Q8Div d = q8_div(am);
+    for (int t = 0; t < RT; ++t) {
+      const long row = r0 + t * R;
+      if (row > rows) break;
+      unsigned am = 0;
 #pragma unroll
-    for (int i = 0; i < QPL; ++i) {
-      const int c = 4 * (l + i * L);
-      if (c < Cp) *reinterpret_cast<int*>(codes + row * Cp + c) = q8_code4(v[i], d);
+      for (int i = 0; i < QPL; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (VEC && 4 * (l + i * L) + j >= C) v[t][i][j] = 0.f;
+          am = max(am, __float_as_uint(v[t][i][j]) & 0x7fffffffu);
+        }
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) am = max(am, (unsigned)__shfl_xor((int)am, o, 64));
+      const Q8Div d = q8_div(am);
+#pragma unroll
+      for (int i = 0; i < QPL; ++i) {
+        const int c = 4 * (l + i * L);
+        if (c < Cp) *reinterpret_cast<int*>(codes + row * Cp + c) = q8_code4(v[t][i], d);
+      }
+      if (l == 0) scales[row] = q8_scale(am);      // (row `rows`: no channel was read, scale 0)
     }
-    if (l == 0) scales[row] = q8_scale(am);      // (row `rows`: no channel was read, scale 0)
   }
 }
 
@@ -705,24 +718,26 @@ int tde_q8_rows(int rows, int C, const float* x, int x_cstride, int x_coff, int8
   const int Cp = q8_row(C), nq = Cp / 4;
   const bool vec = tde_aligned16(x) && x_cstride % 4 == 0 && x_coff % 4 == 0 && x_coff + (C + 3) / 4 * 4 <= x_cstride;
   hipStream_t st = static_cast<hipStream_t>(stream);
-#define R(LL, QQ)                                                                                                     \
+#define R(LL, QQ, TT)                                                                                                 \
   do {                                                                                                                \
-    const dim3 grid((unsigned)(tde_cdiv((long)rows + 1, 256 / LL) < (1 << 20) ? tde_cdiv((long)rows + 1, 256 / LL) : 1 << 20)); \
+    const long nb = tde_cdiv((long)rows + 1, 256 / LL * TT);                                                          \
+    const dim3 grid((unsigned)(nb < (1 << 20) ? nb : 1 << 20));                                                       \
     if (vec)                                                                                                          \
-      hipLaunchKernelGGL((q8_rows_kernel<LL, QQ, true>), grid, dim3(256), 0, st, (long)rows, C, Cp, x, (long)x_cstride, \
-                         x_coff, codes, scales);                                                                      \
+      hipLaunchKernelGGL((q8_rows_kernel<LL, QQ, TT, true>), grid, dim3(256), 0, st, (long)rows, C, Cp, x,            \
+                         (long)x_cstride, x_coff, codes, scales);                                                     \
     else                                                                                                              \
-      hipLaunchKernelGGL((q8_rows_kernel<LL, QQ, false>), grid, dim3(256), 0, st, (long)rows, C, Cp, x,               \
+      hipLaunchKernelGGL((q8_rows_kernel<LL, QQ, TT, false>), grid, dim3(256), 0, st, (long)rows, C, Cp, x,           \
                          (long)x_cstride, x_coff, codes, scales);                                                     \
   } while (0)
-  if (nq <= 8) R(8, 1);
-  else if (nq <= 16) R(16, 1);
-  else if (nq <= 32) R(32, 1);
-  else if (nq <= 64) R(64, 1);
-  else if (nq <= 128) R(64, 2);
-  else if (nq <= 256) R(64, 4);
-  else if (nq <= 512) R(64, 8);
-  else R(64, 16);
+  const bool many = rows >= 1 << 15;      // one row per lane group in flight where there are few rows
+  if (nq <= 8) { if (many) R(8, 1, 4); else R(8, 1, 1); }
+  else if (nq <= 16) { if (many) R(16, 1, 4); else R(16, 1, 1); }
+  else if (nq <= 32) { if (many) R(32, 1, 4); else R(32, 1, 1); }
+  else if (nq <= 64) { if (many) R(64, 1, 4); else R(64, 1, 1); }
+  else if (nq <= 128) R(64, 2, 1);
+  else if (nq <= 256) R(64, 4, 1);
+  else if (nq <= 512) R(64, 8, 1);
+  else R(64, 16, 1);
 #undef R
   return tde_launch_status();
 }

@@ -260,25 +260,32 @@ __global__ void __launch_bounds__(256) tape_fwd_apply_kernel(const TapeFwd p, co
   if (rl >= R) return;
   const int b = q / L, c = 4 * q, g = blockIdx.y;
   const bool on = c < p.C;
+  const long base = (long)g * p.Mg;
+  const int r0 = blockIdx.x * rpb, r1 = min(p.Mg, r0 + rpb);
+  f4 v[APPLY_RB];
+  auto load = [&](int rb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < APPLY_RB; ++i) {
+      const int r = min(rb + i * R, r1 - 1);
+      v[i] = on ? *reinterpret_cast<const f4*>(p.z + (base + r) * p.C + c) : f4{0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  load(r0 + rl);                       // in flight while the statistics are evaluated
   d4 mu = {0, 0, 0, 0}, is = {0, 0, 0, 0}, bt = {0, 0, 0, 0};
   if (on) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      double m, v, i;
-      tape_stats(sums[(long)g * 2 * p.C + c + j], sums[(long)g * 2 * p.C + p.C + c + j], p.Mt, p.invM, p.eps, m, v, i);
+      double m, var, i;
+      tape_stats(sums[(long)g * 2 * p.C + c + j], sums[(long)g * 2 * p.C + p.C + c + j], p.Mt, p.invM, p.eps, m, var, i);
       mu[j] = m; is[j] = i; bt[j] = (double)p.beta[c + j];
       if (blockIdx.x == 0 && g == 0 && rl == 0) tape_publish(p, sums, c + j);
     }
   }
-  const long base = (long)g * p.Mg;
-  const int r0 = blockIdx.x * rpb, r1 = min(p.Mg, r0 + rpb);
   for (int rb = r0 + rl; rb < r1; rb += APPLY_RB * R) {
-    f4 v[APPLY_RB];
+    f4 w[APPLY_RB];
 #pragma unroll
-    for (int i = 0; i < APPLY_RB; ++i) {
-      const int r = rb + i * R;
-      v[i] = on && r < r1 ? *reinterpret_cast<const f4*>(p.z + (base + r) * p.C + c) : f4{0.f, 0.f, 0.f, 0.f};
-    }
+    for (int i = 0; i < APPLY_RB; ++i) w[i] = v[i];
+    if (rb + APPLY_RB * R < r1) load(rb + APPLY_RB * R);
 #pragma unroll
     for (int i = 0; i < APPLY_RB; ++i) {
       const int r = rb + i * R;
@@ -286,7 +293,7 @@ __global__ void __launch_bounds__(256) tape_fwd_apply_kernel(const TapeFwd p, co
       const long row = base + r;
       d4 u;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = fma((double)v[i][j] - mu[j], is[j], bt[j]);
+      for (int j = 0; j < 4; ++j) u[j] = fma((double)w[i][j] - mu[j], is[j], bt[j]);
       f4 y;
       int packed;
       float s;
@@ -434,7 +441,7 @@ struct TapeBwd {
   const int8_t* codes;
   const float *scales, *save_invstd, *beta, *dy;
   int dycs, dyco;
-  double Mt;
+  double invM;               // 1 / rows per group over all replicas
   float *dz, *dbeta, *absmax;
   int acc;
 };
@@ -457,11 +464,26 @@ __global__ void __launch_bounds__(256) tape_bwd_apply_kernel(const TapeBwd p, co
   const int rl = threadIdx.x / nl, q = threadIdx.x - rl * nl, b = q / L, c = 4 * q, g = blockIdx.y;
   float mx = 0.f;
   if (rl < R && c < p.C) {
+    const long base = (long)g * p.Mg;
+    const int r0 = blockIdx.x * rpb, r1 = min(p.Mg, r0 + rpb);
+    f4 v[APPLY_RB];
+    int cd[APPLY_RB];
+    float s[APPLY_RB];
+    auto load = [&](int rb) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < APPLY_RB; ++i) {
+        const long row = base + min(rb + i * R, r1 - 1);
+        v[i] = *reinterpret_cast<const f4*>(p.dy + row * p.dycs + p.dyco + c);
+        cd[i] = *reinterpret_cast<const int*>(p.codes + row * p.C + c);
+        s[i] = p.scales[row * p.NB + b];
+      }
+    };
+    load(r0 + rl);                     // in flight while the means are evaluated
     f4 m0, m1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      m0[j] = (float)(gsums[(long)g * 2 * p.C + c + j] / p.Mt);
-      m1[j] = (float)(gsums[(long)g * 2 * p.C + p.C + c + j] / p.Mt);
+      m0[j] = (float)(gsums[(long)g * 2 * p.C + c + j] * p.invM);
+      m1[j] = (float)(gsums[(long)g * 2 * p.C + p.C + c + j] * p.invM);
     }
     if (p.dbeta && blockIdx.x == 0 && g == 0 && rl == 0)
 #pragma unroll
@@ -472,27 +494,15 @@ __global__ void __launch_bounds__(256) tape_bwd_apply_kernel(const TapeBwd p, co
       }
     const f4 is = *reinterpret_cast<const f4*>(p.save_invstd + (long)g * p.C + c);
     const f4 bt = *reinterpret_cast<const f4*>(p.beta + c);
-    const long base = (long)g * p.Mg;
-    const int r0 = blockIdx.x * rpb, r1 = min(p.Mg, r0 + rpb);
     for (int rb = r0 + rl; rb < r1; rb += APPLY_RB * R) {
-      f4 v[APPLY_RB];
-      int cd[APPLY_RB];
-      float s[APPLY_RB];
+      f4 o[APPLY_RB];
 #pragma unroll
-      for (int i = 0; i < APPLY_RB; ++i) {
-        const long row = base + min(rb + i * R, r1 - 1);
-        v[i] = *reinterpret_cast<const f4*>(p.dy + row * p.dycs + p.dyco + c);
-        cd[i] = *reinterpret_cast<const int*>(p.codes + row * p.C + c);
-        s[i] = p.scales[row * p.NB + b];
-      }
+      for (int i = 0; i < APPLY_RB; ++i)
+        if (rb + i * R < r1) tape_dz_row(v[i], cd[i], s[i], bt, m0, m1, is, o[i], mx);
+      if (rb + APPLY_RB * R < r1) load(rb + APPLY_RB * R);
 #pragma unroll
-      for (int i = 0; i < APPLY_RB; ++i) {
-        const int r = rb + i * R;
-        if (r >= r1) break;
-        f4 o;
-        tape_dz_row(v[i], cd[i], s[i], bt, m0, m1, is, o, mx);
-        tde_st(reinterpret_cast<f4*>(p.dz + (base + r) * p.C + c), o);
-      }
+      for (int i = 0; i < APPLY_RB; ++i)
+        if (rb + i * R < r1) tde_st(reinterpret_cast<f4*>(p.dz + (base + rb + i * R) * p.C + c), o[i]);
     }
   }
   block_absmax_to(mx, p.absmax);
@@ -562,8 +572,8 @@ __global__ void __launch_bounds__(SMALL_NT) tape_bwd_small_kernel(const TapeBwd 
       f4 m0, m1;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        m0[j] = (float)(tot[l][j] / p.Mt);
-        m1[j] = (float)(tot[l][4 + j] / p.Mt);
+        m0[j] = (float)(tot[l][j] * p.invM);
+        m1[j] = (float)(tot[l][4 + j] * p.invM);
         db[j] += (float)tot[l][j];
       }
       const f4 is = *reinterpret_cast<const f4*>(p.save_invstd + (long)g * p.C + c);
@@ -759,7 +769,7 @@ int tde_tape8_bn_bwd_from_sums(int M, int C, int groups, long M_total, const int
                 global_sums && local_sums && dz && tde_aligned16(dz));
   const TapePlan t = tape_plan(M, C, groups);
   const TapeBwd p{M / groups, C, t.NB, groups, codes, scales, save_invstd, beta, dy, dy_cstride, dy_coff,
-                  (double)M_total, dz, dbeta, dz_absmax, accumulate_dbeta};
+                  1.0 / (double)M_total, dz, dbeta, dz_absmax, accumulate_dbeta};
   tape_bwd_apply_launch(t, p, global_sums, local_sums, static_cast<hipStream_t>(stream));
   return tde_launch_status();
 }
@@ -774,7 +784,7 @@ int tde_tape8_bn_bwd(int M, int C, int groups, const int8_t* codes, const float*
   hipStream_t st = static_cast<hipStream_t>(stream);
   const TapePlan t = tape_plan(M, C, groups);
   const TapeBwd p{M / groups, C, t.NB, groups, codes, scales, save_invstd, beta, dy, dy_cstride, dy_coff,
-                  (double)(M / groups), dz, dbeta, dz_absmax, accumulate_dbeta};
+                  1.0 / (double)(M / groups), dz, dbeta, dz_absmax, accumulate_dbeta};
   if (tape_small(p.Mg, t.L)) {
 #define F(LL)                                                                                                       \
   if (p.Mg <= 2 * SMALL_NT / LL)                                                                                    \
