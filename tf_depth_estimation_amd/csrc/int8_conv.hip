@@ -204,24 +204,42 @@ struct Q8Frag<32> {
   static __device__ __forceinline__ i4 mfma(T a, T b, i4 c) { return __builtin_amdgcn_mfma_i32_16x16x32_i8(a, b, c, 0, 0, 0); }
 };
 
-// bias, scale, ReLU and store of one tile: four channels k.. of the pixel at py
-__device__ __forceinline__ void q8_store(const Q8Conv& p, float* py, int k, const f4& acc) {
-  if (k >= p.K) return;
-  const f4 ws = *reinterpret_cast<const f4*>(p.ws + k);       // (scales are padded to Kp)
-  f4 o;
+// scales and biases of a lane's channels (k0 + 16 a ..+3), loaded together before the stores
+template <int TM>
+struct Q8Epi {
+  f4 ws[TM], bs[TM];
+  __device__ __forceinline__ Q8Epi(const Q8Conv& p, int k0) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float v = fmaf(acc[e], ws[e], p.bias && k + e < p.K ? p.bias[k + e] : 0.f);
-    o[e] = p.relu && v < 0.f ? 0.f : v;
-  }
-  if (p.vec && k + 3 < p.K) {
-    tde_st(reinterpret_cast<f4*>(py + k), o);
-  } else {
+    for (int a = 0; a < TM; ++a) {
+      const int k = k0 + 16 * a;
+      ws[a] = bs[a] = f4{0.f, 0.f, 0.f, 0.f};
+      if (k < p.K) {
+        ws[a] = *reinterpret_cast<const f4*>(p.ws + k);       // (scales are padded to Kp)
+        if (p.bias)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (k + e < p.K) py[k + e] = o[e];
+          for (int e = 0; e < 4; ++e) bs[a][e] = p.bias[min(k + e, p.K - 1)];
+      }
+    }
   }
-}
+  // scale, bias, ReLU and store of tile a: four channels of the pixel at py
+  __device__ __forceinline__ void store(const Q8Conv& p, float* py, int k0, int a, const f4& acc) const {
+    const int k = k0 + 16 * a;
+    if (k >= p.K) return;
+    f4 o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float v = fmaf(acc[e], ws[a][e], bs[a][e]);
+      o[e] = p.relu && v < 0.f ? 0.f : v;
+    }
+    if (p.vec && k + 3 < p.K) {
+      tde_st(reinterpret_cast<f4*>(py + k), o);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (k + e < p.K) py[k + e] = o[e];
+    }
+  }
+};
 __device__ __forceinline__ float* q8_out(const Q8Conv& p, const Q8Class& cl, int n, int i, int j) {
   return p.y + (((long)n * p.OH + i * p.os + cl.py) * p.OW + j * p.os + cl.px) * p.ycs + p.yco;
 }
@@ -306,6 +324,7 @@ __global__ void __launch_bounds__(64 * WK) q8_split_kernel(const Q8Conv p) {
     for (int a = 0; a < TM; ++a)
 #pragma unroll
       for (int b = 0; b < TN; ++b) acc[a][b] += red[(w * TM * TN + a * TN + b) * 64 + lane];
+  const Q8Epi<TM> epi(p, n0 + 4 * kq);
 #pragma unroll
   for (int b = 0; b < TN; ++b) {
     const int m = m0 + 16 * b + r16;
@@ -313,7 +332,7 @@ __global__ void __launch_bounds__(64 * WK) q8_split_kernel(const Q8Conv p) {
     const int hw = cl.GH * cl.GW, n = m / hw, r = m - n * hw, i = r / cl.GW, j = r - i * cl.GW;
     float* py = q8_out(p, cl, n, i, j);
 #pragma unroll
-    for (int a = 0; a < TM; ++a) q8_store(p, py, n0 + 16 * a + 4 * kq, acc[a][b]);
+    for (int a = 0; a < TM; ++a) epi.store(p, py, n0 + 4 * kq, a, acc[a][b]);
   }
 }
 
@@ -504,13 +523,14 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
 #pragma unroll
         for (int b = 0; b < TN; ++b) acc[a][b] += red[(w * TM * TN + a * TN + b) * 64 + lane];
   }
+  const Q8Epi<TM> epi(p, n0 + 4 * kq);
 #pragma unroll
   for (int b = 0; b < TN; ++b) {
     const int q = 16 * (wp * TN + b) + r16, i = i0 + q / tl.TW, j = j0 + q % tl.TW;
     if (i >= cl.GH || j >= cl.GW) continue;
     float* py = q8_out(p, cl, n, i, j);
 #pragma unroll
-    for (int a = 0; a < TM; ++a) q8_store(p, py, n0 + 16 * a + 4 * kq, acc[a][b]);
+    for (int a = 0; a < TM; ++a) epi.store(p, py, n0 + 4 * kq, a, acc[a][b]);
   }
 }
 
@@ -523,7 +543,14 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
 // tiles read 128 bytes a clock for the same products and take 65 us, and serve where the large ones leave CUs idle.
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef __attribute__((address_space(1))) void* gbl_ptr_t;
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// this wave's LDS reads are done (written as a builtin, so that the compiler knows and waits for none of them again), then
+// the barrier
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);      // lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 template <int N>
 __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
@@ -560,42 +587,61 @@ __global__ void __launch_bounds__(64 * WC * WP) q8_gemm_kernel(const Q8Conv p, i
 
   const int lofs = r16 * 64 + ((kq ^ ((r16 >> 1) & 3)) << 4);
   const int steps = p.Cp / 64, last = steps - 1;
-  auto compute = [&](int slot) __attribute__((always_inline)) {
+  struct Frag {
+    i4 a[TM], b[TN];
+  };
+  auto read = [&](Frag& f, int slot) __attribute__((always_inline)) {
     const char* base = q8_lds + slot * SLOT + lofs;
-    i4 fa[TM], fb[TN];
 #pragma unroll
-    for (int b = 0; b < TN; ++b) fb[b] = *reinterpret_cast<const i4*>(base + BC * 64 + (wp * TN + b) * 1024);
+    for (int b = 0; b < TN; ++b) f.b[b] = *reinterpret_cast<const i4*>(base + BC * 64 + (wp * TN + b) * 1024);
 #pragma unroll
-    for (int a = 0; a < TM; ++a) fa[a] = *reinterpret_cast<const i4*>(base + (wc * TM + a) * 1024);
+    for (int a = 0; a < TM; ++a) f.a[a] = *reinterpret_cast<const i4*>(base + (wc * TM + a) * 1024);
+  };
+  auto next = [](int slot) __attribute__((always_inline)) { return slot == 2 ? 0 : slot + 1; };
+  // step s: its fragments are in registers; those of step s + 1 are read under its products, step s + 3 replaces it in LDS
+  auto step = [&](int s, int slot, const Frag& f, Frag& fn) __attribute__((always_inline)) {
+    vm_wait<DI>();        // this wave's part of step s + 1 has landed (step s + 2 may still fly)
+    lds_barrier();        // everybody's has, and everybody has read step s
+    dma(min(s + 3, last), slot);
+    read(fn, next(slot));
+    __builtin_amdgcn_sched_barrier(0);      // (left alone, the scheduler puts the reads behind the products)
 #pragma unroll
     for (int a = 0; a < TM; ++a)
 #pragma unroll
-      for (int b = 0; b < TN; ++b) acc[a][b] = Q8Frag<64>::mfma(fa[a], fb[b], acc[a][b]);
+      for (int b = 0; b < TN; ++b) acc[a][b] = Q8Frag<64>::mfma(f.a[a], f.b[b], acc[a][b]);
   };
   dma(0, 0);
   dma(min(1, last), 1);
+  dma(min(2, last), 2);
+  Frag f0, f1;
+  vm_wait<2 * DI>();
+  lds_barrier();
+  read(f0, 0);
   int slot = 0;
-  for (int s = 0; s < steps; ++s) {
-    vm_wait<DI>();        // this wave's part of step s has landed (step s + 1 may still fly)
-    lds_barrier();        // everybody's has, and everybody is done with the slot of step s - 1
-    dma(min(s + 2, last), slot == 0 ? 2 : slot - 1);
-    compute(slot);
-    slot = slot == 2 ? 0 : slot + 1;
+  for (int s = 0; s < steps; s += 2) {
+    step(s, slot, f0, f1);
+    slot = next(slot);
+    if (s + 1 < steps) step(s + 1, slot, f1, f0);
+    slot = next(slot);
   }
   vm_wait<0>();           // no DMA may outlive the block's LDS
 
+  const int k0 = n0 + wc * TM * 16 + 4 * kq;
+  const Q8Epi<TM> epi(p, k0);
+  float xs[TN];
+#pragma unroll
+  for (int b = 0; b < TN; ++b) xs[b] = p.xs[min(m0 + (wp * TN + b) * 16 + r16, M)];
 #pragma unroll
   for (int b = 0; b < TN; ++b) {
     const int m = m0 + (wp * TN + b) * 16 + r16;
     if (m >= M) continue;
-    const float xs = p.xs[m];
     float* py = p.y + (long)m * p.ycs + p.yco;
 #pragma unroll
     for (int a = 0; a < TM; ++a) {
       f4 v;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = (float)acc[a][b][j] * xs;
-      q8_store(p, py, n0 + (wc * TM + a) * 16 + 4 * kq, v);
+      for (int j = 0; j < 4; ++j) v[j] = (float)acc[a][b][j] * xs[b];
+      epi.store(p, py, k0, a, v);
     }
   }
 }
