@@ -1,6 +1,6 @@
 """Inference-path measurement: batch_prediction.py's disp_net(is_training=False)
-per-image latency at 224x224 batch 1, plus batched throughput, for the folded-BN graph predictor and the
-unfolded (conv -> BN(moving) -> ReLU) path, graph and eager.  Prints one JSON line.
+per-image latency at 224x224 batch 1, plus batched throughput, for the folded-BN graph predictor (fp32 and 8-bit) and
+the unfolded (conv -> BN(moving) -> ReLU) path, graph and eager.  Prints one JSON line.
 
     python scripts/infer_bench.py [--iters 200] [--warmup 20]
 """
@@ -44,17 +44,24 @@ def main():
     _lib.check(lib.tde_set_conv_math(_lib.CONV_MATH[args.math]))
     rows = []
     for net, H, W, B in [("disp_net", 224, 224, 1), ("disp_net", 192, 256, 8), ("disp_net", 192, 256, 64)]:
-        for fold, graph in [(True, True), (False, True), (True, False)]:
+        ref = None
+        for fold, graph, int8 in [(True, True, False), (True, True, True), (False, True, False), (True, False, False)]:
             variables.get_store().reset(seed=1)
             _api.clear_programs()
-            pred = batch_prediction.Predictor(net, H, W, batch=B, fold_bn=fold, graph=graph)
-            x = torch.rand((B, H, W, 3), device="cuda") - 0.5
+            pred = batch_prediction.Predictor(net, H, W, batch=B, fold_bn=fold, graph=graph, int8=int8)
+            x = torch.rand((B, H, W, 3), generator=torch.Generator().manual_seed(1)).cuda() - 0.5
             iters = args.iters if B == 1 else max(20, args.iters // 4)
             s = timed(pred, x, iters, args.warmup)
             f = flops(pred.prog, B)
             rows.append({"net": net, "HxW": f"{H}x{W}", "batch": B, "fold_bn": fold, "hip_graph": graph,
                          "ms_per_call": round(s * 1e3, 4), "images_per_s": round(B / s, 1),
                          "conv_tflops": round(f / s / 1e12, 2)})
+            if int8:      # (random-init weights: what the 8-bit rounding does to the maps of this network)
+                outs = pred(x)
+                rows[-1].update(int8=True, mean_abs_vs_fp32_over_mean=[round(float((o - r).abs().mean() / r.abs().mean()), 5)
+                                                                       for o, r in zip(outs, ref)])
+            elif ref is None:
+                ref = [o.clone() for o in pred(x)]
             print(json.dumps(rows[-1]), file=sys.stderr, flush=True)
     # the whole loop body of batch_prediction.py:58-75 on the GPU: INTER_AREA of a decoded 480x640 uint8 image into
     # the 224x224 input, the folded-BN graph, INTER_CUBIC of disp1 to 240x720 and bilateralFilter(9, 75, 75); and

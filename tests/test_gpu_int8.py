@@ -329,6 +329,78 @@ def test_tape_of_bad_values():
     assert np.isnan(val[:, :64]).all() and np.isfinite(val[:, 64:]).all()
 
 
+# ---------------------------------------------------------------- offsets past 32 bits
+def test_offsets_past_32_bits_in_views():
+    """Five pixels 2^29 floats apart: the last one's offset passes 2^31."""
+    step, C, K = 1 << 29, 20, 12
+    big = torch.empty(4 * step + 64, device="cuda")
+    x, w, b = conv_inputs(1, 1, 5, C, K, 1, False)
+    x = x[0, 0]
+    xv = big.as_strided((5, C), (step, 1))
+    xv.copy_(dev(x))
+    assert torch.equal(int8.quantize_rows(xv).codes, int8.quantize_rows(dev(x)).codes)
+    conv = int8.Conv8(dev(w), dev(b))
+    y = conv(dev(x))
+    yv = big.as_strided((5, K), (step, 1), 32)
+    conv(xv, out=yv)
+    assert torch.equal(yv, y)
+    z, beta, r = tape_data(5, C)
+    _, tape = int8.bn_relu_forward(dev(z), dev(beta), out=xv)
+    y2, tape2 = int8.bn_relu_forward(dev(z), dev(beta))
+    assert torch.equal(xv, y2) and torch.equal(tape.codes, tape2.codes)
+    tape.restore(out=xv)
+    assert torch.equal(xv, tape.restore())
+    dy = dev(r.standard_normal((5, C)).astype(np.float32))
+    xv.copy_(dy)
+    for a, c in zip(int8.bn_relu_backward(tape, dev(beta), xv), int8.bn_relu_backward(tape, dev(beta), dy)):
+        assert torch.equal(a, c)
+
+
+def test_more_than_2_31_codes():
+    """Tensors whose code count passes 2^31: the last rows and pixels against small problems that hold only them."""
+    C, K = 64, 16
+    r = rng(12)
+    w = (r.uniform(-1, 1, (3, 3, C, K)) * 0.1).astype(np.float32)
+    conv = int8.Conv8(dev(w), None, relu=False)
+    side = 5800
+    x = torch.zeros(1, side, side, C, device="cuda")
+    patch = torch.from_numpy(r.standard_normal((12, 12, C)).astype(np.float32)).cuda()
+    x[0, -12:, -12:] = patch
+    y = conv(x)
+    small = torch.zeros(1, 40, 40, C, device="cuda")
+    small[0, -12:, -12:] = patch
+    ys = conv(small)
+    # (the corner's outputs read the same pixels; tiles and their sums over taps differ)
+    assert float((y[0, -13:, -13:] - ys[0, -13:, -13:]).abs().max()) <= 1e-5 * float(ys.abs().max())
+    assert not bool(y[0, :-13].any()) and not bool(y[0, -13:, :-13].any())
+    del y, small
+    one = int8.Conv8(dev(w[:1, :1]), None, relu=False)
+    rows = x.view(-1, C)
+    yt = one(rows)
+    assert torch.equal(yt[-12:], one(rows[-12:].clone()))
+    del x, rows, yt
+    M, C = (1 << 21) + 3, 1024
+    z = torch.randn(M, C, device="cuda")
+    beta = torch.zeros(C, device="cuda")
+    y, tape = int8.bn_relu_forward(z, beta)
+    mean = torch.stack([zc.double().sum(0) for zc in z.split(1 << 18)]).sum(0) / M
+    ref = (z[-3:].double() - mean) * tape.invstd[0].double()
+    assert float((y[-3:] - ref.clamp(min=0)).abs().max()) <= 1e-5
+    del y
+    tail = tape.restore(relu=False)[-3:]
+    step = tape.scales[-3:].double().repeat_interleave(64, 1)
+    assert bool(((tail.double() - ref).abs() <= 0.51 * step).all())
+    dz, db = int8.bn_relu_backward(tape, beta, z)
+    g = torch.where(tape.codes[-3:] >= 0, z[-3:], torch.zeros_like(z[-3:])).double()
+    assert float((db.double() - torch.stack([torch.where(c >= 0, v, torch.zeros_like(v)).double().sum(0) for c, v in zip(
+        tape.codes.split(1 << 18), z.split(1 << 18))]).sum(0)).abs().max()) <= 1e-6 * M
+    m0 = db.double() / M
+    m1 = torch.stack([(torch.where(c >= 0, v, torch.zeros_like(v)) * t).double().sum(0) for c, v, t in zip(
+        tape.codes.split(1 << 18), z.split(1 << 18), tape.restore(relu=False).split(1 << 18))]).sum(0) / M
+    want = tape.invstd[0].double() * (g - m0 - tail.double() * m1)
+    assert float((dz[-3:].double() - want).abs().max()) <= 1e-5
+
+
 # ---------------------------------------------------------------- graphs and streams
 def test_captured_and_other_streams():
     """The operators together, captured once and replayed with new inputs between eager work, and on a stream of their

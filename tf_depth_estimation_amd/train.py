@@ -305,7 +305,7 @@ class Trainer:
         its 64 channels).  Call before capture()."""
         if self.graphs is not None or getattr(self, "ov_seq", None) is not None:
             raise ValueError("enable_tape8 before capture(): the captured step holds the fp32 tape's buffers")
-        for run in getattr(self, "runs", {"": getattr(self, "run", None)}).values():
+        for run in (self.runs.values() if hasattr(self, "runs") else [self.run]):
             run.enable_tape8()
         return self
 
