@@ -10,6 +10,8 @@
 // tile, loaded by the lane that needs it, and the result leaves as one 16-byte store.
 #include "tde_common.h"
 
+#include "split_math.h"      // FDiv: division by a launch constant
+
 namespace {
 
 typedef int i4 __attribute__((ext_vector_type(4)));
@@ -252,7 +254,7 @@ template <int TM, int TN, int KC, int WK, int U>
 __global__ void __launch_bounds__(64 * WK) q8_split_kernel(const Q8Conv p) {
   using F = typename Q8Frag<KC>::T;
   __shared__ f4 red[(WK - 1) * TM * TN * 64];
-  const int lane = threadIdx.x & 63, wk = threadIdx.x >> 6, r16 = lane & 15, kq = lane >> 4;
+  const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kq = lane >> 4;
   const Q8Class cl = q8_class(p, blockIdx.z);
   const int m0 = blockIdx.x * 16 * TN, n0 = blockIdx.y * 16 * TM;
   const long zero_row = (long)p.N * p.H * p.W;
@@ -346,7 +348,9 @@ __global__ void __launch_bounds__(64 * WK) q8_split_kernel(const Q8Conv p) {
 // matrix unit.  (The second launch bound keeps the products out of the accumulator file: with it, 2 moves per result and
 // step cost more than the products.)
 struct Q8Tile {
-  int TW, tx, ty, cb;        // tile width, tiles per row and column of the class grid, channel bytes per patch fill
+  int lw, tx, ty, cb;        // log2 of the tile width, tiles per row and column of the class grid, channel bytes per patch fill
+  int PH, PW;                // patch rows and columns (of the class with the most taps)
+  FDiv fPW, fnq, fnq1;       // by PW, by the 16-byte pieces of a pixel in a fill and in the last one
 };
 
 template <int TM, int TN, int KC, bool ONE, int WC, int WP, int WK>
@@ -360,10 +364,10 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
   const Q8Class cl = q8_class(p, blockIdx.z);
   const int per = tl.tx * tl.ty;
   const int n = blockIdx.x / per, rem = blockIdx.x - n * per, tyi = rem / tl.tx, txi = rem - tyi * tl.tx;
-  const int TH = BP / tl.TW, i0 = tyi * TH, j0 = txi * tl.TW;
+  const int TW = 1 << tl.lw, i0 = tyi * (BP >> tl.lw), j0 = txi * TW;
   if (i0 >= cl.GH || j0 >= cl.GW) return;                   // (tiles are counted for the largest class)
   const int n0 = (blockIdx.y * WC + wc) * 16 * TM;
-  const int PH = (TH - 1) * p.is + cl.nty, PW = (tl.TW - 1) * p.is + cl.ntx, NP = PH * PW;
+  const int PW = tl.PW, NP = tl.PH * PW;
   const int back = p.dir < 0;
   const int oy = i0 * p.is + cl.iy0 - (back ? cl.nty - 1 : 0), ox = j0 * p.is + cl.ix0 - (back ? cl.ntx - 1 : 0);
   const int RB = tl.cb + HEAD;                              // bytes of a patch row
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
   int prow[TN];                                             // this lane's pixels in the patch (bytes), at tap offset 0
 #pragma unroll
   for (int b = 0; b < TN; ++b) {
-    const int q = 16 * (wp * TN + b) + r16, i = q / tl.TW, j = q - i * tl.TW;
+    const int q = 16 * (wp * TN + b) + r16, i = q >> tl.lw, j = q & (TW - 1);
     prow[b] = (i * PW + j) * p.is * RB;
   }
   const int kofs = HEAD + kq * (KC / 4);                    // this lane's k-quarter in a row
@@ -391,19 +395,22 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
   for (int c0 = 0; c0 < p.Cp && taps > 0; c0 += tl.cb) {
     const int cbytes = min(tl.cb, p.Cp - c0), nq = cbytes / 16, total = NP * nq;
     if (c0 > 0) __syncthreads();                            // the last fill's fragments have been read
-    for (int base = tid; base < total; base += 4 * NT) {
-      i4 v[4];
-      int dst[4];
-      float sc[4];
+    const FDiv fnq = c0 + tl.cb < p.Cp ? tl.fnq : tl.fnq1;
+    constexpr int U = 4;                                    // pieces in flight per lane (8: 169 registers, two waves a SIMD)
+    for (int base = tid; base < total; base += U * NT) {
+      i4 v[U];
+      int dst[U];
+      float sc[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < U; ++u) {
         const int idx = base + u * NT;
         v[u] = i4{0, 0, 0, 0};
-        sc[u] = 0.f;
+        sc[u] = -1.f;                                       // (a scale is never negative: not a row's first piece)
         dst[u] = -1;
         if (idx < total) {
-          const int pp = idx / nq, c = idx - pp * nq, y = pp / PW, x = pp - y * PW, iy = oy + y, ix = ox + x;
+          const int pp = fdiv(idx, fnq), c = idx - pp * nq, y = fdiv(pp, tl.fPW), x = pp - y * PW, iy = oy + y, ix = ox + x;
           dst[u] = pp * RB + HEAD + 16 * c;
+          if (c == 0) sc[u] = 0.f;
           if ((unsigned)iy < (unsigned)p.H && (unsigned)ix < (unsigned)p.W) {
             const long pix = ((long)n * p.H + iy) * p.W + ix;
             v[u] = *reinterpret_cast<const i4*>(p.x + pix * p.Cp + c0 + 16 * c);
@@ -412,7 +419,7 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
         }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < U; ++u)
         if (dst[u] >= 0) {
           if (KC == 64) {
             *reinterpret_cast<i4*>(q8_lds + dst[u]) = v[u];
@@ -421,7 +428,7 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
             d[0] = int2{v[u][0], v[u][1]};
             d[1] = int2{v[u][2], v[u][3]};
           }
-          if ((base + u * NT) % nq == 0) *reinterpret_cast<float*>(q8_lds + dst[u] - HEAD) = sc[u];
+          if (!(sc[u] < 0.f)) *reinterpret_cast<float*>(q8_lds + dst[u] - HEAD) = sc[u];
         }
     }
     __syncthreads();
@@ -526,7 +533,7 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
   const Q8Epi<TM> epi(p, n0 + 4 * kq);
 #pragma unroll
   for (int b = 0; b < TN; ++b) {
-    const int q = 16 * (wp * TN + b) + r16, i = i0 + q / tl.TW, j = j0 + q % tl.TW;
+    const int q = 16 * (wp * TN + b) + r16, i = i0 + (q >> tl.lw), j = j0 + (q & (TW - 1));
     if (i >= cl.GH || j >= cl.GW) continue;
     float* py = q8_out(p, cl, n, i, j);
 #pragma unroll
@@ -658,25 +665,25 @@ void q8_split_launch(const Q8Conv& p, long Mmax, int classes, hipStream_t st) {
 
 constexpr int Q8_LDS = 64 * 1024;      // patch bytes of a halo block: two blocks fit a CU's 160 KB
 
-// patch pixels of a TH x TW tile (the class with the most taps)
-inline int q8_patch(const Q8Conv& p, int TH, int TW) {
-  const int nty = p.deconv ? (p.KH + p.os - 1) / p.os : p.KH, ntx = p.deconv ? (p.KW + p.os - 1) / p.os : p.KW;
-  return ((TH - 1) * p.is + nty) * ((TW - 1) * p.is + ntx);
-}
-
 template <int TM, int TN, int WC, int WP, int WK>
 bool q8_halo_launch(const Q8Conv& p, int GH, int GW, int classes, hipStream_t st) {
   constexpr int BP = 16 * TN * WP, BC = 16 * TM * WC, NT = 64 * WC * WP * WK;
   constexpr int RED = (WK - 1) * WC * WP * TM * TN * 1024;
   static_assert(RED <= Q8_LDS, "partial sums fit the patch's LDS");
   Q8Tile t;
-  t.TW = GW > 8 ? 16 : (GW > 4 ? 8 : 4);
-  const int TH = BP / t.TW, NP = q8_patch(p, TH, t.TW), kc = p.Cp % 64 == 0 ? 64 : 32;
-  t.tx = tde_cdiv(GW, t.TW); t.ty = tde_cdiv(GH, TH);
-  t.cb = Q8_LDS / NP - kc / 4;
+  t.lw = GW > 8 ? 4 : (GW > 4 ? 3 : 2);
+  const int TW = 1 << t.lw, TH = BP / TW, kc = p.Cp % 64 == 0 ? 64 : 32;
+  t.PH = (TH - 1) * p.is + (p.KH + p.kst - 1) / p.kst;
+  t.PW = (TW - 1) * p.is + (p.KW + p.kst - 1) / p.kst;
+  const long NP = (long)t.PH * t.PW;
+  t.tx = tde_cdiv(GW, TW); t.ty = tde_cdiv(GH, TH);
+  t.cb = (int)(Q8_LDS / NP) - kc / 4;
   t.cb = t.cb >= p.Cp ? p.Cp : t.cb / kc * kc;
   if (t.cb < kc) return false;
-  const int patch = NP * (t.cb + kc / 4), lds = patch > RED ? patch : RED;
+  t.fPW = make_fdiv(t.PW);
+  t.fnq = make_fdiv(t.cb / 16);
+  t.fnq1 = make_fdiv((p.Cp - (p.Cp - 1) / t.cb * t.cb) / 16);
+  const int patch = (int)NP * (t.cb + kc / 4), lds = patch > RED ? patch : RED;
   const long blocks = (long)p.N * t.tx * t.ty;
   if (blocks * NT >= (1L << 32)) return false;
   const dim3 grid((unsigned)blocks, tde_cdiv(p.K, BC), classes);
