@@ -83,6 +83,8 @@ CONVS = [
     (4, 24, 32, 64, 32, 3, 2, True, True),
     (1, 10, 9, 16, 8, 3, 3, False, True),
     (1, 4, 5, 16, 8, 3, 3, True, True),
+    (1, 2, 2, 8, 1100, 3, 2, True, True),
+    (1, 3, 2, 12, 1030, 3, 1, False, False),
     (16, 40, 48, 32, 24, 3, 1, False, True),
     (16, 32, 48, 16, 130, 3, 1, False, True),
     (1, 32, 48, 1024, 40, 7, 1, False, True),     # a patch filled in several channel chunks

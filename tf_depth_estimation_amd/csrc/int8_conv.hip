@@ -126,34 +126,45 @@ __global__ void __launch_bounds__(256) q8_rows_kernel(long rows, int C, int Cp, 
   }
 }
 
-// ---- weights: one block per output channel (padding channels write zeros)
-__global__ void __launch_bounds__(256) q8_weights_kernel(int taps, int cin, int K, int Kp, int Cp, int layout,
-                                                         const float* w, int8_t* codes, float* scales) {
-  __shared__ unsigned sh[4];
-  const int k = blockIdx.x;
-  unsigned am = 0;
-  if (k < K)
-    for (int i = threadIdx.x; i < taps * cin; i += 256) {
-      const int t = i / cin, c = i - t * cin;
-      const float v = layout == 0 ? w[((long)t * cin + c) * K + k] : w[((long)t * K + k) * cin + c];
-      am = max(am, __float_as_uint(v) & 0x7fffffffu);
-    }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) am = max(am, (unsigned)__shfl_xor((int)am, o, 64));
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = am;
+// ---- weights: a block takes KB output channels (padding channels write zeros), 1024 / KB lanes each; lanes run along the
+// contiguous dimension of the layout (0: output channels, 1: input channels).  The maximum's atomics are on integers in
+// LDS: the order does not matter.  KB 16 for many channels (2048 x 2048: 19 us, 52 with one block a channel), 4 for few,
+// where blocks count for more than whole lines.
+template <int KB>
+__global__ void __launch_bounds__(1024) q8_weights_kernel(int taps, int cin, int K, int Kp, int Cp, int layout,
+                                                          const float* w, int8_t* codes, float* scales) {
+  constexpr int NL = 1024 / KB;
+  __shared__ unsigned mx[KB];
+  const int kk = layout == 0 ? threadIdx.x % KB : threadIdx.x / NL, rl = layout == 0 ? threadIdx.x / KB : threadIdx.x % NL;
+  const int k = blockIdx.x * KB + kk, rows = taps * cin;
+  if (threadIdx.x < KB) mx[threadIdx.x] = 0;
   __syncthreads();
-  am = max(max(sh[0], sh[1]), max(sh[2], sh[3]));
+  // element (tap t, input channel c) of this channel; the two layouts' strides
+  const long st = layout == 0 ? (long)cin * K : (long)K * cin, sc = layout == 0 ? K : 1;
+  const float* wk = w + (layout == 0 ? (long)k : (long)k * cin);
+  unsigned am = 0;
+  if (k < K) {
+#pragma unroll 4
+    for (int i = rl; i < rows; i += NL) {
+      const int t = i / cin, c = i - t * cin;
+      am = max(am, __float_as_uint(wk[t * st + c * sc]) & 0x7fffffffu);
+    }
+    atomicMax(&mx[kk], am);
+  }
+  __syncthreads();
+  am = mx[kk];
   const Q8Div d = q8_div(am);
-  for (int i = threadIdx.x; i < taps * Cp / 4; i += 256) {
-    const int t = 4 * i / Cp, c = 4 * i - t * Cp;
+  const int nq = Cp / 4, quads = taps * nq;
+#pragma unroll 2
+  for (int i = rl; i < quads; i += NL) {
+    const int t = i / nq, c = 4 * (i - t * nq);
     f4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (k < K && c + j < cin)
-        v[j] = layout == 0 ? w[((long)t * cin + c + j) * K + k] : w[((long)t * K + k) * cin + c + j];
+      if (k < K && c + j < cin) v[j] = wk[t * st + (c + j) * sc];
     *reinterpret_cast<int*>(codes + ((long)t * Kp + k) * Cp + c) = q8_code4(v, d);
   }
-  if (threadIdx.x == 0) scales[k] = q8_scale(am);
+  if (rl == 0) scales[k] = q8_scale(am);
 }
 
 // ---- the product.  One class of output pixels (a conv has one; a stride-s transposed conv s * s parities): output
@@ -804,8 +815,13 @@ int tde_q8_weights(int taps, int cin, int K, int layout, const float* w, int8_t*
   tde_clear_error();
   TDE_CHECK_ARG(tde_q8_weights_size(taps, cin, K) > 0 && taps <= 4096 && (layout == 0 || layout == 1) && w && codes &&
                 scales && tde_aligned16(codes));
-  hipLaunchKernelGGL(q8_weights_kernel, dim3(q8_cols(K)), dim3(256), 0, static_cast<hipStream_t>(stream), taps, cin, K,
-                     q8_cols(K), q8_row(cin), layout, w, codes, scales);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  if (K >= 1024)
+    hipLaunchKernelGGL(q8_weights_kernel<16>, dim3(q8_cols(K) / 16), dim3(1024), 0, st, taps, cin, K, q8_cols(K), q8_row(cin),
+                       layout, w, codes, scales);
+  else
+    hipLaunchKernelGGL(q8_weights_kernel<4>, dim3(q8_cols(K) / 4), dim3(1024), 0, st, taps, cin, K, q8_cols(K), q8_row(cin),
+                       layout, w, codes, scales);
   return tde_launch_status();
 }
 
