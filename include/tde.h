@@ -337,6 +337,15 @@ int tde_tape8_bn_fwd_from_sums(int M, int C, int groups, long M_total, const flo
  * gradients read it; relu 0: the coded pre-activation. */
 int tde_tape8_restore(int M, int C, const int8_t* codes, const float* scales, int relu, float* y, int y_cstride,
                       int y_coff, void* stream);
+/* n <= TDE_TAPE8_MULTI_MAX independent tde_tape8_restore calls (the layers of a network) in ONE launch; the views must be
+ * disjoint. */
+#define TDE_TAPE8_MULTI_MAX 16
+typedef struct {
+  int M, C;
+  const int8_t* codes; const float* scales;
+  float* y; int y_cstride, y_coff;
+} tde_tape8_restore_t;
+int tde_tape8_restore_multi(const tde_tape8_restore_t* jobs, int n, int relu, void* stream);
 /* Backward from the tape: g = dy where code >= 0 else 0, xhat = (code + 1/2) s - beta,
  * dz = invstd (g - mean g - xhat mean(g xhat)) (means over a group's rows), dbeta (+)= sum g; dz_absmax as tde_bn_bwd.
  * beta is the one of the forward. */

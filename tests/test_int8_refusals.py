@@ -129,6 +129,14 @@ def test_tape_arguments(p):
     assert bwd(M=1 << 20, nb=16) == -2
     assert lib.tde_tape8_restore(8, 4, p, p, 2, p, 4, 0, None) == -1
     assert lib.tde_tape8_restore(8, 4, p, p, 1, p, 4, 4, None) == -1
+    good = _lib.TapeRestore(8, 4, p.value, p.value, p.value, 4, 0)
+    for n, bad in ((0, good), (17, good), (1, _lib.TapeRestore(8, 6, p.value, p.value, p.value, 8, 0)),
+                   (2, _lib.TapeRestore(8, 4, p.value, p.value, odd.value, 4, 0)),
+                   (2, _lib.TapeRestore(8, 4, p.value, None, p.value, 4, 0))):
+        jobs = (_lib.TapeRestore * 17)(*([good] * 17))
+        jobs[max(n - 1, 0)] = bad
+        assert lib.tde_tape8_restore_multi(jobs, n, 1, None) == -1, n
+    assert lib.tde_tape8_restore_multi(None, 1, 1, None) == -1
     assert lib.tde_tape8_bn_fwd_from_sums(8, 4, 2, 3, p, p, p, 1e-3, 0.99, 1, None, None, p, p, p, 4, 0, p, p, None) == -1
     assert lib.tde_tape8_bn_bwd_sums(8, 4, 1, p, p, p, p, 4, 0, None, None, p, big, None) == -1
     assert lib.tde_tape8_bn_bwd_from_sums(8, 4, 1, 7, p, p, p, p, p, 4, 0, p, p, p, None, 0, None, None) == -1

@@ -65,7 +65,14 @@ class PoseGradArgs(ctypes.Structure):
                 ("dpose", P), ("hw", c_int), ("dpose_cstride", c_int), ("dpose_accumulate", c_int)]
 
 
+class TapeRestore(ctypes.Structure):
+    """Mirror of tde_tape8_restore_t (include/tde.h): one job of tde_tape8_restore_multi."""
+    _fields_ = [("M", c_int), ("C", c_int), ("codes", P), ("scales", P), ("y", P), ("y_cstride", c_int),
+                ("y_coff", c_int)]
+
+
 WARP_MULTI_MAX = 8      # TDE_WARP_MULTI_MAX
+TAPE8_MULTI_MAX = 16    # TDE_TAPE8_MULTI_MAX
 PYR_MULTI_MAX = 4       # TDE_PYR_MULTI_MAX
 
 
@@ -163,6 +170,7 @@ _SIGS = {
     "tde_tape8_bn_fwd_from_sums": (c_int, [c_int, c_int, c_int, ctypes.c_long, P, P, P, c_float, c_float, c_int, P, P,
                                            P, P, P, c_int, c_int, P, P, P]),
     "tde_tape8_restore": (c_int, [c_int, c_int, P, P, c_int, P, c_int, c_int, P]),
+    "tde_tape8_restore_multi": (c_int, [P, c_int, c_int, P]),
     "tde_tape8_bn_bwd": (c_int, [c_int, c_int, c_int, P, P, P, P, P, c_int, c_int, P, P, c_int, P, P, c_size_t, P]),
     "tde_tape8_bn_bwd_sums": (c_int, [c_int, c_int, c_int, P, P, P, P, c_int, c_int, P, P, P, c_size_t, P]),
     "tde_tape8_bn_bwd_from_sums": (c_int, [c_int, c_int, c_int, ctypes.c_long, P, P, P, P, P, c_int, c_int, P, P, P, P,

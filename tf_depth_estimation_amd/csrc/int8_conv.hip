@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256) q8_rows_kernel(long rows, int C, int Cp, 
         const int c = 4 * (l + i * L);
         v[t][i] = f4{0.f, 0.f, 0.f, 0.f};
         if (row < rows && c < C) {
-          if (VEC) {
+          if (VEC && (c + 3 < C || row + 1 < rows)) {      // (the last row's padding may lie behind the tensor)
             v[t][i] = *reinterpret_cast<const f4*>(px + c);
           } else {
 #pragma unroll

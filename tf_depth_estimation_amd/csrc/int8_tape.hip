@@ -403,22 +403,31 @@ __global__ void __launch_bounds__(SMALL_NT) tape_fwd_small_kernel(const TapeFwd 
     for (int j = 0; j < 4; ++j) { p.mm[c + j] = m0[j]; p.mv[c + j] = v0[j]; }
 }
 
-// ---- restore: the tape's values into a channel view
-template <int L>
-__global__ void __launch_bounds__(256) tape_restore_kernel(int M, int C, int NB, const int8_t* codes, const float* scales,
-                                                           int relu, float* y, int ycs, int yco, int rpb) {
-  const int nl = NB * L, R = 256 / nl;
-  const int rl = threadIdx.x / nl, q = threadIdx.x - rl * nl, c = 4 * q, b = q / L;
-  if (rl >= R || c >= C) return;
-  const long r0 = (long)blockIdx.x * rpb, r1 = min((long)M, r0 + rpb);
+// ---- restore: the tape's values into channel views, one job per layer.  A row is C / 4 lanes, 256 / (C / 4) rows a step,
+// eight rows in flight per lane.
+struct TapeRestore {
+  tde_tape8_restore_t job[TDE_TAPE8_MULTI_MAX];
+  int first[TDE_TAPE8_MULTI_MAX + 1];      // blocks of the jobs before this one
+  int rpb[TDE_TAPE8_MULTI_MAX];            // rows per block
+  int n, relu;
+};
+
+__global__ void __launch_bounds__(256) tape_restore_kernel(const TapeRestore p) {
+  int k = 0;
+  while (k + 1 < p.n && (int)blockIdx.x >= p.first[k + 1]) ++k;
+  const tde_tape8_restore_t jb = p.job[k];
+  const int nl = jb.C / 4, R = 256 / nl, NB = (jb.C + TDE_TAPE8_BLOCK - 1) / TDE_TAPE8_BLOCK;
+  const int rl = threadIdx.x / nl, q = threadIdx.x - rl * nl, c = 4 * q, b = c / TDE_TAPE8_BLOCK;
+  if (rl >= R) return;
+  const long r0 = (long)(blockIdx.x - p.first[k]) * p.rpb[k], r1 = min((long)jb.M, r0 + p.rpb[k]);
   for (long rb = r0 + rl; rb < r1; rb += 8 * R) {
     int cd[8];
     float s[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const long r = min(rb + i * R, r1 - 1);
-      cd[i] = *reinterpret_cast<const int*>(codes + r * C + c);
-      s[i] = scales[r * NB + b];
+      cd[i] = *reinterpret_cast<const int*>(jb.codes + r * jb.C + c);
+      s[i] = jb.scales[r * NB + b];
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -428,9 +437,9 @@ __global__ void __launch_bounds__(256) tape_restore_kernel(int M, int C, int NB,
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float v = tape_value(cd[i], j, s[i]);
-        o[j] = relu && v < 0.f ? 0.f : v;
+        o[j] = p.relu && v < 0.f ? 0.f : v;
       }
-      tde_st(reinterpret_cast<f4*>(y + r * ycs + yco + c), o);
+      tde_st(reinterpret_cast<f4*>(jb.y + r * jb.y_cstride + jb.y_coff + c), o);
     }
   }
 }
@@ -729,19 +738,28 @@ int tde_tape8_bn_fwd_from_sums(int M, int C, int groups, long M_total, const flo
   return tde_launch_status();
 }
 
+int tde_tape8_restore_multi(const tde_tape8_restore_t* jobs, int n, int relu, void* stream) {
+  tde_clear_error();
+  TDE_CHECK_ARG(jobs && n > 0 && n <= TDE_TAPE8_MULTI_MAX && (relu == 0 || relu == 1));
+  TapeRestore p{};
+  p.n = n; p.relu = relu;
+  for (int k = 0; k < n; ++k) {
+    const tde_tape8_restore_t& j = jobs[k];
+    TDE_CHECK_ARG(tape_shape_ok(j.M, j.C, 1) && tape_ok(j.codes, j.scales) && tape_view_ok(j.y, j.C, j.y_cstride, j.y_coff));
+    p.job[k] = j;
+    const int R = 256 / (j.C / 4);
+    const long want = ((long)j.M + 2047) / 2048;      // at most 2048 blocks a job, eight steps of its row lanes each
+    p.rpb[k] = (int)(want > 8 * R ? want : 8 * R);
+    p.first[k + 1] = p.first[k] + tde_cdiv(j.M, p.rpb[k]);
+  }
+  hipLaunchKernelGGL(tape_restore_kernel, dim3(p.first[n]), dim3(256), 0, static_cast<hipStream_t>(stream), p);
+  return tde_launch_status();
+}
+
 int tde_tape8_restore(int M, int C, const int8_t* codes, const float* scales, int relu, float* y, int y_cstride,
                       int y_coff, void* stream) {
-  tde_clear_error();
-  TDE_CHECK_ARG(tape_shape_ok(M, C, 1) && tape_ok(codes, scales) && (relu == 0 || relu == 1) &&
-                tape_view_ok(y, C, y_cstride, y_coff));
-  const TapePlan t = tape_plan(M, C, 1);
-  const int rpb = tape_apply_rows(M, C, t);
-#define F(LL)                                                                                                  \
-  hipLaunchKernelGGL(tape_restore_kernel<LL>, dim3(tde_cdiv(M, rpb)), dim3(256), 0, static_cast<hipStream_t>(stream), M, \
-                     C, t.NB, codes, scales, relu, y, y_cstride, y_coff, rpb)
-  TAPE_L(t.L, F)
-#undef F
-  return tde_launch_status();
+  const tde_tape8_restore_t job{M, C, codes, scales, y, y_cstride, y_coff};
+  return tde_tape8_restore_multi(&job, 1, relu, stream);
 }
 
 int tde_tape8_bn_bwd_sums(int M, int C, int groups, const int8_t* codes, const float* scales, const float* beta,

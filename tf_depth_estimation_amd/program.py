@@ -432,16 +432,17 @@ class NetProgram:
         return sh
 
     def _restore_tape8(self, run):
-        """The activations of run's forward into the shared buffers, in forward order: layer outputs from the tape,
-        resizes and copies from what is restored (or kept: head results) before them."""
+        """The activations of run's forward into the shared buffers: layer outputs from the tape (a launch per 16 layers),
+        then, in forward order, resizes and copies from what is restored or kept (head results)."""
         lib, st, N = _lib.load(), _lib.stream_ptr(), run.N
-        for i, op in enumerate(self.spec.ops):
-            if isinstance(op, ConvBN):
-                codes, scales = run.tape[i]
-                _lib.check(lib.tde_tape8_restore(N * op.dst.H * op.dst.W, op.K, ptr(codes), ptr(scales), 1,
-                                                 run.vptr(op.dst), op.dst.buf.cs, op.dst.coff, st),
-                           op.layer + " tape restore")
-            elif isinstance(op, (Resize, Copy)):
+        jobs = [_lib.TapeRestore(N * op.dst.H * op.dst.W, op.K, run.tape[i][0].data_ptr(), run.tape[i][1].data_ptr(),
+                                 run.vptr(op.dst).value, op.dst.buf.cs, op.dst.coff)
+                for i, op in enumerate(self.spec.ops) if isinstance(op, ConvBN)]
+        for k in range(0, len(jobs), _lib.TAPE8_MULTI_MAX):
+            part = jobs[k:k + _lib.TAPE8_MULTI_MAX]
+            _lib.check(lib.tde_tape8_restore_multi((_lib.TapeRestore * len(part))(*part), len(part), 1, st), "tape restore")
+        for op in self.spec.ops:
+            if isinstance(op, (Resize, Copy)):
                 self._place(run, op, st)
 
     def _place(self, run, op, st):
