@@ -8,8 +8,7 @@
 // accumulator with its pixel's scale.  The product is taken transposed (weights are the matrix instruction's rows,
 // pixels its columns): then a lane's four results are four channels of ONE pixel, so the scale is one register per
 // tile, loaded by the lane that needs it, and the result leaves as one 16-byte store.
-#include "tde_common.h"
-
+#include "int8_common.h"
 #include "split_math.h"      // FDiv: division by a launch constant
 
 namespace {
@@ -51,26 +50,27 @@ __device__ __noinline__ int q8_code_exact(float x, double a) {
   if (r < -a || (r == -a && (q & 1))) --q;
   return q;
 }
-// codes of four channels, packed
+// codes of four channels, packed.  (q + 128 as an unsigned byte, whose top bit is then turned.)
 __device__ __forceinline__ int q8_code4(const f4& x, const Q8Div& d) {
   f4 q;
-  bool near = false;
+  bool near = d.mode == 2;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float t = x[j] * d.inv;
     q[j] = rintf(t);
-    near |= fabsf(fabsf(t - q[j]) - 0.5f) < 5e-5f;
+    near |= fabsf(t - q[j]) > 0.49995f;
   }
-  int p = 0;
-  if (d.mode == 2 || (near && d.mode == 1)) {
+  if (near) {                          // (mode 0: t is 0 or, where x is not finite, NaN: never near)
+    int p = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) p |= (q8_code_exact(x[j], d.a) & 0xff) << (8 * j);
     return p;
   }
-  if (d.mode == 0) return 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) p |= ((int)q[j] & 0xff) << (8 * j);
-  return p;
+  unsigned p = put_byte<0>(q[0] + 128.f, 0);
+  p = put_byte<1>(q[1] + 128.f, p);
+  p = put_byte<2>(q[2] + 128.f, p);
+  p = put_byte<3>(q[3] + 128.f, p);
+  return d.mode == 0 ? 0 : (int)(p ^ 0x80808080u);
 }
 
 // ---- rows: L lanes per row (a power of two <= 64), QPL quads of channels per lane and RT rows held in registers, so that
@@ -107,14 +107,15 @@ __global__ void __launch_bounds__(256) q8_rows_kernel(long rows, int C, int Cp, 
       if (row > rows) break;
       unsigned am = 0;
 #pragma unroll
-      for (int i = 0; i < QPL; ++i)
+      for (int i = 0; i < QPL; ++i) {
+        if (VEC && (C & 3))            // a last quad that holds the view's padding
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (VEC && 4 * (l + i * L) + j >= C) v[t][i][j] = 0.f;
-          am = max(am, __float_as_uint(v[t][i][j]) & 0x7fffffffu);
-        }
+          for (int j = 1; j < 4; ++j)
+            if (4 * (l + i * L) + j >= C) v[t][i][j] = 0.f;
 #pragma unroll
-      for (int o = 1; o < L; o <<= 1) am = max(am, (unsigned)__shfl_xor((int)am, o, 64));
+        for (int j = 0; j < 4; ++j) am = max(am, abs_bits(v[t][i][j]));
+      }
+      am = group_umax<L>(am);
       const Q8Div d = q8_div(am);
 #pragma unroll
       for (int i = 0; i < QPL; ++i) {
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(1024) q8_weights_kernel(int taps, int cin, int
 #pragma unroll 4
     for (int i = rl; i < rows; i += NL) {
       const int t = i / cin, c = i - t * cin;
-      am = max(am, __float_as_uint(wk[t * st + c * sc]) & 0x7fffffffu);
+      am = max(am, abs_bits(wk[t * st + c * sc]));
     }
     atomicMax(&mx[kk], am);
   }

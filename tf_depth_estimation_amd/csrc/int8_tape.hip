@@ -10,7 +10,7 @@
 //
 // Lanes: a row's block of 64 channels is one 16-lane DPP row, four channels per lane (narrower layers use 1-8 lanes per
 // row), so max|u| is four DPP moves, a row's z / dy is one 16-byte and its codes one 4-byte access per lane.
-#include "tde_common.h"
+#include "int8_common.h"
 
 #include "bn_internal.h"
 
@@ -25,48 +25,44 @@ int tape_lanes(int C) {
   return l;
 }
 
-// maximum over the aligned group of L lanes (L <= 16), in every lane: quad swaps, then the mirrors of half a DPP row
-// and of the row.  All L lanes must be active.
-template <int L>
-__device__ __forceinline__ unsigned group_umax(unsigned v) {
-  if (L >= 2) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));   // lane ^ 1
-  if (L >= 4) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));   // lane ^ 2
-  if (L >= 8) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));  // 7 - lane
-  if (L >= 16) v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true)); // 15 - lane
-  return v;
-}
-
-// codes of four u under scale s, packed: the exact floor(|u| / s) clamped to 127, sign folded in.  The fp32 estimate
-// t = |u| / s is off by less than 4e-5 (three roundings of at most 128), so unless t lies that close to an integer its floor
-// is the quotient's; near one (1 element in 10^4; values past 127.5 are clamped anyway) the fp64 remainder decides.
+// codes of four u under scale s, packed: the exact floor(|u| / s) clamped to 127, sign folded in (~q for u <= 0).  The fp32
+// estimate t = |u| / s is off by less than 4e-5 (three roundings of at most 128), so unless t lies that close to an integer
+// its floor is the quotient's; near one (1 element in 10^4) the fp64 remainder decides.  Estimates past 127.25 are set
+// there: they are clamped to 127 anyway, and every block's maximum, at 128, would take the exact path.
 __device__ __noinline__ int tape_code_exact(double u, float s) {
-  const double au = fabs(u);
-  int q = (int)fmin(floor(au / (double)s), 127.0);
-  const double r = fma(-(double)q, (double)s, au);
-  if (r < 0.0) --q;
-  if (r >= (double)s && q < 127) ++q;
+  int q = 0;
+  if (s > 0.f) {                       // (s zero or NaN: 0 / -1)
+    const double au = fabs(u);
+    q = (int)fmin(floor(au / (double)s), 127.0);
+    const double r = fma(-(double)q, (double)s, au);
+    if (r < 0.0) --q;
+    if (r >= (double)s && q < 127) ++q;
+  }
   return u > 0.0 ? q : -1 - q;
 }
 __device__ __forceinline__ int tape_code4(const d4& u, const f4& uf, float s) {
-  const bool est = s >= 0x1p-100f, any = s > 0.f;      // (s NaN or 0: codes 0 / -1; below 2^-100 1 / s may overflow)
-  const float inv = est ? __builtin_amdgcn_rcpf(s) : 0.f;
-  int q[4], p = 0;
-  bool near = any && !est;
+  bool near = !(s >= 0x1p-100f);       // (1 / s may be no normal number)
+  const float inv = __builtin_amdgcn_rcpf(s);
+  f4 q;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float t = fabsf(uf[j]) * inv;
-    const float fl = floorf(fminf(t, 127.f));
-    q[j] = est ? (int)fl : 0;
-    near |= est && t > 0.5f && t < 127.5f && fabsf(t - rintf(t)) < 5e-5f;
+    const float t = fminf(fabsf(uf[j]) * inv, 127.25f);
+    q[j] = floorf(t);
+    near |= fabsf((t - q[j]) - 0.5f) > 0.49995f && t > 0.5f;
   }
   if (near) {
+    int p = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) p |= (tape_code_exact(u[j], s) & 0xff) << (8 * j);
     return p;
   }
+  unsigned p = put_byte<0>(q[0], 0);
+  p = put_byte<1>(q[1], p);
+  p = put_byte<2>(q[2], p);
+  p = put_byte<3>(q[3], p);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) p |= ((u[j] > 0.0 ? q[j] : -1 - q[j]) & 0xff) << (8 * j);
-  return p;
+  for (int j = 0; j < 4; ++j) p ^= u[j] > 0.0 ? 0u : 0xffu << (8 * j);
+  return (int)p;
 }
 
 // scale of a block from the bits of max|u| (NaN and infinity order above every finite value)
@@ -88,7 +84,7 @@ __device__ __forceinline__ void tape_row(const d4& u, f4& y, int& packed, float&
   for (int j = 0; j < 4; ++j) {
     uf[j] = (float)u[j];
     y[j] = uf[j] < 0.f ? 0.f : uf[j];
-    am = max(am, __float_as_uint(uf[j]) & 0x7fffffffu);
+    am = max(am, abs_bits(uf[j]));
   }
   s = tape_scale(group_umax<L>(am));
   packed = tape_code4(u, uf, s);
@@ -262,15 +258,17 @@ __global__ void __launch_bounds__(256) tape_fwd_apply_kernel(const TapeFwd p, co
   const bool on = c < p.C;
   const long base = (long)g * p.Mg;
   const int r0 = blockIdx.x * rpb, r1 = min(p.Mg, r0 + rpb);
+  // row of step i: uniform row rb + i R (addresses in scalar registers) + this lane's rl (32-bit offsets)
+  const unsigned zo = rl * p.C + c, yo = rl * p.ycs + c, so = rl * p.NB + b;
   f4 v[APPLY_RB];
   auto load = [&](int rb) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < APPLY_RB; ++i) {
-      const int r = min(rb + i * R, r1 - 1);
-      v[i] = on ? *reinterpret_cast<const f4*>(p.z + (base + r) * p.C + c) : f4{0.f, 0.f, 0.f, 0.f};
+      v[i] = f4{0.f, 0.f, 0.f, 0.f};
+      if (on && rb + i * R + rl < r1) v[i] = *reinterpret_cast<const f4*>(p.z + (base + rb + i * R) * p.C + zo);
     }
   };
-  load(r0 + rl);                       // in flight while the statistics are evaluated
+  load(r0);                            // in flight while the statistics are evaluated
   d4 mu = {0, 0, 0, 0}, is = {0, 0, 0, 0}, bt = {0, 0, 0, 0};
   if (on) {
 #pragma unroll
@@ -281,16 +279,15 @@ __global__ void __launch_bounds__(256) tape_fwd_apply_kernel(const TapeFwd p, co
       if (blockIdx.x == 0 && g == 0 && rl == 0) tape_publish(p, sums, c + j);
     }
   }
-  for (int rb = r0 + rl; rb < r1; rb += APPLY_RB * R) {
+  for (int rb = r0; rb < r1; rb += APPLY_RB * R) {
     f4 w[APPLY_RB];
 #pragma unroll
     for (int i = 0; i < APPLY_RB; ++i) w[i] = v[i];
     if (rb + APPLY_RB * R < r1) load(rb + APPLY_RB * R);
 #pragma unroll
     for (int i = 0; i < APPLY_RB; ++i) {
-      const int r = rb + i * R;
-      if (r >= r1) break;
-      const long row = base + r;
+      if (rb + i * R + rl >= r1) break;
+      const long row = base + rb + i * R;
       d4 u;
 #pragma unroll
       for (int j = 0; j < 4; ++j) u[j] = fma((double)w[i][j] - mu[j], is[j], bt[j]);
@@ -299,9 +296,9 @@ __global__ void __launch_bounds__(256) tape_fwd_apply_kernel(const TapeFwd p, co
       float s;
       tape_row<L>(u, y, packed, s);
       if (on) {
-        tde_st(reinterpret_cast<f4*>(p.y + row * p.ycs + p.yco + c), y);
-        *reinterpret_cast<int*>(p.codes + row * p.C + c) = packed;
-        if (q % L == 0) p.scales[row * p.NB + b] = s;
+        tde_st(reinterpret_cast<f4*>(p.y + row * p.ycs + p.yco + yo), y);
+        *reinterpret_cast<int*>(p.codes + row * p.C + zo) = packed;
+        if (q % L == 0) p.scales[row * p.NB + so] = s;
       }
     }
   }
@@ -475,19 +472,22 @@ __global__ void __launch_bounds__(256) tape_bwd_apply_kernel(const TapeBwd p, co
   if (rl < R && c < p.C) {
     const long base = (long)g * p.Mg;
     const int r0 = blockIdx.x * rpb, r1 = min(p.Mg, r0 + rpb);
+    // (row addresses as in the forward)
+    const unsigned zo = rl * p.C + c, yo = rl * p.dycs + c, so = rl * p.NB + b;
     f4 v[APPLY_RB];
     int cd[APPLY_RB];
     float s[APPLY_RB];
     auto load = [&](int rb) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < APPLY_RB; ++i) {
-        const long row = base + min(rb + i * R, r1 - 1);
-        v[i] = *reinterpret_cast<const f4*>(p.dy + row * p.dycs + p.dyco + c);
-        cd[i] = *reinterpret_cast<const int*>(p.codes + row * p.C + c);
-        s[i] = p.scales[row * p.NB + b];
-      }
+      for (int i = 0; i < APPLY_RB; ++i)
+        if (rb + i * R + rl < r1) {
+          const long row = base + rb + i * R;
+          v[i] = *reinterpret_cast<const f4*>(p.dy + row * p.dycs + p.dyco + yo);
+          cd[i] = *reinterpret_cast<const int*>(p.codes + row * p.C + zo);
+          s[i] = p.scales[row * p.NB + so];
+        }
     };
-    load(r0 + rl);                     // in flight while the means are evaluated
+    load(r0);                          // in flight while the means are evaluated
     f4 m0, m1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -503,15 +503,15 @@ __global__ void __launch_bounds__(256) tape_bwd_apply_kernel(const TapeBwd p, co
       }
     const f4 is = *reinterpret_cast<const f4*>(p.save_invstd + (long)g * p.C + c);
     const f4 bt = *reinterpret_cast<const f4*>(p.beta + c);
-    for (int rb = r0 + rl; rb < r1; rb += APPLY_RB * R) {
+    for (int rb = r0; rb < r1; rb += APPLY_RB * R) {
       f4 o[APPLY_RB];
 #pragma unroll
       for (int i = 0; i < APPLY_RB; ++i)
-        if (rb + i * R < r1) tape_dz_row(v[i], cd[i], s[i], bt, m0, m1, is, o[i], mx);
+        if (rb + i * R + rl < r1) tape_dz_row(v[i], cd[i], s[i], bt, m0, m1, is, o[i], mx);
       if (rb + APPLY_RB * R < r1) load(rb + APPLY_RB * R);
 #pragma unroll
       for (int i = 0; i < APPLY_RB; ++i)
-        if (rb + i * R < r1) tde_st(reinterpret_cast<f4*>(p.dz + (base + rb + i * R) * p.C + c), o[i]);
+        if (rb + i * R + rl < r1) tde_st(reinterpret_cast<f4*>(p.dz + (base + rb + i * R) * p.C + zo), o[i]);
     }
   }
   block_absmax_to(mx, p.absmax);
