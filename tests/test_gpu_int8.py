@@ -99,6 +99,24 @@ CONVS = [
     (1, 1, 8200, 64, 1600, 1, 1, False, False),
     (2, 50, 60, 128, 96, 1, 1, False, True),
     (2, 50, 60, 128, 96, 1, 2, False, True),
+    (1, 1, 1, 64, 16, 1, 1, False, True),         # tokens: each tile size, rows of 32 bytes, sizes inside and on a tile's edge
+    (1, 1, 1, 2048, 100, 1, 1, False, False),
+    (1, 1, 17, 2050, 33, 1, 1, False, True),
+    (1, 1, 31, 5, 3, 1, 1, False, False),
+    (1, 1, 64, 32, 64, 1, 1, False, True),
+    (1, 1, 512, 448, 510, 1, 1, False, True),
+    (1, 1, 900, 130, 700, 1, 1, False, True),
+    (1, 1, 640, 20, 1024, 1, 1, False, False),
+    (3, 20, 41, 17, 256, 1, 1, False, True),
+    (1, 1, 8000, 20, 300, 1, 1, False, True),
+    (1, 1, 40000, 64, 50, 1, 1, False, True),
+    (1, 1, 8065, 130, 260, 1, 1, False, False),
+    (1, 1, 24700, 20, 400, 1, 1, False, True),
+    (1, 1, 24576, 70, 513, 1, 1, False, True),
+    (16, 3, 3, 96, 500, 3, 1, False, True),       # small maps: each split of the steps
+    (70, 3, 3, 70, 100, 3, 1, False, True),
+    (300, 2, 3, 64, 130, 3, 1, False, True),
+    (200, 2, 2, 20, 40, 3, 2, True, True),
 ]
 
 

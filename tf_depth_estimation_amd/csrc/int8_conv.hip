@@ -127,14 +127,12 @@ __global__ void __launch_bounds__(256) q8_rows_kernel(long rows, int C, int Cp, 
   }
 }
 
-// ---- weights: a block takes KB output channels (padding channels write zeros), 1024 / KB lanes each; lanes run along the
+// ---- weights: a block takes four output channels (padding channels write zeros), 256 lanes each; lanes run along the
 // contiguous dimension of the layout (0: output channels, 1: input channels).  The maximum's atomics are on integers in
-// LDS: the order does not matter.  KB 16 for many channels (2048 x 2048: 19 us, 52 with one block a channel), 4 for few,
-// where blocks count for more than whole lines.
-template <int KB>
+// LDS: the order does not matter.
 __global__ void __launch_bounds__(1024) q8_weights_kernel(int taps, int cin, int K, int Kp, int Cp, int layout,
                                                           const float* w, int8_t* codes, float* scales) {
-  constexpr int NL = 1024 / KB;
+  constexpr int KB = 4, NL = 1024 / KB;
   __shared__ unsigned mx[KB];
   const int kk = layout == 0 ? threadIdx.x % KB : threadIdx.x / NL, rl = layout == 0 ? threadIdx.x / KB : threadIdx.x % NL;
   const int k = blockIdx.x * KB + kk, rows = taps * cin;
@@ -166,6 +164,50 @@ __global__ void __launch_bounds__(1024) q8_weights_kernel(int taps, int cin, int
     *reinterpret_cast<int*>(codes + ((long)t * Kp + k) * Cp + c) = q8_code4(v, d);
   }
   if (rl == 0) scales[k] = q8_scale(am);
+}
+
+// The same for layout 0 with K % 4 == 0 and 16-byte rows: a lane reads four output channels at a time, and writes four
+// codes of each from four rows turned in registers.  Block = 16 channels x 256 rows.  (3x3x512 -> 512: 19 us, 31 by the
+// kernel above; 2048 x 2048: 15.)
+__global__ void __launch_bounds__(1024) q8_weights4_kernel(int taps, int cin, int K, int Kp, int Cp, const float* w,
+                                                           int8_t* codes, float* scales) {
+  __shared__ unsigned mx[16];
+  const int kl = 4 * (threadIdx.x & 3), rl = threadIdx.x >> 2, k = blockIdx.x * 16 + kl, rows = taps * cin;
+  const bool on = k < K;
+  if (threadIdx.x < 16) mx[threadIdx.x] = 0;
+  __syncthreads();
+  unsigned am[4] = {0, 0, 0, 0};
+  if (on) {
+#pragma unroll 6
+    for (int i = rl; i < rows; i += 256) {
+      const f4 v = *reinterpret_cast<const f4*>(w + (long)i * K + k);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) am[j] = max(am[j], abs_bits(v[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) atomicMax(&mx[kl + j], am[j]);
+  }
+  __syncthreads();
+  Q8Div d[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) d[j] = q8_div(mx[kl + j]);
+  const int nq = Cp / 4, quads = taps * nq;
+#pragma unroll 2
+  for (int i = rl; i < quads; i += 256) {
+    const int t = i / nq, c = 4 * (i - t * nq);
+    f4 v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      v[r] = f4{0.f, 0.f, 0.f, 0.f};
+      if (on && c + r < cin) v[r] = *reinterpret_cast<const f4*>(w + ((long)t * cin + c + r) * K + k);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      *reinterpret_cast<int*>(codes + ((long)t * Kp + k + j) * Cp + c) = q8_code4(f4{v[0][j], v[1][j], v[2][j], v[3][j]}, d[j]);
+  }
+  if (rl == 0)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) scales[k + j] = q8_scale(mx[kl + j]);
 }
 
 // ---- the product.  One class of output pixels (a conv has one; a stride-s transposed conv s * s parities): output
@@ -259,10 +301,10 @@ __device__ __forceinline__ float* q8_out(const Q8Conv& p, const Q8Class& cl, int
 }
 
 // ---- few pixels: WK waves take turns at the (tap, channel chunk) steps of a tile of 16 TM channels x 16 TN pixels and
-// add their fp32 sums through LDS in wave order.  The time is the latency of the weights, so a wave has the fragments of U
-// steps in flight, straight from the caches (a lane's 16 / 8 bytes are its row's k-quarter), and every step is scaled by
-// itself.  (4x4x512 -> 512, one image: 7.2 us with one step in flight.)
-template <int TM, int TN, int KC, int WK, int U>
+// add their fp32 sums through LDS in wave order.  The time is the latency of the weights, which come straight from the
+// caches (a lane's 16 / 8 bytes are its row's k-quarter); the waves of a SIMD cover it for each other.  (4x4x512 -> 512, one
+// image: 6.6 us; with the fragments of 2 / 4 steps in flight per wave 7.0 / 7.8: their addresses delay the first load.)
+template <int TM, int TN, int KC, int WK>
 __global__ void __launch_bounds__(64 * WK) q8_split_kernel(const Q8Conv p) {
   using F = typename Q8Frag<KC>::T;
   __shared__ f4 red[(WK - 1) * TM * TN * 64];
@@ -295,35 +337,29 @@ __global__ void __launch_bounds__(64 * WK) q8_split_kernel(const Q8Conv p) {
     for (int b = 0; b < TN; ++b) acc[a][b] = f4{0.f, 0.f, 0.f, 0.f};
 
   const int nch = p.Cp / KC, steps = cl.nty * cl.ntx * nch;
-  for (int s0 = wk; s0 < steps; s0 += WK * U) {
-    F fa[U][TM], fb[U][TN];
-    float xs[U][TN];
+  for (int s = wk; s < steps; s += WK) {
+    const int t = s / nch, ch = s - t * nch, ty = t / cl.ntx, tx = t - ty * cl.ntx;
+    const long wtap = ((long)(cl.ky0 + p.kst * ty) * p.KW + cl.kx0 + p.kst * tx) * p.Kp * p.Cp + ch * KC;
+    F fa[TM], fb[TN];
+    float xs[TN];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int sr = s0 + u * WK, s = min(sr, steps - 1);      // (a step past the end: a valid load, scale 0)
-      const int t = s / nch, ch = s - t * nch, ty = t / cl.ntx, tx = t - ty * cl.ntx;
-      const long wtap = ((long)(cl.ky0 + p.kst * ty) * p.KW + cl.kx0 + p.kst * tx) * p.Kp * p.Cp + ch * KC;
+    for (int a = 0; a < TM; ++a) fa[a] = *reinterpret_cast<const F*>(wrow[a] + wtap);
 #pragma unroll
-      for (int a = 0; a < TM; ++a) fa[u][a] = *reinterpret_cast<const F*>(wrow[a] + wtap);
-#pragma unroll
-      for (int b = 0; b < TN; ++b) {
-        const int yy = iy[b] + p.dir * ty, xx = ix[b] + p.dir * tx;
-        const bool in = (unsigned)yy < (unsigned)p.H && (unsigned)xx < (unsigned)p.W && sr < steps;
-        const long pix = in ? pb[b] + (long)yy * p.W + xx : zero_row;
-        fb[u][b] = *reinterpret_cast<const F*>(p.x + pix * p.Cp + kq * (KC / 4) + ch * KC);
-        xs[u][b] = p.xs[pix];
-      }
+    for (int b = 0; b < TN; ++b) {
+      const int yy = iy[b] + p.dir * ty, xx = ix[b] + p.dir * tx;
+      const bool in = (unsigned)yy < (unsigned)p.H && (unsigned)xx < (unsigned)p.W;
+      const long pix = in ? pb[b] + (long)yy * p.W + xx : zero_row;
+      fb[b] = *reinterpret_cast<const F*>(p.x + pix * p.Cp + kq * (KC / 4) + ch * KC);
+      xs[b] = p.xs[pix];
     }
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int a = 0; a < TM; ++a)
 #pragma unroll
-      for (int a = 0; a < TM; ++a)
+      for (int b = 0; b < TN; ++b) {
+        const i4 ia = Q8Frag<KC>::mfma(fa[a], fb[b], i4{0, 0, 0, 0});
 #pragma unroll
-        for (int b = 0; b < TN; ++b) {
-          const i4 ia = Q8Frag<KC>::mfma(fa[u][a], fb[u][b], i4{0, 0, 0, 0});
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[a][b][j] = fmaf((float)ia[j], xs[u][b], acc[a][b][j]);
-        }
+        for (int j = 0; j < 4; ++j) acc[a][b][j] = fmaf((float)ia[j], xs[b], acc[a][b][j]);
+      }
   }
 
   if (wk > 0)
@@ -557,9 +593,10 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
 // (global_load_lds_dwordx4: a wave instruction copies 16 rows of 64 bytes) into a ring of three slots, two steps in
 // flight across the barriers; the 16-byte quarters of a row are exchanged by (row >> 1) & 3 on the way, so that the
 // fragment reads of 8 neighbouring rows hit different banks.  All sums stay integers until the end.
-// 8192 x 2048 x 2048: 43 us = 1590 TOP/s with 256 x 256 tiles on 8 waves, whose LDS reads (96 bytes a clock) run under the
-// products because the pixel fragments, which every product needs, are read first (55 us the other way round); 128 x 128
-// tiles read 128 bytes a clock for the same products and take 65 us, and serve where the large ones leave CUs idle.
+// 8192 x 2048 x 2048: 42 us = 1640 TOP/s with 256 x 256 tiles on 8 waves, whose LDS reads (96 bytes a clock) run under the
+// products because the pixel fragments, which every product needs, are read first (55 us the other way round).  The matrix
+// unit is busy 42 % of the time; the rest are the barriers of a step and the 67 MB that all blocks write at their ends.
+// Smaller tiles read more LDS bytes per product and serve where the large ones would leave CUs idle.
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef __attribute__((address_space(1))) void* gbl_ptr_t;
 // this wave's LDS reads are done (written as a builtin, so that the compiler knows and waits for none of them again), then
@@ -589,8 +626,9 @@ __global__ void __launch_bounds__(64 * WC * WP) q8_gemm_kernel(const Q8Conv p, i
   for (int j = 0; j < DI; ++j) {
     const int row = (wv * DI + j) * 16 + (lane >> 2);
     const int q = ((lane & 3) ^ ((row >> 1) & 3)) * 16;
-    src[j] = row < BC ? p.w + (long)min(n0 + row, p.Kp - 1) * p.Cp + q
-                      : p.x + (long)min(m0 + row - BC, M) * p.Cp + q;       // (row M of the codes is zero)
+    const bool in = q < p.Cp;               // rows of 32 bytes: the pixels' upper half is the zero row (row M of the codes)
+    src[j] = row < BC ? p.w + (long)min(n0 + row, p.Kp - 1) * p.Cp + (in ? q : q - 32)
+                      : p.x + (long)(in ? min(m0 + row - BC, M) : M) * p.Cp + (in ? q : q - 32);
   }
   auto dma = [&](int s, int slot) __attribute__((always_inline)) {
 #pragma unroll
@@ -605,7 +643,7 @@ __global__ void __launch_bounds__(64 * WC * WP) q8_gemm_kernel(const Q8Conv p, i
     for (int b = 0; b < TN; ++b) acc[a][b] = i4{0, 0, 0, 0};
 
   const int lofs = r16 * 64 + ((kq ^ ((r16 >> 1) & 3)) << 4);
-  const int steps = p.Cp / 64, last = steps - 1;
+  const int steps = (p.Cp + 63) / 64, last = steps - 1;
   struct Frag {
     i4 a[TM], b[TN];
   };
@@ -666,13 +704,13 @@ __global__ void __launch_bounds__(64 * WC * WP) q8_gemm_kernel(const Q8Conv p, i
 }
 
 // ---- launches
-template <int TM, int TN, int WK, int U>
+template <int TM, int TN, int WK>
 void q8_split_launch(const Q8Conv& p, long Mmax, int classes, hipStream_t st) {
   const dim3 grid(tde_cdiv(Mmax, 16 * TN), tde_cdiv(p.K, 16 * TM), classes);
   if (p.Cp % 64 == 0)
-    hipLaunchKernelGGL((q8_split_kernel<TM, TN, 64, WK, U>), grid, dim3(64 * WK), 0, st, p);
+    hipLaunchKernelGGL((q8_split_kernel<TM, TN, 64, WK>), grid, dim3(64 * WK), 0, st, p);
   else
-    hipLaunchKernelGGL((q8_split_kernel<TM, TN, 32, WK, U>), grid, dim3(64 * WK), 0, st, p);
+    hipLaunchKernelGGL((q8_split_kernel<TM, TN, 32, WK>), grid, dim3(64 * WK), 0, st, p);
 }
 
 constexpr int Q8_LDS = 64 * 1024;      // patch bytes of a halo block: two blocks fit a CU's 160 KB
@@ -724,19 +762,26 @@ int q8_conv(Q8Conv p, hipStream_t st) {
   const int GH = (p.OH + s - 1) / s, GW = (p.OW + s - 1) / s;
   const long Mmax = (long)p.N * GH * GW;
   const long tiles = ((Mmax + 15) / 16) * ((p.K + 15) / 16) * classes;      // 16 x 16 tiles
-  if (p.KH == 1 && p.KW == 1 && p.is == 1 && p.os == 1 && p.OH == p.H && p.OW == p.W && p.Cp % 64 == 0 && tiles > 2048) {
-    const long big = (long)tde_cdiv(Mmax, 256) * tde_cdiv(p.K, 256);      // tiles of 256 x 256
-    if (big >= 192) q8_gemm_launch<8, 4, 2, 4>(p, (int)Mmax, st);
-    else q8_gemm_launch<4, 4, 2, 2>(p, (int)Mmax, st);
+  if (p.KH == 1 && p.KW == 1 && p.is == 1 && p.os == 1 && p.OH == p.H && p.OW == p.W && (Mmax > 16 || p.Cp < 2048)) {
+    // The largest tiles that still fill the CUs.  us, this choice / its neighbour (tokens x input x output channels):
+    // 128x2048x2048 5.1 / 6.7 with the next larger tiles, 256x2048x2048 6.9 / 8.8 with the next smaller;
+    // 8192x256x256 4.9 / 6.3 (larger), 8192x1024x1024 21.9 / 23.7 (smaller); 393216x64x128 42 / 69 (larger),
+    // 49152x512x256 20.9 / 22.6 (smaller).  One token of 2048 -> 2048 channels: 4.2 by the split kernel below, 4.7 here.
+    const auto blocks = [&](int k, int m) { return (long)tde_cdiv(Mmax, m) * tde_cdiv(p.K, k); };
+    if (blocks(32, 32) <= 256) q8_gemm_launch<1, 1, 2, 2>(p, (int)Mmax, st);
+    else if (blocks(64, 64) <= 512) q8_gemm_launch<1, 2, 4, 2>(p, (int)Mmax, st);
+    else if (p.K <= 128 || blocks(256, 256) < 192) q8_gemm_launch<2, 4, 2, 2>(p, (int)Mmax, st);
+    else q8_gemm_launch<8, 4, 2, 4>(p, (int)Mmax, st);
     return tde_launch_status();
   }
   bool done = false;
-  if (GH * GW >= 12 && tiles > 64) {
+  if (GH * GW >= 12 && tiles > 256) {
     // Blocks of fewer pixels and channels, and more wave groups that split the steps, the fewer tiles there are; timed for
     // each size on the networks' layers at batch 1, 8 and 32 (us, this choice / the next larger block):
-    // 14x14x512 -> 256 8.3 / 10.4, 28x28x256 -> 128 6.4 / 7.9, 6x8x1024 -> 512 (8) 16.1 / 19.3, 24x32x128 -> 128 (8)
-    // 9.6 / 10.5, 12x16x512 -> 256 (8) 15.3 / 18.0, 48x64x64 -> 64 k5 (8) 11.6 / 13.4, 96x128x32 -> 32 k7 (8) 22.0 / 28.2,
-    // (32) 64.8 / 72.9 with this choice's smaller neighbour, 24x32x256 -> 128 (32) 23.7 / 28.1
+    // 28x28x256 -> 128 6.3 / 7.9 (14x14x512 -> 256, 208 tiles: 7.9, 7.2 by the split kernel below), 6x8x1024 -> 512 (8)
+    // 16.1 / 19.3, 24x32x128 -> 128 (8) 9.6 / 10.5, 12x16x512 -> 256 (8) 15.3 / 18.0, 48x64x64 -> 64 k5 (8) 11.6 / 13.4,
+    // 96x128x32 -> 32 k7 (8) 22.0 / 28.2, (32) 64.8 / 72.9 with this choice's smaller neighbour, 24x32x256 -> 128 (32)
+    // 23.7 / 28.1
     if (tiles < 512) done = q8_halo_launch<1, 2, 1, 1, 8>(p, GH, GW, classes, st);
     else if (tiles < 1536) done = q8_halo_launch<2, 2, 1, 1, 8>(p, GH, GW, classes, st);
     else if (p.K <= 16) done = tiles < 8192 ? q8_halo_launch<1, 4, 1, 2, 2>(p, GH, GW, classes, st)
@@ -750,8 +795,10 @@ int q8_conv(Q8Conv p, hipStream_t st) {
     else done = q8_halo_launch<2, 4, 1, 4, 1>(p, GH, GW, classes, st);
   }
   if (!done) {
-    if (tiles <= 4096) q8_split_launch<1, 1, 16, 4>(p, Mmax, classes, st);
-    else q8_split_launch<2, 2, 4, 2>(p, Mmax, classes, st);
+    // 8x 3x3x512 -> 512 7.0 / 9.3 with the next larger tiles, 16x 9.4 / 11.6 (smaller), 64x 20.2 / 28.0 (smaller)
+    if (tiles <= 256) q8_split_launch<1, 1, 16>(p, Mmax, classes, st);
+    else if (tiles <= 512) q8_split_launch<1, 2, 8>(p, Mmax, classes, st);
+    else q8_split_launch<2, 2, 4>(p, Mmax, classes, st);
   }
   return tde_launch_status();
 }
@@ -817,11 +864,11 @@ int tde_q8_weights(int taps, int cin, int K, int layout, const float* w, int8_t*
   TDE_CHECK_ARG(tde_q8_weights_size(taps, cin, K) > 0 && taps <= 4096 && (layout == 0 || layout == 1) && w && codes &&
                 scales && tde_aligned16(codes));
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (K >= 1024)
-    hipLaunchKernelGGL(q8_weights_kernel<16>, dim3(q8_cols(K) / 16), dim3(1024), 0, st, taps, cin, K, q8_cols(K), q8_row(cin),
-                       layout, w, codes, scales);
+  if (layout == 0 && K % 4 == 0 && tde_aligned16(w))
+    hipLaunchKernelGGL(q8_weights4_kernel, dim3(q8_cols(K) / 16), dim3(1024), 0, st, taps, cin, K, q8_cols(K), q8_row(cin), w,
+                       codes, scales);
   else
-    hipLaunchKernelGGL(q8_weights_kernel<4>, dim3(q8_cols(K) / 4), dim3(1024), 0, st, taps, cin, K, q8_cols(K), q8_row(cin),
+    hipLaunchKernelGGL(q8_weights_kernel, dim3(q8_cols(K) / 4), dim3(1024), 0, st, taps, cin, K, q8_cols(K), q8_row(cin),
                        layout, w, codes, scales);
   return tde_launch_status();
 }
