@@ -308,6 +308,16 @@ int tde_q8_conv2d_bias_act(const tde_conv_desc_t* d, const int8_t* x_codes, cons
 int tde_q8_deconv2d_bias_act(const tde_conv_desc_t* d, const int8_t* x_codes, const float* x_scales,
                              const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y_big,
                              void* stream);
+/* tde_q8_rows and the conv in one call: `d` also names the fp32 input's channel view (as for tde_conv2d_fwd_bias_act /
+ * tde_deconv2d_fwd_bias_act, without their alignments).  x_codes / x_scales: buffers for the rows' codes.  Where
+ * tde_q8_one_launch(d, deconv) is 1 and x starts on 16 bytes the call is one launch that uses neither (they may be NULL). */
+int tde_q8_one_launch(const tde_conv_desc_t* d, int deconv);
+int tde_q8_conv2d_f32_bias_act(const tde_conv_desc_t* d, const float* x, int8_t* x_codes, float* x_scales,
+                               const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y,
+                               void* stream);
+int tde_q8_deconv2d_f32_bias_act(const tde_conv_desc_t* d, const float* x_small, int8_t* x_codes, float* x_scales,
+                                 const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y_big,
+                                 void* stream);
 
 /* (2) The 8-bit tape of training BatchNorm + ReLU: what the backward pass needs of a layer -- its pre-BN output z, the
  * ReLU mask and its output y -- as ONE 8-bit code per element instead of two fp32 tensors.  The pre-activation

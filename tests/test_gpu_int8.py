@@ -38,7 +38,7 @@ def rows_data(M, C, seed):
 
 
 @pytest.mark.parametrize("M,C", [(1, 1), (5, 3), (17, 4), (33, 17), (64, 32), (40, 33), (257, 64), (31, 100), (20, 512),
-                                 (19, 1000), (18, 2048), (17, 4096)])
+                                 (19, 1000), (18, 1023), (18, 2048), (16, 2046), (17, 4096), (16, 3999), (1, 4096)])
 def test_rows_codes_are_exact(M, C):
     x = rows_data(M, C, 1)
     q, s = O.quantize(x, 1)
@@ -124,7 +124,7 @@ def conv_inputs(N, H, W, C, K, k, deconv, seed=3):
     r = rng(seed, N, H, W, C, K, k)
     x = np.maximum(r.standard_normal((N, H, W, C)) * r.uniform(0.5, 1.5, C), 0).astype(np.float32)
     x[..., -1] = r.uniform(0, 4, (N, H, W))
-    if H * W > 4:
+    if W > 1 and H * W > 4:
         x[0, 0, 1] = 0
     shape = (k, k, K, C) if deconv else (k, k, C, K)
     w = (r.uniform(-1, 1, shape) * (6.0 / (k * k * (C + K))) ** 0.5).astype(np.float32)
@@ -150,6 +150,47 @@ def test_conv_matches_the_definition(N, H, W, C, K, k, s, deconv, relu):
     assert y.shape == ref.shape
     err = np.abs(y - ref)
     assert (err <= conv_bound(mag, k * k)).all(), (err - conv_bound(mag, k * k)).max()
+    # the rows quantised by a call of their own
+    y8 = conv(int8.quantize_rows(dev(x))).cpu().numpy()
+    assert (np.abs(y8 - ref) <= conv_bound(mag, k * k)).all()
+
+
+# few pixels: one launch that quantises in LDS.  Blocks inside one image row, over rows, over images, on the last row of a
+# padded view
+SMALL = [
+    (1, 1, 1, 64, 16, 1, 1, False), (1, 1, 5, 1024, 40, 1, 1, False), (1, 1, 200, 100, 33, 1, 1, False),
+    (2, 1, 12, 70, 20, 1, 1, False), (1, 4, 4, 512, 64, 3, 1, False), (3, 3, 5, 300, 30, 3, 1, False),
+    (1, 6, 5, 66, 50, 5, 2, False), (1, 1, 32, 130, 17, 3, 1, False), (1, 31, 1, 130, 17, 3, 2, False),
+    (5, 2, 3, 1024, 18, 3, 1, False), (1, 5, 6, 64, 32, 7, 1, False), (1, 4, 4, 256, 20, 3, 2, True),
+    (3, 3, 2, 70, 40, 3, 2, True), (1, 1, 1, 513, 9, 3, 2, True), (2, 3, 5, 90, 12, 5, 3, True), (1, 2, 9, 65, 8, 1, 2, True),
+]
+
+
+@pytest.mark.parametrize("N,H,W,C,K,k,s,deconv", SMALL)
+def test_conv_of_few_pixels_in_one_launch(N, H, W, C, K, k, s, deconv):
+    x, w, b = conv_inputs(N, H, W, C, K, k, deconv, seed=13)
+    ref, mag = O.conv8(x, w, b, s, deconv, False)
+    conv = int8.Conv8(dev(w), dev(b), stride=s, relu=False, deconv=deconv)
+    cs = (C + 3) // 4 * 4 + 8
+    buf = torch.full((N * H * W, cs), float("nan"), device="cuda")       # padding is not read as channels
+    xv = buf.view(N, H, W, cs)[..., 4:4 + C]
+    xv.copy_(dev(x))
+    d, one = conv._desc(N, H, W, cs, K)
+    assert one
+    y = conv(xv)
+    assert (np.abs(y.cpu().numpy() - ref) <= conv_bound(mag, k * k)).all()
+    # an unaligned view of the same input takes two launches; the same codes, sums of other parts
+    odd = torch.empty(N * H * W * (C + 1) + 1, device="cuda")[1:].view(N, H, W, C + 1)[..., :C]
+    odd.copy_(xv)
+    assert (np.abs(conv(odd).cpu().numpy() - ref) <= conv_bound(mag, k * k)).all()
+    # a bad pixel shows in exactly the outputs that read it
+    bad = x.copy()
+    bad[-1, -1, -1, C // 2] = np.inf
+    xv.copy_(dev(bad))
+    marked = x * 0
+    marked[-1, -1, -1] = 1
+    reads, _ = O.conv8(marked, np.ones_like(w), np.zeros_like(b), s, deconv, False)
+    np.testing.assert_array_equal(np.isnan(conv(xv).cpu().numpy()), reads > 0)
 
 
 @pytest.mark.parametrize("deconv", [False, True])

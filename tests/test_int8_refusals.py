@@ -98,6 +98,25 @@ def test_conv_arguments(p):
             args[i] = None
             assert fn(desc(), args[0], args[1], args[2], args[3], None, 1, args[5], None) == -1, i
         assert fn(None, p, p, p, p, None, 1, p, None) == -1
+    for fn, view, src in ((lib.tde_q8_conv2d_f32_bias_act, "y", "x"), (lib.tde_q8_deconv2d_f32_bias_act, "x", "y")):
+        for kw in (dict(N=0), dict(stride=0), dict(pad_top=3), dict(N=1 << 28), {view + "_cstride": 3}, {src + "_coff": 1},
+                   {src + "_coff": -4}, {src + "_cstride": 3}, dict(w_cin=5000, K=5000)):
+            assert fn(desc(**kw), p, p, p, p, p, None, 1, p, None) == -1, kw
+        for i in (0, 1, 2, 3, 4, 6):          # (codes and scales: this geometry takes two launches)
+            args = [p, p, p, p, p, None, p]
+            args[i] = None
+            assert fn(desc(), *args[:6], 1, args[6], None) == -1, i
+        assert fn(None, p, p, p, p, p, None, 1, p, None) == -1
+
+
+def test_one_launch():
+    lib = _lib.load()
+    small = dict(H=4, W=4, OH=4, OW=4, C=64, w_cin=64, K=64, x_cstride=64, y_cstride=64)
+    assert [lib.tde_q8_one_launch(desc(**{**small, **kw}), dec) for kw, dec in (
+        (dict(), 0), (dict(), 1), (dict(x_cstride=66), 0), (dict(x_coff=2, x_cstride=68), 0), (dict(w_cin=32), 0),
+        (dict(N=0), 0), (dict(H=400, W=400, OH=400, OW=400), 0), (dict(H=40, W=40, OH=4, OW=4, stride=10), 0))
+            ] == [1, 1, 0, 0, 0, 0, 0, 0]
+    assert lib.tde_q8_one_launch(None, 0) == 0
 
 
 def test_tape_arguments(p):

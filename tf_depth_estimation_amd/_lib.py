@@ -163,6 +163,9 @@ _SIGS = {
     "tde_q8_weights": (c_int, [c_int, c_int, c_int, c_int, P, P, P, P]),
     "tde_q8_conv2d_bias_act": (c_int, [P, P, P, P, P, P, c_int, P, P]),
     "tde_q8_deconv2d_bias_act": (c_int, [P, P, P, P, P, P, c_int, P, P]),
+    "tde_q8_one_launch": (c_int, [P, c_int]),
+    "tde_q8_conv2d_f32_bias_act": (c_int, [P, P, P, P, P, P, P, c_int, P, P]),
+    "tde_q8_deconv2d_f32_bias_act": (c_int, [P, P, P, P, P, P, P, c_int, P, P]),
     "tde_tape8_workspace_size": (c_size_t, [c_int, c_int]),
     "tde_tape8_one_launch": (c_int, [c_int, c_int, c_int]),
     "tde_tape8_bn_fwd": (c_int, [c_int, c_int, c_int, P, P, c_float, c_float, c_int, P, P, P, P, P, c_int, c_int, P, P,

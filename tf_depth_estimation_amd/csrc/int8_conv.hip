@@ -26,105 +26,154 @@ __device__ __forceinline__ float q8_scale(unsigned amax_bits) {
 }
 
 // rne(127 x / a), exact.  The fp32 estimate t = x * (127 / a) is off by less than 4e-5 (three roundings of at most 127),
-// so unless t lies that close to a half-integer its rounding is the quotient's.  Near one (1 element in 10^4) the fp64
-// remainder 254 x - 2 q a (exact: 24-bit factors) decides, and breaks a tie to even.  a: finite maximum, |x| <= a.
+// so unless t lies that close to a half-integer its rounding is the quotient's.  Near one (1 element in 10^4) the quotient
+// lies between floor(t) and floor(t) + 1, and the sign of 254 x - (2 floor(t) + 1) a decides (both products are exact in
+// fp64: 32 bits), 0 being a tie, to even.  Where 1 / a may be no normal number x and a are first scaled by a power of two (an
+// x that this makes subnormal has code 0 anyway).  a: finite maximum, |x| <= a.
 struct Q8Div {
-  double a;
-  float inv;
-  int mode;          // 0: the row is zero or not finite, 1: fp32 estimate, 2: fp64 division (1 / a may be no normal number)
+  float a, inv, sc;          // inv 0: the row is zero or not finite
 };
 __device__ __forceinline__ Q8Div q8_div(unsigned amax_bits) {
   Q8Div d;
-  const float a = __uint_as_float(amax_bits);
-  d.a = (double)a;
-  d.inv = 0.f;
-  d.mode = amax_bits == 0 || amax_bits >= 0x7f800000u ? 0 : (a >= 0x1p-100f && a <= 0x1p100f ? 1 : 2);
-  if (d.mode == 1) d.inv = 127.f * __builtin_amdgcn_rcpf(a);
+  d.a = __uint_as_float(amax_bits);
+  d.sc = d.a < 0x1p-100f ? 0x1p64f : (d.a > 0x1p100f ? 0x1p-64f : 1.f);
+  d.inv = amax_bits == 0 || amax_bits >= 0x7f800000u ? 0.f : 127.f * __builtin_amdgcn_rcpf(d.a * d.sc);
   return d;
 }
-__device__ __noinline__ int q8_code_exact(float x, double a) {
-  const double xd = 127.0 * (double)x;
-  int q = (int)rint(xd / a);
-  const double r = 2.0 * fma(-(double)q, a, xd);
-  if (r > a || (r == a && (q & 1))) ++q;
-  if (r < -a || (r == -a && (q & 1))) --q;
-  return q;
-}
-// codes of four channels, packed.  (q + 128 as an unsigned byte, whose top bit is then turned.)
+// codes of four channels, packed.  (1.5 * 2^23 + t is rounded to an integer, whose code is then its low byte.)
 __device__ __forceinline__ int q8_code4(const f4& x, const Q8Div& d) {
-  f4 q;
-  bool near = d.mode == 2;
+  constexpr float MAGIC = 0x1.8p23f;
+  f4 t = x, r, e;
+  if (d.sc != 1.f)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] *= d.sc;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float t = x[j] * d.inv;
-    q[j] = rintf(t);
-    near |= fabsf(t - q[j]) > 0.49995f;
+    r[j] = fmaf(t[j], d.inv, MAGIC);
+    e[j] = fabsf(fmaf(t[j], d.inv, MAGIC - r[j]));
   }
-  if (near) {                          // (mode 0: t is 0 or, where x is not finite, NaN: never near)
-    int p = 0;
+  // (inv 0: t is 0 or, where x is not finite, NaN; either way the row's codes are 0)
+  if (fmaxf(fmaxf(e[0], e[1]), fmaxf(e[2], e[3])) > 0.49995f)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) p |= (q8_code_exact(x[j], d.a) & 0xff) << (8 * j);
-    return p;
-  }
-  unsigned p = put_byte<0>(q[0] + 128.f, 0);
-  p = put_byte<1>(q[1] + 128.f, p);
-  p = put_byte<2>(q[2] + 128.f, p);
-  p = put_byte<3>(q[3] + 128.f, p);
-  return d.mode == 0 ? 0 : (int)(p ^ 0x80808080u);
+    for (int j = 0; j < 4; ++j) {
+      const float k = floorf(t[j] * d.inv);
+      const double s = 254.0 * (double)x[j] - (double)(2.f * k + 1.f) * (double)d.a;
+      r[j] = MAGIC + (s > 0.0 || (s == 0.0 && ((int)k & 1)) ? k + 1.f : k);
+    }
+  const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(r[1]), __float_as_uint(r[0]), 0x0c0c0400);
+  const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(r[3]), __float_as_uint(r[2]), 0x0c0c0400);
+  return d.inv == 0.f ? 0 : (int)__builtin_amdgcn_perm(hi, lo, 0x05040100);
 }
 
 // ---- rows: L lanes per row (a power of two <= 64), QPL quads of channels per lane and RT rows held in registers, so that
-// a lane has about four loads in flight; VEC: 16-byte loads
+// a lane has about four loads in flight; VEC: 16-byte loads.  Quantises rows r0, r0 + R, ..; row `rows` becomes zero.
+template <int L, int QPL, int RT, bool VEC, class Put, class PutScale>
+__device__ __forceinline__ void q8_quantize(int l, long r0, int R, long rows, int C, int Cp, const float* x, long cs, Put put,
+                                            PutScale put_scale) {
+  f4 v[RT][QPL];
+  const bool full = VEC && C == 4 * L * QPL;      // every lane has channels: no mask per load
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const long row = r0 + t * R;
+    const float* px = x + row * cs;
+#pragma unroll
+    for (int i = 0; i < QPL; ++i) v[t][i] = f4{0.f, 0.f, 0.f, 0.f};
+    if (full && row < rows)
+#pragma unroll
+      for (int i = 0; i < QPL; ++i) v[t][i] = *reinterpret_cast<const f4*>(px + 4 * (l + i * L));
+#pragma unroll
+    for (int i = 0; i < QPL; ++i) {
+      const int c = 4 * (l + i * L);
+      if (!full && row < rows && c < C) {
+        if (VEC && (c + 3 < C || row + 1 < rows)) {      // (the last row's padding may lie behind the tensor)
+          v[t][i] = *reinterpret_cast<const f4*>(px + c);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c + j < C) v[t][i][j] = px[c + j];
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const long row = r0 + t * R;
+    if (row > rows) break;
+    unsigned am = 0;
+#pragma unroll
+    for (int i = 0; i < QPL; ++i) {
+      if (VEC && (C & 3))            // a last quad that holds the view's padding
+#pragma unroll
+        for (int j = 1; j < 4; ++j)
+          if (4 * (l + i * L) + j >= C) v[t][i][j] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) am = max(am, abs_bits(v[t][i][j]));
+    }
+    am = group_umax<L>(am);
+    const Q8Div d = q8_div(am);
+#pragma unroll
+    for (int i = 0; i < QPL; ++i) {
+      const int c = 4 * (l + i * L);
+      if (c < Cp) put(row, c, 4 * i * L < C ? q8_code4(v[t][i], d) : 0);
+    }
+    if (l == 0) put_scale(row, q8_scale(am));      // (row `rows`: no channel was read, scale 0)
+  }
+}
+// 43200 x 512 18.2 us (6.1 TB/s of reads and writes), 393216 x 32 14.9 us (4.3 TB/s; half of it VALU work: 20 instructions
+// for four codes, the maximum and the scale of a row for eight lanes); few rows 2.4 us, a launch's latency.  Up to 16
+// channels four lanes a row: 172800 x 12 5.4 us, 7.1 with eight.
 template <int L, int QPL, int RT, bool VEC>
 __global__ void __launch_bounds__(256) q8_rows_kernel(long rows, int C, int Cp, const float* x, long cs, int co,
                                                       int8_t* codes, float* scales) {
   constexpr int R = 256 / L;
-  const int l = threadIdx.x % L;
-  for (long r0 = (long)blockIdx.x * (R * RT) + threadIdx.x / L; r0 <= rows; r0 += (long)gridDim.x * (R * RT)) {
-    f4 v[RT][QPL];
+  const int g = L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / L) : threadIdx.x / L;
+  for (long r0 = (long)blockIdx.x * (R * RT) + g; r0 <= rows; r0 += (long)gridDim.x * (R * RT))
+    q8_quantize<L, QPL, RT, VEC>(
+        threadIdx.x % L, r0, R, rows, C, Cp, x + co, cs,
+        [&](long row, int c, int q) { *reinterpret_cast<int*>(codes + row * Cp + c) = q; },
+        [&](long row, float sc) { scales[row] = sc; });
+}
+
+// ---- long rows: 256 lanes each, so that few rows are not one wave's work and many keep few registers (8192 x 2048 14.5 us,
+// 5.8 TB/s, and 17.4 with a wave per row; one row of 4096 2.8 / 6.0)
+template <int QPL, bool VEC>
+__global__ void __launch_bounds__(256) q8_rows_wide_kernel(long rows, int C, int Cp, const float* x, long cs, int co,
+                                                           int8_t* codes, float* scales) {
+  __shared__ unsigned mx[4];
+  const long row = (long)blockIdx.y * 65535 + blockIdx.x;
+  if (row > rows) return;
+  const float* px = x + row * cs + co;
+  f4 v[QPL];
+  unsigned am = 0;
 #pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const long row = r0 + t * R;
-      const float* px = x + row * cs + co;
+  for (int i = 0; i < QPL; ++i) {
+    const int c = 4 * (threadIdx.x + i * 256);
+    v[i] = f4{0.f, 0.f, 0.f, 0.f};
+    if (row < rows && c < C) {
+      if (VEC && c + 3 < C) {
+        v[i] = *reinterpret_cast<const f4*>(px + c);
+      } else {
 #pragma unroll
-      for (int i = 0; i < QPL; ++i) {
-        const int c = 4 * (l + i * L);
-        v[t][i] = f4{0.f, 0.f, 0.f, 0.f};
-        if (row < rows && c < C) {
-          if (VEC && (c + 3 < C || row + 1 < rows)) {      // (the last row's padding may lie behind the tensor)
-            v[t][i] = *reinterpret_cast<const f4*>(px + c);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (c + j < C) v[t][i][j] = px[c + j];
-          }
-        }
+        for (int j = 0; j < 4; ++j)
+          if (c + j < C) v[i][j] = px[c + j];
       }
-    }
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      const long row = r0 + t * R;
-      if (row > rows) break;
-      unsigned am = 0;
-#pragma unroll
-      for (int i = 0; i < QPL; ++i) {
-        if (VEC && (C & 3))            // a last quad that holds the view's padding
-#pragma unroll
-          for (int j = 1; j < 4; ++j)
-            if (4 * (l + i * L) + j >= C) v[t][i][j] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) am = max(am, abs_bits(v[t][i][j]));
-      }
-      am = group_umax<L>(am);
-      const Q8Div d = q8_div(am);
-#pragma unroll
-      for (int i = 0; i < QPL; ++i) {
-        const int c = 4 * (l + i * L);
-        if (c < Cp) *reinterpret_cast<int*>(codes + row * Cp + c) = q8_code4(v[t][i], d);
-      }
-      if (l == 0) scales[row] = q8_scale(am);      // (row `rows`: no channel was read, scale 0)
     }
   }
+#pragma unroll
+  for (int i = 0; i < QPL; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) am = max(am, abs_bits(v[i][j]));
+  am = group_umax<64>(am);
+  if ((threadIdx.x & 63) == 0) mx[threadIdx.x >> 6] = am;
+  __syncthreads();
+  am = max(max(mx[0], mx[1]), max(mx[2], mx[3]));
+  const Q8Div d = q8_div(am);
+#pragma unroll
+  for (int i = 0; i < QPL; ++i) {
+    const int c = 4 * (threadIdx.x + i * 256);
+    if (c < Cp) *reinterpret_cast<int*>(codes + row * Cp + c) = q8_code4(v[i], d);
+  }
+  if (threadIdx.x == 0) scales[row] = q8_scale(am);
 }
 
 // ---- weights: a block takes four output channels (padding channels write zeros), 256 lanes each; lanes run along the
@@ -384,6 +433,92 @@ __global__ void __launch_bounds__(64 * WK) q8_split_kernel(const Q8Conv p) {
 #pragma unroll
     for (int a = 0; a < TM; ++a) epi.store(p, py, n0 + 4 * kq, a, acc[a][b]);
   }
+}
+
+// ---- the same on the fp32 input, in one launch: a block of 16 channels x 16 pixels quantises the input pixels that its
+// taps reach into LDS by itself (rows [scale | codes] as in the kernel below), the weights of its first U steps in flight
+// meanwhile.  Each of the ceil(K / 16) blocks of the same pixels does that work again, so this serves where it is small (up to
+// 32 rows) and a launch counts.  4x4x512 -> 512 9.5 us in a graph, as the two kernels (9.2), but 9.4 / 13.7 called one after
+// the other, where the host's launches are the time; one token of 1024 -> 1024 channels 5.4 / 6.6.
+struct Q8Src {
+  const float* x;            // channel view of the input
+  long cs;
+  int C, cap;                // channels, LDS rows of pixels
+};
+template <int QPL, int RT>
+__global__ void __launch_bounds__(1024) q8_small_kernel(const Q8Conv p, const Q8Src in) {
+  constexpr int WK = 16, KC = 64, HEAD = 16, U = 4;
+  extern __shared__ __attribute__((aligned(16))) char q8_lds[];
+  const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kq = lane >> 4;
+  const Q8Class cl = q8_class(p, blockIdx.z);
+  const int m0 = blockIdx.x * 16, n0 = blockIdx.y * 16;
+  if (m0 >= cl.M) return;                                   // (pixels are counted for the largest class)
+  const int RB = p.Cp + HEAD;
+
+  const int nch = p.Cp / KC, steps = cl.nty * cl.ntx * nch;
+  const int8_t* const wrow = p.w + (long)(n0 + r16) * p.Cp + kq * (KC / 4);
+  auto wload = [&](int s) __attribute__((always_inline)) {
+    const int t = s / nch, ch = s - t * nch, ty = t / cl.ntx, tx = t - ty * cl.ntx;
+    return *reinterpret_cast<const i4*>(wrow + ((long)(cl.ky0 + p.kst * ty) * p.KW + cl.kx0 + p.kst * tx) * p.Kp * p.Cp +
+                                        ch * KC);
+  };
+  i4 fa[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) fa[u] = wk + u * WK < steps ? wload(wk + u * WK) : i4{0, 0, 0, 0};
+
+  // the input pixels [base, base + rows) that the block's taps reach: whole images, rows of one, or part of a row
+  const int hw = cl.GH * cl.GW, HW = p.H * p.W, mh = min(m0 + 15, cl.M - 1);
+  const int nl = m0 / hw, nh = mh / hw;
+  long base = (long)nl * HW;
+  int rows = (nh - nl + 1) * HW;
+  if (nl == nh) {
+    const int rl = m0 - nl * hw, rh = mh - nh * hw, il = rl / cl.GW, ih = rh / cl.GW;
+    const int yb = p.dir < 0 ? cl.nty - 1 : 0, yf = p.dir < 0 ? 0 : cl.nty - 1;
+    const int yl = max(il * p.is + cl.iy0 - yb, 0), yh = min(ih * p.is + cl.iy0 + yf, p.H - 1);
+    int xl = 0, xh = p.W - 1;
+    if (il == ih) {
+      const int xb = p.dir < 0 ? cl.ntx - 1 : 0, xf = p.dir < 0 ? 0 : cl.ntx - 1;
+      xl = max((rl - il * cl.GW) * p.is + cl.ix0 - xb, 0);
+      xh = min((rh - ih * cl.GW) * p.is + cl.ix0 + xf, p.W - 1);
+    }
+    base += (long)yl * p.W + xl;
+    rows = max((yh - yl) * p.W + xh - xl + 1, 0);           // (0: no tap reaches the image)
+  }
+  rows = min(rows, in.cap);
+  for (int r0 = wk; r0 <= rows; r0 += WK * RT)
+    q8_quantize<64, QPL, RT, true>(
+        lane, r0, WK, rows, in.C, p.Cp, in.x + base * in.cs, in.cs,
+        [&](long row, int c, int q) { *reinterpret_cast<int*>(q8_lds + (int)row * RB + HEAD + c) = q; },
+        [&](long row, float sc) { *reinterpret_cast<float*>(q8_lds + (int)row * RB) = sc; });
+  __syncthreads();
+
+  const int m = m0 + r16, n = m / hw, rr = m - n * hw, i = rr / cl.GW, j = rr - i * cl.GW;
+  const int iy = m < cl.M ? i * p.is + cl.iy0 : -(1 << 29), ix = j * p.is + cl.ix0;
+  const int pb = (int)((long)n * HW - base);
+  f4 acc = {0.f, 0.f, 0.f, 0.f};
+  auto step = [&](int s, const i4& a) __attribute__((always_inline)) {
+    const int t = s / nch, ch = s - t * nch, ty = t / cl.ntx, tx = t - ty * cl.ntx;
+    const int yy = iy + p.dir * ty, xx = ix + p.dir * tx;
+    const bool inside = (unsigned)yy < (unsigned)p.H && (unsigned)xx < (unsigned)p.W;
+    const char* row = q8_lds + (inside ? pb + yy * p.W + xx : rows) * RB;
+    const i4 ia = Q8Frag<KC>::mfma(a, *reinterpret_cast<const i4*>(row + HEAD + kq * (KC / 4) + ch * KC), i4{0, 0, 0, 0});
+    const float xs = *reinterpret_cast<const float*>(row);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = fmaf((float)ia[e], xs, acc[e]);
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (wk + u * WK < steps) step(wk + u * WK, fa[u]);
+  for (int s = wk + U * WK; s < steps; s += WK) step(s, wload(s));
+
+  f4* red = reinterpret_cast<f4*>(q8_lds + (in.cap + 1) * RB);
+  if (wk > 0) red[(wk - 1) * 64 + lane] = acc;
+  __syncthreads();
+  if (wk > 0) return;
+#pragma unroll
+  for (int w = 0; w < WK - 1; ++w) acc += red[w * 64 + lane];
+  const Q8Epi<1> epi(p, n0 + 4 * kq);
+  if (m < cl.M) epi.store(p, q8_out(p, cl, n, i, j), n0 + 4 * kq, 0, acc);
 }
 
 // ---- maps: a block computes 16 TM WC channels of a TH x TW tile of pixels (16 TN WP of them) of one image and class.  The
@@ -803,33 +938,17 @@ int q8_conv(Q8Conv p, hipStream_t st) {
   return tde_launch_status();
 }
 
-// what both entries check: geometry within int arithmetic, pointers, alignment of codes and scales
-bool q8_args_ok(const tde_conv_desc_t* d, const int8_t* xc, const float* xs, const int8_t* wc, const float* ws, int relu,
-                const float* y, int cin, int cout, int ocs, int oco) {
-  if (!d || !xc || !xs || !wc || !ws || !y) return false;
-  if (d->N <= 0 || d->H <= 0 || d->W <= 0 || d->OH <= 0 || d->OW <= 0 || d->KH <= 0 || d->KW <= 0 || d->stride <= 0 ||
-      d->pad_top < 0 || d->pad_left < 0 || d->pad_top >= d->KH || d->pad_left >= d->KW)
-    return false;
-  if (cin <= 0 || cin > Q8_MAXC || cout <= 0 || cout > 65535 || d->KH > 64 || d->KW > 64 || d->stride > 64) return false;
-  if ((long)d->N * d->H * d->W > Q8_MAXPIX || (long)d->N * d->OH * d->OW > Q8_MAXPIX) return false;
-  if (ocs <= 0 || oco < 0 || oco + cout > ocs) return false;
-  return (relu == 0 || relu == 1) && tde_aligned16(xc) && tde_aligned16(wc) && tde_aligned16(ws) &&
-         (reinterpret_cast<uintptr_t>(xs) & 3u) == 0 && (reinterpret_cast<uintptr_t>(y) & 3u) == 0;
+bool q8_rows_ok(int rows, int C, const float* x, int x_cstride, int x_coff, const int8_t* codes, const float* scales) {
+  return rows > 0 && rows <= (1 << 30) && C > 0 && C <= Q8_MAXC && x && codes && scales && tde_aligned16(codes) &&
+         x_coff >= 0 && x_coff + C <= x_cstride;
 }
-
-}  // namespace
-
-extern "C" {
-
-int tde_q8_row_bytes(int C) { return C > 0 && C <= Q8_MAXC ? q8_row(C) : 0; }
-
-int tde_q8_rows(int rows, int C, const float* x, int x_cstride, int x_coff, int8_t* codes, float* scales, void* stream) {
-  tde_clear_error();
-  TDE_CHECK_ARG(rows > 0 && rows <= (1 << 30) && C > 0 && C <= Q8_MAXC && x && codes && scales && tde_aligned16(codes) &&
-                x_coff >= 0 && x_coff + C <= x_cstride);
+// 16-byte loads of a channel view (a row's padding up to a multiple of four channels is read)
+bool q8_rows_vec(int C, const float* x, int x_cstride, int x_coff) {
+  return tde_aligned16(x) && x_cstride % 4 == 0 && x_coff % 4 == 0 && x_coff + (C + 3) / 4 * 4 <= x_cstride;
+}
+int q8_rows(int rows, int C, const float* x, int x_cstride, int x_coff, int8_t* codes, float* scales, hipStream_t st) {
   const int Cp = q8_row(C), nq = Cp / 4;
-  const bool vec = tde_aligned16(x) && x_cstride % 4 == 0 && x_coff % 4 == 0 && x_coff + (C + 3) / 4 * 4 <= x_cstride;
-  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool vec = q8_rows_vec(C, x, x_cstride, x_coff);
 #define R(LL, QQ, TT)                                                                                                 \
   do {                                                                                                                \
     const long nb = tde_cdiv((long)rows + 1, 256 / LL * TT);                                                          \
@@ -841,17 +960,127 @@ int tde_q8_rows(int rows, int C, const float* x, int x_cstride, int x_coff, int8
       hipLaunchKernelGGL((q8_rows_kernel<LL, QQ, TT, false>), grid, dim3(256), 0, st, (long)rows, C, Cp, x,           \
                          (long)x_cstride, x_coff, codes, scales);                                                     \
   } while (0)
+#define W(QQ)                                                                                                          \
+  do {                                                                                                                 \
+    const long nr = (long)rows + 1;                                                                                    \
+    const dim3 grid((unsigned)(nr < 65535 ? nr : 65535), (unsigned)((nr + 65534) / 65535));                            \
+    if (vec)                                                                                                           \
+      hipLaunchKernelGGL((q8_rows_wide_kernel<QQ, true>), grid, dim3(256), 0, st, (long)rows, C, Cp, x,                \
+                         (long)x_cstride, x_coff, codes, scales);                                                      \
+    else                                                                                                               \
+      hipLaunchKernelGGL((q8_rows_wide_kernel<QQ, false>), grid, dim3(256), 0, st, (long)rows, C, Cp, x,               \
+                         (long)x_cstride, x_coff, codes, scales);                                                      \
+  } while (0)
   const bool many = rows >= 1 << 15;      // one row per lane group in flight where there are few rows
-  if (nq <= 8) { if (many) R(8, 1, 4); else R(8, 1, 1); }
+  if (C <= 16) { if (many) R(4, 2, 4); else R(4, 2, 1); }
+  else if (nq <= 8) { if (many) R(8, 1, 4); else R(8, 1, 1); }
   else if (nq <= 16) { if (many) R(16, 1, 4); else R(16, 1, 1); }
   else if (nq <= 32) { if (many) R(32, 1, 4); else R(32, 1, 1); }
   else if (nq <= 64) { if (many) R(64, 1, 4); else R(64, 1, 1); }
   else if (nq <= 128) R(64, 2, 1);
-  else if (nq <= 256) R(64, 4, 1);
-  else if (nq <= 512) R(64, 8, 1);
-  else R(64, 16, 1);
+  else if (nq <= 256) W(1);
+  else if (nq <= 512) W(2);
+  else W(4);
+#undef W
 #undef R
   return tde_launch_status();
+}
+
+// The small kernel's LDS rows for a geometry, 0: it does not serve.  A block's 16 pixels lie in one image, on at most
+// ceil(15 / GW) + 1 rows of its grid, or in several images.
+int q8_small_rows(const Q8Conv& p) {
+  const int s = p.deconv ? p.os : 1, GH = (p.OH + s - 1) / s, GW = (p.OW + s - 1) / s;
+  const long tiles = ((long)tde_cdiv((long)p.N * GH * GW, 16)) * tde_cdiv(p.K, 16) * s * s;
+  if (p.Cp % 64 != 0 || p.Cp > 1024 || tiles > 256) return 0;
+  const int gh = p.OH / s > 0 ? p.OH / s : 1, gw = p.OW / s > 0 ? p.OW / s : 1;      // the smallest class that has pixels
+  const int nty = (p.KH + p.kst - 1) / p.kst, ntx = (p.KW + p.kst - 1) / p.kst;
+  const long HW = (long)p.H * p.W;
+  long rows;
+  if (GH == 1 && gh == 1) rows = (long)(nty < p.H ? nty : p.H) * p.W < (long)(nty - 1) * p.W + 15 * p.is + ntx
+                                     ? (long)(nty < p.H ? nty : p.H) * p.W : (long)(nty - 1) * p.W + 15 * p.is + ntx;
+  else {
+    const long ny = (long)((15 + gw - 1) / gw) * p.is + nty;
+    rows = (ny < p.H ? ny : p.H) * p.W;
+  }
+  if (p.N > 1) {
+    const long ni = (15 + gh * gw - 1) / (gh * gw) + 1, all = (ni < p.N ? ni : p.N) * HW;
+    if (all > rows) rows = all;
+  }
+  return rows <= 32 ? (int)rows : 0;
+}
+int q8_small_launch(const Q8Conv& p, const float* x, long cs, int C, int cap, hipStream_t st) {
+  const int s = p.deconv ? p.os : 1, GH = (p.OH + s - 1) / s, GW = (p.OW + s - 1) / s;
+  const dim3 grid(tde_cdiv((long)p.N * GH * GW, 16), tde_cdiv(p.K, 16), s * s);
+  const Q8Src in{x, cs, C, cap};
+  const int lds = (cap + 1) * (p.Cp + 16) + 15 * 1024;
+  if (p.Cp <= 256) hipLaunchKernelGGL((q8_small_kernel<1, 4>), grid, dim3(1024), lds, st, p, in);
+  else if (p.Cp <= 512) hipLaunchKernelGGL((q8_small_kernel<2, 2>), grid, dim3(1024), lds, st, p, in);
+  else hipLaunchKernelGGL((q8_small_kernel<4, 1>), grid, dim3(1024), lds, st, p, in);
+  return tde_launch_status();
+}
+
+// what the entries check: geometry within int arithmetic, pointers, alignment of codes and scales
+bool q8_geometry_ok(const tde_conv_desc_t* d, int cin, int cout) {
+  if (d->N <= 0 || d->H <= 0 || d->W <= 0 || d->OH <= 0 || d->OW <= 0 || d->KH <= 0 || d->KW <= 0 || d->stride <= 0 ||
+      d->pad_top < 0 || d->pad_left < 0 || d->pad_top >= d->KH || d->pad_left >= d->KW)
+    return false;
+  if (cin <= 0 || cin > Q8_MAXC || cout <= 0 || cout > 65535 || d->KH > 64 || d->KW > 64 || d->stride > 64) return false;
+  return (long)d->N * d->H * d->W <= Q8_MAXPIX && (long)d->N * d->OH * d->OW <= Q8_MAXPIX;
+}
+bool q8_args_ok(const tde_conv_desc_t* d, const int8_t* xc, const float* xs, const int8_t* wc, const float* ws, int relu,
+                const float* y, int cin, int cout, int ocs, int oco) {
+  if (!wc || !ws || !y || !q8_geometry_ok(d, cin, cout)) return false;
+  if (ocs <= 0 || oco < 0 || oco + cout > ocs) return false;
+  return (relu == 0 || relu == 1) && tde_aligned16(xc) && tde_aligned16(wc) && tde_aligned16(ws) &&
+         (reinterpret_cast<uintptr_t>(xs) & 3u) == 0 && (reinterpret_cast<uintptr_t>(y) & 3u) == 0;
+}
+
+Q8Conv q8_conv_args(const tde_conv_desc_t* d, const int8_t* x_codes, const float* x_scales, const int8_t* w_codes,
+                    const float* w_scales, const float* bias, int relu, float* y) {
+  Q8Conv p{};
+  p.N = d->N; p.H = d->H; p.W = d->W; p.OH = d->OH; p.OW = d->OW;
+  p.Cp = q8_row(d->w_cin); p.K = d->K; p.Kp = q8_cols(d->K);
+  p.KH = d->KH; p.KW = d->KW; p.pt = d->pad_top; p.pl = d->pad_left;
+  p.is = d->stride; p.os = 1; p.dir = 1; p.kst = 1; p.deconv = 0;
+  p.x = x_codes; p.xs = x_scales; p.w = w_codes; p.ws = w_scales; p.bias = bias; p.y = y;
+  p.ycs = d->y_cstride; p.yco = d->y_coff; p.relu = relu;
+  p.vec = tde_aligned16(y) && p.ycs % 4 == 0 && p.yco % 4 == 0;
+  return p;
+}
+Q8Conv q8_deconv_args(const tde_conv_desc_t* d, const int8_t* x_codes, const float* x_scales, const int8_t* w_codes,
+                      const float* w_scales, const float* bias, int relu, float* y_big) {
+  Q8Conv p{};
+  p.N = d->N; p.H = d->OH; p.W = d->OW; p.OH = d->H; p.OW = d->W;
+  p.Cp = q8_row(d->K); p.K = d->C; p.Kp = q8_cols(d->C);
+  p.KH = d->KH; p.KW = d->KW; p.pt = d->pad_top; p.pl = d->pad_left;
+  p.is = 1; p.os = d->stride; p.dir = -1; p.kst = d->stride; p.deconv = 1;
+  p.x = x_codes; p.xs = x_scales; p.w = w_codes; p.ws = w_scales; p.bias = bias; p.y = y_big;
+  p.ycs = d->x_cstride; p.yco = d->x_coff; p.relu = relu;
+  p.vec = tde_aligned16(y_big) && p.ycs % 4 == 0 && p.yco % 4 == 0;
+  return p;
+}
+
+// from the fp32 input (its channel view): in one launch, or quantised into codes and scales first
+int q8_conv_f32(const Q8Conv& p, const float* x, int C, int cs, int co, int8_t* codes, float* scales, hipStream_t st) {
+  TDE_CHECK_ARG(x && co >= 0 && co + C <= cs);
+  const int cap = q8_rows_vec(C, x, cs, co) ? q8_small_rows(p) : 0;
+  if (cap > 0) return q8_small_launch(p, x + co, cs, C, cap, st);
+  const int rows = p.N * p.H * p.W;
+  TDE_CHECK_ARG(q8_rows_ok(rows, C, x, cs, co, codes, scales));
+  const int rc = q8_rows(rows, C, x, cs, co, codes, scales, st);
+  return rc != TDE_OK ? rc : q8_conv(p, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int tde_q8_row_bytes(int C) { return C > 0 && C <= Q8_MAXC ? q8_row(C) : 0; }
+
+int tde_q8_rows(int rows, int C, const float* x, int x_cstride, int x_coff, int8_t* codes, float* scales, void* stream) {
+  tde_clear_error();
+  TDE_CHECK_ARG(q8_rows_ok(rows, C, x, x_cstride, x_coff, codes, scales));
+  return q8_rows(rows, C, x, x_cstride, x_coff, codes, scales, static_cast<hipStream_t>(stream));
 }
 
 size_t tde_q8_weights_size(int taps, int cin, int K) {
@@ -877,35 +1106,49 @@ int tde_q8_conv2d_bias_act(const tde_conv_desc_t* d, const int8_t* x_codes, cons
                            const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y,
                            void* stream) {
   tde_clear_error();
-  TDE_CHECK_ARG(d != nullptr);
+  TDE_CHECK_ARG(d != nullptr && x_codes && x_scales);
   TDE_CHECK_ARG(q8_args_ok(d, x_codes, x_scales, w_codes, w_scales, relu, y, d->w_cin, d->K, d->y_cstride, d->y_coff));
-  Q8Conv p{};
-  p.N = d->N; p.H = d->H; p.W = d->W; p.OH = d->OH; p.OW = d->OW;
-  p.Cp = q8_row(d->w_cin); p.K = d->K; p.Kp = q8_cols(d->K);
-  p.KH = d->KH; p.KW = d->KW; p.pt = d->pad_top; p.pl = d->pad_left;
-  p.is = d->stride; p.os = 1; p.dir = 1; p.kst = 1; p.deconv = 0;
-  p.x = x_codes; p.xs = x_scales; p.w = w_codes; p.ws = w_scales; p.bias = bias; p.y = y;
-  p.ycs = d->y_cstride; p.yco = d->y_coff; p.relu = relu;
-  p.vec = tde_aligned16(y) && p.ycs % 4 == 0 && p.yco % 4 == 0;
-  return q8_conv(p, static_cast<hipStream_t>(stream));
+  return q8_conv(q8_conv_args(d, x_codes, x_scales, w_codes, w_scales, bias, relu, y), static_cast<hipStream_t>(stream));
 }
 
 int tde_q8_deconv2d_bias_act(const tde_conv_desc_t* d, const int8_t* x_codes, const float* x_scales,
                              const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y_big,
                              void* stream) {
   tde_clear_error();
-  TDE_CHECK_ARG(d != nullptr);
+  TDE_CHECK_ARG(d != nullptr && x_codes && x_scales);
   // the virtual conv's x is the output, its y the input
   TDE_CHECK_ARG(q8_args_ok(d, x_codes, x_scales, w_codes, w_scales, relu, y_big, d->K, d->C, d->x_cstride, d->x_coff));
-  Q8Conv p{};
-  p.N = d->N; p.H = d->OH; p.W = d->OW; p.OH = d->H; p.OW = d->W;
-  p.Cp = q8_row(d->K); p.K = d->C; p.Kp = q8_cols(d->C);
-  p.KH = d->KH; p.KW = d->KW; p.pt = d->pad_top; p.pl = d->pad_left;
-  p.is = 1; p.os = d->stride; p.dir = -1; p.kst = d->stride; p.deconv = 1;
-  p.x = x_codes; p.xs = x_scales; p.w = w_codes; p.ws = w_scales; p.bias = bias; p.y = y_big;
-  p.ycs = d->x_cstride; p.yco = d->x_coff; p.relu = relu;
-  p.vec = tde_aligned16(y_big) && p.ycs % 4 == 0 && p.yco % 4 == 0;
-  return q8_conv(p, static_cast<hipStream_t>(stream));
+  return q8_conv(q8_deconv_args(d, x_codes, x_scales, w_codes, w_scales, bias, relu, y_big),
+                 static_cast<hipStream_t>(stream));
+}
+
+int tde_q8_one_launch(const tde_conv_desc_t* d, int deconv) {
+  if (!d || !q8_geometry_ok(d, deconv ? d->K : d->w_cin, deconv ? d->C : d->K)) return 0;
+  const int cs = deconv ? d->y_cstride : d->x_cstride, co = deconv ? d->y_coff : d->x_coff;
+  if (!q8_rows_vec(deconv ? d->K : d->w_cin, nullptr, cs, co)) return 0;
+  const Q8Conv p = deconv ? q8_deconv_args(d, nullptr, nullptr, nullptr, nullptr, nullptr, 0, nullptr)
+                          : q8_conv_args(d, nullptr, nullptr, nullptr, nullptr, nullptr, 0, nullptr);
+  return q8_small_rows(p) > 0;
+}
+
+int tde_q8_conv2d_f32_bias_act(const tde_conv_desc_t* d, const float* x, int8_t* x_codes, float* x_scales,
+                               const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y,
+                               void* stream) {
+  tde_clear_error();
+  TDE_CHECK_ARG(d != nullptr);
+  TDE_CHECK_ARG(q8_args_ok(d, x_codes, x_scales, w_codes, w_scales, relu, y, d->w_cin, d->K, d->y_cstride, d->y_coff));
+  return q8_conv_f32(q8_conv_args(d, x_codes, x_scales, w_codes, w_scales, bias, relu, y), x, d->w_cin, d->x_cstride,
+                     d->x_coff, x_codes, x_scales, static_cast<hipStream_t>(stream));
+}
+
+int tde_q8_deconv2d_f32_bias_act(const tde_conv_desc_t* d, const float* x_small, int8_t* x_codes, float* x_scales,
+                                 const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y_big,
+                                 void* stream) {
+  tde_clear_error();
+  TDE_CHECK_ARG(d != nullptr);
+  TDE_CHECK_ARG(q8_args_ok(d, x_codes, x_scales, w_codes, w_scales, relu, y_big, d->K, d->C, d->x_cstride, d->x_coff));
+  return q8_conv_f32(q8_deconv_args(d, x_codes, x_scales, w_codes, w_scales, bias, relu, y_big), x_small, d->K,
+                     d->y_cstride, d->y_coff, x_codes, x_scales, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -172,13 +172,13 @@ class Conv8:
         if len(shape) == 2 and (self.kh, self.kw, self.stride) == (1, 1, 1):
             return 1, 1, shape[0], torch.Size((shape[0], self.K))
         if len(shape) != 4:
-            raise ValueError(f"x must be [N, H, W, C], or [M, C] for a 1x1 stride-1 conv, got {shape}")
+            raise ValueError(f"x must be [N, H, W, C], or [M, C] for a 1x1 stride-1 conv, got {tuple(shape)}")
         N, H, W = shape[:3]
         return N, H, W, torch.Size((N,) + self.out_size(H, W) + (self.K,))
 
-    def _make_desc(self, N, H, W, ocs):
-        """The conv descriptor of a batch whose output has pixel stride ocs (a transposed conv's is that of its virtual
-        forward conv)."""
+    def _make_desc(self, N, H, W, ics, ocs):
+        """The conv descriptor of a batch whose input and output have pixel strides ics and ocs (a transposed conv's is
+        that of its virtual forward conv), and whether the call is one launch if the input starts on 16 bytes."""
         OH, OW = self.out_size(H, W)
         d = ConvDesc()
         big, small = ((OH, OW), (H, W)) if self.deconv else ((H, W), (OH, OW))
@@ -187,30 +187,37 @@ class Conv8:
         d.w_cin = d.C
         d.KH, d.KW, d.stride = self.kh, self.kw, self.stride
         d.pad_top, d.pad_left = same_pad(d.H, self.kh, self.stride)[1], same_pad(d.W, self.kw, self.stride)[1]
-        d.x_cstride, d.y_cstride = (ocs, d.K) if self.deconv else (d.C, ocs)
-        return d
+        d.x_cstride, d.y_cstride = (ocs, ics) if self.deconv else (ics, ocs)
+        return d, bool(_lib.load().tde_q8_one_launch(ctypes.byref(d), self.deconv))
 
     quantize = staticmethod(quantize_rows)      # the Rows8 of an input, for several layers that read it
 
     def __call__(self, x, out=None):
         """x: fp32 [N, H, W, Cin] channel view (or its Rows8), or [M, Cin] rows for a 1x1 stride-1 conv.  Returns
         [N, OH, OW, Cout] ([M, Cout]), written into the channel view `out` if given."""
-        if isinstance(x, Rows8):
-            N, H, W, oshape = self._geometry(x.shape)
-            _check(x.buffer, "x", torch.int8)
-            x8 = x
-        else:
-            N, H, W, oshape = self._geometry(tuple(getattr(x, "shape", (0,))))
-            x8 = quantize_rows(x)
-        y = _out(out, oshape, x8.buffer.device)
+        rows8 = isinstance(x, Rows8)
+        _check(x.buffer if rows8 else x, "x", torch.int8 if rows8 else torch.float32)
+        ics = self.cin if rows8 else _rows(x, "x")[2]
+        N, H, W, oshape = self._geometry(x.shape)
+        y = _out(out, oshape, x.buffer.device if rows8 else x.device)
         rows, _, ocs = _rows(y, "out")
         if rows:
-            xc, xs = x8.pointers()
             lib = _lib.load()
-            fn = lib.tde_q8_deconv2d_bias_act if self.deconv else lib.tde_q8_conv2d_bias_act
-            _lib.check(fn(ctypes.byref(self._desc(N, H, W, ocs)), xc, xs, self.codes.data_ptr(), self.scales.data_ptr(),
-                          None if self.bias is None else self.bias.data_ptr(), self.relu, y.data_ptr(),
-                          _lib.raw_stream(y.get_device())), "Conv8")
+            desc, one = self._desc(N, H, W, ics, ocs)
+            tail = (self.codes.data_ptr(), self.scales.data_ptr(), None if self.bias is None else self.bias.data_ptr(),
+                    self.relu, y.data_ptr(), _lib.raw_stream(y.get_device()))
+            if rows8:
+                fn = lib.tde_q8_deconv2d_bias_act if self.deconv else lib.tde_q8_conv2d_bias_act
+                rc = fn(ctypes.byref(desc), *x.pointers(), *tail)
+            else:
+                fn = lib.tde_q8_deconv2d_f32_bias_act if self.deconv else lib.tde_q8_conv2d_f32_bias_act
+                px = x.data_ptr()
+                if one and px % 16 == 0:
+                    rc = fn(ctypes.byref(desc), px, None, None, *tail)
+                else:
+                    x8 = Rows8(x.shape, x.device)
+                    rc = fn(ctypes.byref(desc), px, *x8.pointers(), *tail)
+            _lib.check(rc, "Conv8")
         return y
 
 

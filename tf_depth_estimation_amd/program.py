@@ -15,6 +15,7 @@ accumulate into the ParamChunk's flat gradient buffer, which the trainer zeroes 
 network called twice with shared variables (train_depth_then_cam_lr.py:130-136) sums both calls like
 TF does.
 """
+import collections
 import ctypes
 
 import numpy as np
@@ -51,6 +52,10 @@ class View:
     @property
     def W(self):
         return self.buf.W
+
+
+def _view_key(v):
+    return v.buf.name, v.coff, v.creal
 
 
 class Op:
@@ -393,6 +398,7 @@ class NetProgram:
         self.bn_sync, self.bn_world = None, 1
         self._bn_sums = {}
         self._folded = None     # layer -> (weights with BN folded in, bias); see fold_bn()
+        self._readers = collections.Counter(_view_key(op.src) for op in spec.ops if isinstance(op, ConvBN))
         self._tape8 = {}        # batch -> buffers shared by the runs with an 8-bit tape (shared_tape8)
         # filter-gradient overlap (enable_wgrad_overlap): side stream, its workspace per batch, dz ring
         # (every conv layer but the first of forward sends its filter gradient to the side stream, each behind one event,
@@ -672,7 +678,7 @@ class NetProgram:
         if conv8 is not None and not fold_bn:
             raise ValueError("conv8 needs fold_bn")
         run.tape_ready = False
-        rows8 = {}          # view -> its 8-bit rows: a view is complete before its first reader (static schedule)
+        rows8 = {}          # view with several readers -> its 8-bit rows (it is complete before the first: static schedule)
         N = run.N
         lib = _lib.load()
         st = _lib.stream_ptr()
@@ -702,12 +708,15 @@ class NetProgram:
             if self.pre_op is not None and isinstance(op, (ConvBN, Head)):
                 self.pre_op(self, i)
             if isinstance(op, ConvBN) and conv8 is not None:
-                key = (op.src.buf.name, op.src.coff, op.src.creal)
+                key = _view_key(op.src)
                 layer = conv8[op.layer]
-                if key not in rows8:
-                    rows8[key] = layer.quantize(run.view_tensor(op.src)[..., :op.src.creal])
+                src = run.view_tensor(op.src)[..., :op.src.creal]
+                if self._readers[key] > 1:
+                    if key not in rows8:
+                        rows8[key] = layer.quantize(src)
+                    src = rows8[key]
                 with self._span("conv_fwd", conv_flops(op, N), conv_bytes(op, N)):
-                    layer(rows8[key], out=run.view_tensor(op.dst))
+                    layer(src, out=run.view_tensor(op.dst))
             elif isinstance(op, ConvBN):
                 if i in split_todo:
                     # one split launch for every pending layer whose weights are final by now (all of them
