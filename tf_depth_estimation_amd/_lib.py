@@ -250,6 +250,12 @@ def raw_stream(device_index):
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
+def current_device():
+    """Index of the current device, for callers that hold a GPU tensor (torch.cuda.current_device() without its test for
+    initialisation)."""
+    return torch._C._cuda_getDevice()
+
+
 _hip = None
 _own_streams = []
 

@@ -32,8 +32,8 @@ MAX_CHANNELS = 4096   # of a Conv8 input
 def _check(t, name, dtype=torch.float32):
     if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda:
         raise ValueError(f"{name} must be a {str(dtype).split('.')[-1]} tensor on the GPU")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{name} is on {t.device}, not on the current device (cuda:{torch.cuda.current_device()})")
+    if t.get_device() != _lib.current_device():
+        raise ValueError(f"{name} is on {t.device}, not on the current device (cuda:{_lib.current_device()})")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: 8-bit operators record none (detach it, or use torch.no_grad())")
 
@@ -60,9 +60,18 @@ def _rows(t, name):
     return rows, C, cs
 
 
+@functools.lru_cache(maxsize=1024)
+def _strides(shape):
+    st, n = [], 1
+    for s in reversed(shape):
+        st.append(n)
+        n *= max(s, 1)
+    return tuple(reversed(st))
+
+
 def _out(out, shape, device, name="out"):
-    if out is None:
-        return torch.empty(shape, dtype=torch.float32, device=device)
+    if out is None:      # (empty_strided: 1.3 us, torch.empty of a torch.Size 2.1)
+        return torch.empty_strided(shape, _strides(shape), dtype=torch.float32, device=device)
     _check(out, name)
     if out.shape != shape:
         raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(out.shape)}")
