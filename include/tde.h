@@ -310,7 +310,8 @@ int tde_q8_deconv2d_bias_act(const tde_conv_desc_t* d, const int8_t* x_codes, co
                              void* stream);
 /* tde_q8_rows and the conv in one call: `d` also names the fp32 input's channel view (as for tde_conv2d_fwd_bias_act /
  * tde_deconv2d_fwd_bias_act, without their alignments).  x_codes / x_scales: buffers for the rows' codes.  Where
- * tde_q8_one_launch(d, deconv) is 1 and x starts on 16 bytes the call is one launch that uses neither (they may be NULL). */
+ * tde_q8_one_launch(d, deconv) is 1, x starts on 16 bytes and the rows of x and y (pixels times pixel stride from the
+ * pointer on) lie apart, the call is one launch that uses neither (they may be NULL).  y may lie on x otherwise. */
 int tde_q8_one_launch(const tde_conv_desc_t* d, int deconv);
 int tde_q8_conv2d_f32_bias_act(const tde_conv_desc_t* d, const float* x, int8_t* x_codes, float* x_scales,
                                const int8_t* w_codes, const float* w_scales, const float* bias, int relu, float* y,

@@ -183,6 +183,13 @@ def test_conv_of_few_pixels_in_one_launch(N, H, W, C, K, k, s, deconv):
     odd = torch.empty(N * H * W * (C + 1) + 1, device="cuda")[1:].view(N, H, W, C + 1)[..., :C]
     odd.copy_(xv)
     assert (np.abs(conv(odd).cpu().numpy() - ref) <= conv_bound(mag, k * k)).all()
+    # the output on the input itself, and on other channels of its buffer
+    if k == 1 and s == 1 and not deconv:
+        both = torch.zeros(N * H * W, (C + 3) // 4 * 4 + K, device="cuda").view(N, H, W, -1)
+        for at in (0, (C + 3) // 4 * 4):
+            both[..., :C] = dev(x)
+            conv(both[..., :C], out=both[..., at:at + K])
+            assert (np.abs(both[..., at:at + K].cpu().numpy() - ref) <= conv_bound(mag, 1)).all(), at
     # a bad pixel shows in exactly the outputs that read it
     bad = x.copy()
     bad[-1, -1, -1, C // 2] = np.inf

@@ -109,8 +109,11 @@ def test_conv_arguments(p):
         assert fn(None, p, p, p, p, p, None, 1, p, None) == -1
 
 
-def test_one_launch():
+def test_one_launch(p):
     lib = _lib.load()
+    d = desc(H=1, W=1, OH=1, OW=1, KH=1, KW=1, pad_top=0, pad_left=0, C=64, w_cin=64, K=64, x_cstride=64, y_cstride=64)
+    assert lib.tde_q8_one_launch(d, 0) == 1        # ... but not onto the input: then the codes are needed
+    assert lib.tde_q8_conv2d_f32_bias_act(d, p, None, None, p, p, None, 1, p, None) == -1
     small = dict(H=4, W=4, OH=4, OW=4, C=64, w_cin=64, K=64, x_cstride=64, y_cstride=64)
     assert [lib.tde_q8_one_launch(desc(**{**small, **kw}), dec) for kw, dec in (
         (dict(), 0), (dict(), 1), (dict(x_cstride=66), 0), (dict(x_coff=2, x_cstride=68), 0), (dict(w_cin=32), 0),

@@ -1060,11 +1060,14 @@ Q8Conv q8_deconv_args(const tde_conv_desc_t* d, const int8_t* x_codes, const flo
   return p;
 }
 
-// from the fp32 input (its channel view): in one launch, or quantised into codes and scales first
+// from the fp32 input (its channel view): in one launch, or quantised into codes and scales first (always where the output
+// may lie on the input, which a block of one launch could still have to read)
 int q8_conv_f32(const Q8Conv& p, const float* x, int C, int cs, int co, int8_t* codes, float* scales, hipStream_t st) {
   TDE_CHECK_ARG(x && co >= 0 && co + C <= cs);
   const int cap = q8_rows_vec(C, x, cs, co) ? q8_small_rows(p) : 0;
-  if (cap > 0) return q8_small_launch(p, x + co, cs, C, cap, st);
+  const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), x1 = x0 + (size_t)p.N * p.H * p.W * cs * sizeof(float);
+  const uintptr_t y0 = reinterpret_cast<uintptr_t>(p.y), y1 = y0 + (size_t)p.N * p.OH * p.OW * p.ycs * sizeof(float);
+  if (cap > 0 && (x1 <= y0 || y1 <= x0)) return q8_small_launch(p, x + co, cs, C, cap, st);
   const int rows = p.N * p.H * p.W;
   TDE_CHECK_ARG(q8_rows_ok(rows, C, x, cs, co, codes, scales));
   const int rc = q8_rows(rows, C, x, cs, co, codes, scales, st);

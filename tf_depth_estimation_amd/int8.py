@@ -203,7 +203,7 @@ class Conv8:
 
     def __call__(self, x, out=None):
         """x: fp32 [N, H, W, Cin] channel view (or its Rows8), or [M, Cin] rows for a 1x1 stride-1 conv.  Returns
-        [N, OH, OW, Cout] ([M, Cout]), written into the channel view `out` if given."""
+        [N, OH, OW, Cout] ([M, Cout]), written into the channel view `out` if given (which may lie on x)."""
         rows8 = isinstance(x, Rows8)
         _check(x.buffer if rows8 else x, "x", torch.int8 if rows8 else torch.float32)
         ics = self.cin if rows8 else _rows(x, "x")[2]
@@ -220,8 +220,9 @@ class Conv8:
                 rc = fn(ctypes.byref(desc), *x.pointers(), *tail)
             else:
                 fn = lib.tde_q8_deconv2d_f32_bias_act if self.deconv else lib.tde_q8_conv2d_f32_bias_act
-                px = x.data_ptr()
-                if one and px % 16 == 0:
+                px, py = x.data_ptr(), y.data_ptr()
+                apart = px + 4 * N * H * W * ics <= py or py + 4 * rows * ocs <= px
+                if one and px % 16 == 0 and apart:      # (an output on the input: its rows are quantised first)
                     rc = fn(ctypes.byref(desc), px, None, None, *tail)
                 else:
                     x8 = Rows8(x.shape, x.device)
