@@ -21,8 +21,15 @@ inline int q8_cols(int K) { return (K + 15) / 16 * 16; }
 constexpr int Q8_MAXC = 4096;
 constexpr long Q8_MAXPIX = 1 << 26;      // pixels of an input or output: a grid's threads stay below 2^32
 
+// a / 127, correctly rounded: the product with the rounded reciprocal and one step with its exact remainder.  Below 2^-100,
+// where the remainder may be no normal number, by way of fp64: a's 24 bits over 127 never come so near the middle between
+// two fp32 numbers that the fp64 rounding could pass it (24 + 7 bits of numerator and denominator, 53 of quotient).
 __device__ __forceinline__ float q8_scale(unsigned amax_bits) {
-  return amax_bits >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __uint_as_float(amax_bits) / 127.f;
+  const float a = __uint_as_float(amax_bits);
+  if (amax_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+  if (a < 0x1p-100f) return (float)((double)a / 127.0);
+  const float q = a * (1.f / 127.f);
+  return fmaf(fmaf(-q, 127.f, a), 1.f / 127.f, q);
 }
 
 // rne(127 x / a), exact.  The fp32 estimate t = x * (127 / a) is off by less than 4e-5 (three roundings of at most 127),
@@ -66,39 +73,33 @@ __device__ __forceinline__ int q8_code4(const f4& x, const Q8Div& d) {
 }
 
 // ---- rows: L lanes per row (a power of two <= 64), QPL quads of channels per lane and RT rows held in registers, so that
-// a lane has about four loads in flight; VEC: 16-byte loads.  Quantises rows r0, r0 + R, ..; row `rows` becomes zero.
-template <int L, int QPL, int RT, bool VEC, class Put, class PutScale>
-__device__ __forceinline__ void q8_quantize(int l, long r0, int R, long rows, int C, int Cp, const float* x, long cs, Put put,
-                                            PutScale put_scale) {
+// a lane has about four loads in flight; VEC: 16-byte loads.  Quantises rows row, row + R, .. (px: this lane's first quad of
+// the first, step: elements from one to the next); row `rows` becomes zero.  IN: all of them lie before the last row.
+template <int L, int QPL, int RT, bool VEC, bool IN, class Put, class PutScale>
+__device__ __forceinline__ void q8_quantize(int l, int row, int R, int rows, int C, int Cp, const float* px, long step,
+                                            Put put, PutScale put_scale) {
   f4 v[RT][QPL];
-  const bool full = VEC && C == 4 * L * QPL;      // every lane has channels: no mask per load
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    const long row = r0 + t * R;
-    const float* px = x + row * cs;
-#pragma unroll
-    for (int i = 0; i < QPL; ++i) v[t][i] = f4{0.f, 0.f, 0.f, 0.f};
-    if (full && row < rows)
-#pragma unroll
-      for (int i = 0; i < QPL; ++i) v[t][i] = *reinterpret_cast<const f4*>(px + 4 * (l + i * L));
+    const float* pt = px + t * step;
 #pragma unroll
     for (int i = 0; i < QPL; ++i) {
       const int c = 4 * (l + i * L);
-      if (!full && row < rows && c < C) {
-        if (VEC && (c + 3 < C || row + 1 < rows)) {      // (the last row's padding may lie behind the tensor)
-          v[t][i] = *reinterpret_cast<const f4*>(px + c);
+      v[t][i] = f4{0.f, 0.f, 0.f, 0.f};
+      if ((IN || row + t * R < rows) && c < C) {
+        if (VEC && (IN || c + 3 < C || row + t * R + 1 < rows)) {      // (the last row's padding may lie behind the tensor)
+          v[t][i] = *reinterpret_cast<const f4*>(pt + 4 * i * L);
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (c + j < C) v[t][i][j] = px[c + j];
+            if (c + j < C) v[t][i][j] = pt[4 * i * L + j];
         }
       }
     }
   }
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
-    const long row = r0 + t * R;
-    if (row > rows) break;
+    if (!IN && row + t * R > rows) break;
     unsigned am = 0;
 #pragma unroll
     for (int i = 0; i < QPL; ++i) {
@@ -112,26 +113,28 @@ __device__ __forceinline__ void q8_quantize(int l, long r0, int R, long rows, in
     am = group_umax<L>(am);
     const Q8Div d = q8_div(am);
 #pragma unroll
-    for (int i = 0; i < QPL; ++i) {
-      const int c = 4 * (l + i * L);
-      if (c < Cp) put(row, c, 4 * i * L < C ? q8_code4(v[t][i], d) : 0);
-    }
-    if (l == 0) put_scale(row, q8_scale(am));      // (row `rows`: no channel was read, scale 0)
+    for (int i = 0; i < QPL; ++i)
+      if (4 * (l + i * L) < Cp) put(t, i, 4 * i * L < C ? q8_code4(v[t][i], d) : 0);
+    if (l == 0) put_scale(t, q8_scale(am));      // (row `rows`: no channel was read, scale 0)
   }
 }
 // 43200 x 512 18.2 us (6.1 TB/s of reads and writes), 393216 x 32 14.9 us (4.3 TB/s; half of it VALU work: 20 instructions
 // for four codes, the maximum and the scale of a row for eight lanes); few rows 2.4 us, a launch's latency.  Up to 16
 // channels four lanes a row: 172800 x 12 5.4 us, 7.1 with eight.
 template <int L, int QPL, int RT, bool VEC>
-__global__ void __launch_bounds__(256) q8_rows_kernel(long rows, int C, int Cp, const float* x, long cs, int co,
-                                                      int8_t* codes, float* scales) {
+__global__ void __launch_bounds__(256) q8_rows_kernel(int rows, int C, int Cp, const float* x, long cs, int8_t* codes,
+                                                      float* scales) {
   constexpr int R = 256 / L;
-  const int g = L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / L) : threadIdx.x / L;
-  for (long r0 = (long)blockIdx.x * (R * RT) + g; r0 <= rows; r0 += (long)gridDim.x * (R * RT))
-    q8_quantize<L, QPL, RT, VEC>(
-        threadIdx.x % L, r0, R, rows, C, Cp, x + co, cs,
-        [&](long row, int c, int q) { *reinterpret_cast<int*>(codes + row * Cp + c) = q; },
-        [&](long row, float sc) { scales[row] = sc; });
+  const int l = threadIdx.x % L, g = L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / L) : threadIdx.x / L;
+  const long xo = g * cs + 4 * l;
+  const int qo = g * Cp + 4 * l;
+  for (int rb = blockIdx.x * (R * RT); rb <= rows; rb += gridDim.x * (R * RT)) {      // (uniform: addresses in scalar registers)
+    const float* const px = x + rb * cs + xo;
+    const auto put = [&](int t, int i, int q) { *reinterpret_cast<int*>(codes + (long)(rb + t * R) * Cp + 4 * i * L + qo) = q; };
+    const auto put_scale = [&](int t, float sc) { (scales + rb + t * R)[g] = sc; };
+    if (rb + R * RT < rows) q8_quantize<L, QPL, RT, VEC, true>(l, rb + g, R, rows, C, Cp, px, R * cs, put, put_scale);
+    else q8_quantize<L, QPL, RT, VEC, false>(l, rb + g, R, rows, C, Cp, px, R * cs, put, put_scale);
+  }
 }
 
 // ---- long rows: 256 lanes each, so that few rows are not one wave's work and many keep few registers (8192 x 2048 14.5 us,
@@ -486,10 +489,12 @@ __global__ void __launch_bounds__(1024) q8_small_kernel(const Q8Conv p, const Q8
   }
   rows = min(rows, in.cap);
   for (int r0 = wk; r0 <= rows; r0 += WK * RT)
-    q8_quantize<64, QPL, RT, true>(
-        lane, r0, WK, rows, in.C, p.Cp, in.x + base * in.cs, in.cs,
-        [&](long row, int c, int q) { *reinterpret_cast<int*>(q8_lds + (int)row * RB + HEAD + c) = q; },
-        [&](long row, float sc) { *reinterpret_cast<float*>(q8_lds + (int)row * RB) = sc; });
+    q8_quantize<64, QPL, RT, true, false>(
+        lane, r0, WK, rows, in.C, p.Cp, in.x + (base + r0) * in.cs + 4 * lane, WK * in.cs,
+        [&](int t, int i, int q) {
+          *reinterpret_cast<int*>(q8_lds + (r0 + t * WK) * RB + HEAD + 4 * (lane + 64 * i)) = q;
+        },
+        [&](int t, float sc) { *reinterpret_cast<float*>(q8_lds + (r0 + t * WK) * RB) = sc; });
   __syncthreads();
 
   const int m = m0 + r16, n = m / hw, rr = m - n * hw, i = rr / cl.GW, j = rr - i * cl.GW;
@@ -954,11 +959,11 @@ int q8_rows(int rows, int C, const float* x, int x_cstride, int x_coff, int8_t* 
     const long nb = tde_cdiv((long)rows + 1, 256 / LL * TT);                                                          \
     const dim3 grid((unsigned)(nb < (1 << 20) ? nb : 1 << 20));                                                       \
     if (vec)                                                                                                          \
-      hipLaunchKernelGGL((q8_rows_kernel<LL, QQ, TT, true>), grid, dim3(256), 0, st, (long)rows, C, Cp, x,            \
-                         (long)x_cstride, x_coff, codes, scales);                                                     \
+      hipLaunchKernelGGL((q8_rows_kernel<LL, QQ, TT, true>), grid, dim3(256), 0, st, rows, C, Cp, x + x_coff,         \
+                         (long)x_cstride, codes, scales);                                                             \
     else                                                                                                              \
-      hipLaunchKernelGGL((q8_rows_kernel<LL, QQ, TT, false>), grid, dim3(256), 0, st, (long)rows, C, Cp, x,           \
-                         (long)x_cstride, x_coff, codes, scales);                                                     \
+      hipLaunchKernelGGL((q8_rows_kernel<LL, QQ, TT, false>), grid, dim3(256), 0, st, rows, C, Cp, x + x_coff,        \
+                         (long)x_cstride, codes, scales);                                                             \
   } while (0)
 #define W(QQ)                                                                                                          \
   do {                                                                                                                 \
