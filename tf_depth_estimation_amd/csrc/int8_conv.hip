@@ -118,9 +118,9 @@ __device__ __forceinline__ void q8_quantize(int l, int row, int R, int rows, int
     if (l == 0) put_scale(t, q8_scale(am));      // (row `rows`: no channel was read, scale 0)
   }
 }
-// 43200 x 512 18.2 us (6.1 TB/s of reads and writes), 393216 x 32 14.9 us (4.3 TB/s; half of it VALU work: 20 instructions
-// for four codes, the maximum and the scale of a row for eight lanes); few rows 2.4 us, a launch's latency.  Up to 16
-// channels four lanes a row: 172800 x 12 5.4 us, 7.1 with eight.
+// 196608 x 128 19.5 us (6.5 TB/s of reads and writes), 43200 x 512 18.2 us (6.1), 393216 x 32 11.9 us (5.4; half of it VALU
+// work: 20 instructions for four codes, and a row's maximum and scale); few rows 2.4 us, a launch's latency.  Two quads a lane
+// share the row's work: 393216 x 32 13.3 us with one, 393216 x 64 19.7 us, 20.9 with one and 22.5 with four.
 template <int L, int QPL, int RT, bool VEC>
 __global__ void __launch_bounds__(256) q8_rows_kernel(int rows, int C, int Cp, const float* x, long cs, int8_t* codes,
                                                       float* scales) {
@@ -977,11 +977,10 @@ int q8_rows(int rows, int C, const float* x, int x_cstride, int x_coff, int8_t* 
                          (long)x_cstride, x_coff, codes, scales);                                                      \
   } while (0)
   const bool many = rows >= 1 << 15;      // one row per lane group in flight where there are few rows
-  if (C <= 16) { if (many) R(4, 2, 4); else R(4, 2, 1); }
-  else if (nq <= 8) { if (many) R(8, 1, 4); else R(8, 1, 1); }
-  else if (nq <= 16) { if (many) R(16, 1, 4); else R(16, 1, 1); }
-  else if (nq <= 32) { if (many) R(32, 1, 4); else R(32, 1, 1); }
-  else if (nq <= 64) { if (many) R(64, 1, 4); else R(64, 1, 1); }
+  if (nq <= 8) { if (many) R(4, 2, 2); else R(4, 2, 1); }
+  else if (nq <= 16) { if (many) R(8, 2, 2); else R(16, 1, 1); }
+  else if (nq <= 32) { if (many) R(16, 2, 2); else R(32, 1, 1); }
+  else if (nq <= 64) { if (many) R(32, 2, 2); else R(64, 1, 1); }
   else if (nq <= 128) R(64, 2, 1);
   else if (nq <= 256) W(1);
   else if (nq <= 512) W(2);
