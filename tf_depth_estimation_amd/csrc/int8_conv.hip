@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(256) q8_rows_kernel(int rows, int C, int Cp, c
   const int l = threadIdx.x % L, g = L == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / L) : threadIdx.x / L;
   const long xo = g * cs + 4 * l;
   const int qo = g * Cp + 4 * l;
-  for (int rb = blockIdx.x * (R * RT); rb <= rows; rb += gridDim.x * (R * RT)) {      // (uniform: addresses in scalar registers)
+  for (int rb = blockIdx.x * (R * RT); rb <= rows; rb += gridDim.x * (R * RT)) {      // (uniform: scalar addresses)
     const float* const px = x + rb * cs + xo;
     const auto put = [&](int t, int i, int q) { *reinterpret_cast<int*>(codes + (long)(rb + t * R) * Cp + 4 * i * L + qo) = q; };
     const auto put_scale = [&](int t, float sc) { (scales + rb + t * R)[g] = sc; };
@@ -533,8 +533,9 @@ __global__ void __launch_bounds__(1024) q8_small_kernel(const Q8Conv p, const Q8
 // fragments of 8 (16) neighbouring pixels lie in different banks.  WK groups of waves split the steps where there are few
 // tiles, and add their sums through LDS in order.  ONE: a tap is one step (the usual case of few channels), no loop.
 // What bounds it there: a tap's conversion is 8 VALU instructions per 16x16 tile, 32 cycles, against 16 (8) cycles of the
-// matrix unit.  (The second launch bound keeps the products out of the accumulator file: with it, 2 moves per result and
-// step cost more than the products.)
+// matrix unit (96x128x32 -> 32, 7x7, batch 32: 68 us = 580 TOP/s, the VALU busy 91 %, the matrix unit 28 %).  (The second
+// launch bound keeps the products out of the accumulator file: with it, 2 moves per result and step cost more than the
+// products.)
 struct Q8Tile {
   int lw, tx, ty, cb;        // log2 of the tile width, tiles per row and column of the class grid, channel bytes per patch fill
   int PH, PW;                // patch rows and columns (of the class with the most taps)
@@ -733,9 +734,9 @@ __global__ void __launch_bounds__(64 * WC * WP * WK, 2) q8_halo_kernel(const Q8C
 // (global_load_lds_dwordx4: a wave instruction copies 16 rows of 64 bytes) into a ring of three slots, two steps in
 // flight across the barriers; the 16-byte quarters of a row are exchanged by (row >> 1) & 3 on the way, so that the
 // fragment reads of 8 neighbouring rows hit different banks.  All sums stay integers until the end.
-// 8192 x 2048 x 2048: 42 us = 1640 TOP/s with 256 x 256 tiles on 8 waves, whose LDS reads (96 bytes a clock) run under the
-// products because the pixel fragments, which every product needs, are read first (55 us the other way round).  The matrix
-// unit is busy 42 % of the time; the rest are the barriers of a step and the 67 MB that all blocks write at their ends.
+// 8192 x 2048 x 2048: 42-43 us = 1600-1640 TOP/s with 256 x 256 tiles on 8 waves, whose LDS reads (96 bytes a clock) run
+// under the products because the pixel fragments, which every product needs, are read first (55 us the other way round).
+// The matrix unit is busy 42 % of the time; the rest are the barriers of a step and the 67 MB that all blocks write at their ends.
 // Smaller tiles read more LDS bytes per product and serve where the large ones would leave CUs idle.
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
 typedef __attribute__((address_space(1))) void* gbl_ptr_t;
