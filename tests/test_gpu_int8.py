@@ -117,6 +117,10 @@ CONVS = [
     (70, 3, 3, 70, 100, 3, 1, False, True),
     (300, 2, 3, 64, 130, 3, 1, False, True),
     (200, 2, 2, 20, 40, 3, 2, True, True),
+    (2, 50, 60, 128, 96, 3, 1, False, True),      # maps of some thousand tiles: channels over two waves, split steps
+    (8, 24, 31, 64, 70, 3, 1, False, True),
+    (8, 24, 32, 20, 72, 5, 1, False, False),
+    (2, 24, 32, 130, 70, 3, 2, True, True),
 ]
 
 

@@ -920,15 +920,16 @@ int q8_conv(Q8Conv p, hipStream_t st) {
     // Blocks of fewer pixels and channels, and more wave groups that split the steps, the fewer tiles there are; timed for
     // each size on the networks' layers at batch 1, 8 and 32 (us, this choice / the next larger block):
     // 28x28x256 -> 128 6.3 / 7.9 (14x14x512 -> 256, 208 tiles: 7.9, 7.2 by the split kernel below), 6x8x1024 -> 512 (8)
-    // 16.1 / 19.3, 24x32x128 -> 128 (8) 9.6 / 10.5, 12x16x512 -> 256 (8) 15.3 / 18.0, 48x64x64 -> 64 k5 (8) 11.6 / 13.4,
+    // 16.1 / 19.3, 24x32x128 -> 128 (8) 9.3 / 10.3, 24x32x256 -> 128 (8) 11.9 / 13.7, 12x16x512 -> 256 (8) 12.7 / 20.8 (each
+    // 10 % and more above that with two waves' channels in one wave), 48x64x64 -> 64 k5 (8) 11.6 / 13.4,
     // 96x128x32 -> 32 k7 (8) 22.0 / 28.2, (32) 64.8 / 72.9 with this choice's smaller neighbour, 24x32x256 -> 128 (32)
     // 23.7 / 28.1
     if (tiles < 512) done = q8_halo_launch<1, 2, 1, 1, 8>(p, GH, GW, classes, st);
     else if (tiles < 1536) done = q8_halo_launch<2, 2, 1, 1, 8>(p, GH, GW, classes, st);
     else if (p.K <= 16) done = tiles < 8192 ? q8_halo_launch<1, 4, 1, 2, 2>(p, GH, GW, classes, st)
                                             : q8_halo_launch<1, 4, 1, 4, 1>(p, GH, GW, classes, st);
-    else if (tiles < 4096) done = p.K > 64 && p.Cp > 128 ? q8_halo_launch<2, 4, 1, 1, 4>(p, GH, GW, classes, st)
-                                                         : q8_halo_launch<2, 2, 1, 1, 4>(p, GH, GW, classes, st);
+    else if (tiles < 4096) done = p.K > 64 ? q8_halo_launch<1, 4, 2, 1, 4>(p, GH, GW, classes, st)
+                                           : q8_halo_launch<2, 2, 1, 1, 4>(p, GH, GW, classes, st);
     else if (p.K > 64) done = q8_halo_launch<2, 4, 2, 1, 2>(p, GH, GW, classes, st);
     else if (tiles < 8192) done = q8_halo_launch<2, 2, 1, 2, 2>(p, GH, GW, classes, st);
     else if (p.K > 32) done = q8_halo_launch<2, 4, 2, 2, 1>(p, GH, GW, classes, st);
