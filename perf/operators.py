@@ -165,11 +165,11 @@ def _blocks(u):
 def _code(u):
     """8-bit codes [M, C] and scales [M, blocks] of pre-activations (float64)."""
     M, C = u.shape
-    s = _blocks(u).abs().amax(dim=2).float() / 128            # the stored scale: the codes are relative to it
-    sc = s.double().repeat_interleave(BLOCK, dim=1)[:, :C]
-    t = (u.abs() / torch.where(sc > 0, sc, torch.ones_like(sc))).floor_().clamp_(max=127)
+    a = _blocks(u).abs().amax(dim=2)
+    ac = a.repeat_interleave(BLOCK, dim=1)[:, :C]
+    t = (u.abs() * 128 / torch.where(ac > 0, ac, torch.ones_like(ac))).floor_().clamp_(max=127)
     q = torch.where(u > 0, t, -1 - t)
-    return q.to(torch.int8), s
+    return q.to(torch.int8), a.float() / 128
 
 
 def _value(codes, scales):
@@ -311,7 +311,7 @@ def exact(case, seed):
         tape = torch.empty_like(u)
         for c0 in range(0, C, BLOCK):
             ub = u[:, c0:c0 + BLOCK]
-            step = (ub.abs().max(dim=1, keepdim=True).values.float() / 128).double()      # as it is stored
+            step = ub.abs().max(dim=1, keepdim=True).values / 128
             m = torch.trunc(ub / torch.where(step > 0, step, torch.ones_like(step))).clamp(-127, 127)
             tape[:, c0:c0 + BLOCK] = torch.where(ub > 0, m + 0.5, m - 0.5) * step
         return dict(y=torch.relu(u), mean=torch.stack(means), invstd=torch.stack(invs), tape=tape)
