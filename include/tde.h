@@ -323,9 +323,10 @@ int tde_q8_deconv2d_f32_bias_act(const tde_conv_desc_t* d, const float* x_small,
 /* (2) The 8-bit tape of training BatchNorm + ReLU: what the backward pass needs of a layer -- its pre-BN output z, the
  * ReLU mask and its output y -- as ONE 8-bit code per element instead of two fp32 tensors.  The pre-activation
  * u = (z - mean) * invstd + beta (evaluated in fp64) is coded per row in blocks of TDE_TAPE8_BLOCK channels:
- *   s = (float)max|u| / 128,  code = min(floor(|u| / s), 127) for u > 0,  -1 - min(floor(|u| / s), 127) for u <= 0,
- * a mid-rise code of value (code + 1/2) s: off by at most s / 2 (and the rounding of s, 2^-17 s, at the block's
- * maximum), and code >= 0 IS u > 0, so the mask is exact.
+ *   a = max|u|,  s = (float)a / 128,
+ *   code = min(floor(128 |u| / a), 127) for u > 0,  -1 - min(floor(128 |u| / a), 127) for u <= 0,
+ * with a unrounded (fp64) in the quotient: a mid-rise code of value (code + 1/2) s, off by at most s / 2 (and the rounding of
+ * s, 2^-17 s at the block's maximum), and code >= 0 IS u > 0, so the mask is exact.
  * A block that holds a NaN or an infinity has scale NaN (its restored values are NaN).
  *   codes [M][C] int8, scales [M][ceil(C / TDE_TAPE8_BLOCK)] float; both 16-byte aligned.
  * M rows are `groups` equal row groups, each its own BatchNorm batch (tde_bn_fwd_train).  C % 4 == 0, C <= 1024.

@@ -20,7 +20,12 @@ def pytest_collection_modifyitems(session, config, items):
     state (GPUTEST_r05 aborted inside one of them, which also hid every test collected after it)."""
     rest = [it for it in items if it.get_closest_marker("rccl") is None]
     last = [it for it in items if it.get_closest_marker("rccl") is not None]
-    items[:] = rest + last
+    # Two cases expect the 8-bit tape's codes of a division by the rounded scale, where 1 and 3 of their codes are not those
+    # of the definition (tests/test_gpu_tape8_codes.py, which has the same inputs): they fail, and run after everything else,
+    # so that with -x they hide nothing.
+    rounded = ("test_gpu_int8.py::test_tape_forward[8200-4-1-12-8]", "test_gpu_int8.py::test_tape_forward[40000-68-8-68-0]")
+    fail = [it for it in rest if it.nodeid.endswith(rounded)]
+    items[:] = [it for it in rest if it not in fail] + last + fail
 
 
 def gpu_available():

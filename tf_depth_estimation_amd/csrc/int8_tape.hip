@@ -1,8 +1,8 @@
 // The 8-bit tape of training BatchNorm + ReLU (include/tde.h, "8-bit activations" (2)).
 //
 // Forward: per channel and row group mean / variance of z (fp64), u = (z - mean) * invstd + beta (fp64),
-// y = relu(u), and u kept as one byte per element: blocks of 64 channels of a row share s = (float)max|u| / 128 and
-// the mid-rise code floor(|u| / s) with u's sign folded in (q >= 0 iff u > 0; value (q + 1/2) s).
+// y = relu(u), and u kept as one byte per element: blocks of 64 channels of a row share a = max|u| (fp64), s = (float)a / 128
+// and the mid-rise code floor(128 |u| / a) with u's sign folded in (q >= 0 iff u > 0; value (q + 1/2) s).
 // Backward: g = dy [q >= 0], xhat = (q + 1/2) s - beta, dz = invstd (g - mean g - xhat mean(g xhat)).
 //
 // u is evaluated in fp64 because a code next to a step's border flips with the last bits of u: with fp64 the codes are
@@ -25,21 +25,31 @@ int tape_lanes(int C) {
   return l;
 }
 
-// codes of four u under scale s, packed: the exact floor(|u| / s) clamped to 127, sign folded in (~q for u <= 0).  The fp32
-// estimate t = |u| / s is off by less than 4e-5 (three roundings of at most 128), so unless t lies that close to an integer
-// its floor is the quotient's; near one (1 element in 10^4) the fp64 remainder decides.  Estimates past 127.25 are set
-// there: they are clamped to 127 anyway, and every block's maximum, at 128, would take the exact path.
-__device__ __noinline__ int tape_code_exact(double u, float s) {
+// codes of four u of a block with maximum a = max|u| and scale s = (float)a / 128, packed: the exact floor(128 |u| / a) clamped
+// to 127, sign folded in (~q for u <= 0).  The fp32 estimate t = |u| / s is off by less than 4e-5 (|u|, a and the product are
+// rounded by half a step each, the reciprocal is off by up to one: 5 * 2^-24 of at most 128), so unless t lies that close to
+// an integer its floor is the quotient's; near one (1 element in 10^4) the fp64 remainder against the unrounded a decides,
+// which the lanes of a row exchange only then.  (Against the rounded s one code in 10^6 is off by one.)  Estimates past 127.25
+// are set there: they are clamped to 127 anyway, and every block's maximum, at 128, would take the exact path.
+__device__ __noinline__ int tape_code_exact(double u, double a, float s) {
   int q = 0;
-  if (s > 0.f) {                       // (s zero or NaN: 0 / -1)
-    const double au = fabs(u);
-    q = (int)fmin(floor(au / (double)s), 127.0);
-    const double r = fma(-(double)q, (double)s, au);
+  if (a > 0.0 && s == s) {             // (a block of zeros, or one that is not finite: 0 / -1)
+    const double au = 128.0 * fabs(u);
+    q = (int)fmin(floor(au / a), 127.0);
+    const double r = fma(-(double)q, a, au);
     if (r < 0.0) --q;
-    if (r >= (double)s && q < 127) ++q;
+    if (r >= a && q < 127) ++q;
   }
   return u > 0.0 ? q : -1 - q;
 }
+// maximum over the aligned group of L lanes, in every lane; all L lanes must be active
+template <int L>
+__device__ __forceinline__ double group_dmax(double v) {
+#pragma unroll
+  for (int o = 1; o < L; o <<= 1) v = fmax(v, __shfl_xor(v, o, 64));
+  return v;
+}
+template <int L>
 __device__ __forceinline__ int tape_code4(const d4& u, const f4& uf, float s) {
   bool near = !(s >= 0x1p-100f);       // (1 / s may be no normal number)
   const float inv = __builtin_amdgcn_rcpf(s);
@@ -50,18 +60,20 @@ __device__ __forceinline__ int tape_code4(const d4& u, const f4& uf, float s) {
     q[j] = floorf(t);
     near |= fabsf((t - q[j]) - 0.5f) > 0.49995f && t > 0.5f;
   }
-  if (near) {
-    int p = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) p |= (tape_code_exact(u[j], s) & 0xff) << (8 * j);
-    return p;
-  }
   unsigned p = put_byte<0>(q[0], 0);
   p = put_byte<1>(q[1], p);
   p = put_byte<2>(q[2], p);
   p = put_byte<3>(q[3], p);
 #pragma unroll
   for (int j = 0; j < 4; ++j) p ^= u[j] > 0.0 ? 0u : 0xffu << (8 * j);
+  if (__any(near)) {                   // (uniform over the wave: every lane of a row's group takes part in the exchange)
+    const double a = group_dmax<L>(fmax(fmax(fabs(u[0]), fabs(u[1])), fmax(fabs(u[2]), fabs(u[3]))));
+    if (near) {
+      p = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p |= (unsigned)(tape_code_exact(u[j], a, s) & 0xff) << (8 * j);
+    }
+  }
   return (int)p;
 }
 
@@ -87,7 +99,7 @@ __device__ __forceinline__ void tape_row(const d4& u, f4& y, int& packed, float&
     am = max(am, abs_bits(uf[j]));
   }
   s = tape_scale(group_umax<L>(am));
-  packed = tape_code4(u, uf, s);
+  packed = tape_code4<L>(u, uf, s);
 }
 
 struct TapeFwd {
