@@ -1,0 +1,62 @@
+"""What runs of one program with the 8-bit tape hand out does not lie in the buffers they share."""
+import types
+
+import pytest
+import torch
+
+from tf_depth_estimation_amd import _api, _netlib, int8, variables
+from tf_depth_estimation_amd.program import NetProgram, NetRun
+
+
+@pytest.mark.parametrize("cin", [3, 4, 8])
+def test_input_gradients_are_their_own(cin):
+    prog = NetProgram(_netlib.disp_net_spec(64, 96, cin), types.SimpleNamespace(prefix="m"))
+    runs = [NetRun(prog, 2, device="cpu", tape8=True) for _ in range(2)]
+    got = []
+    for i, r in enumerate(runs):
+        r.ensure_grad()
+        r.view_tensor(prog.spec.input_view, True).fill_(i + 1)       # what a backward leaves
+        got.append(r.input_grad())
+    for i, g in enumerate(got):
+        assert tuple(g.shape) == (2, 64, 96, cin) and g.is_contiguous() and bool((g == i + 1).all())
+
+
+@pytest.fixture()
+def fresh_store():
+    variables.get_store().reset(seed=1)
+    _api.clear_programs()
+    yield
+    variables.get_store().reset(seed=1)
+    _api.clear_programs()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cin", [3, 4])
+def test_input_gradients_through_autograd(cin, fresh_store):
+    """Two calls of one network under int8.tape8(): each input's gradient is that of the call alone, one input of both calls
+    gets their sum, and a gradient autograd took over keeps its values."""
+    from tf_depth_estimation_amd import nets_optflow_depth as nd
+
+    def image(seed):
+        return torch.randn(2, 64, 96, cin, generator=torch.Generator().manual_seed(seed)).mul_(0.3).cuda()
+
+    def loss(x):
+        with variables.variable_scope("model"), int8.tape8():
+            return sum((o * o).mean() for o in nd.disp_net(x, True)[0])
+
+    alone = []
+    for s in (1, 2):
+        x = image(s).requires_grad_()
+        loss(x).backward()
+        alone.append(x.grad.clone())
+    assert all(bool(torch.isfinite(g).all()) and float(g.abs().max()) > 0 for g in alone)
+    xs = [image(s).requires_grad_() for s in (1, 2)]
+    (loss(xs[0]) + loss(xs[1])).backward()
+    for x, g in zip(xs, alone):
+        assert torch.equal(x.grad, g)
+    x = image(1).requires_grad_()
+    (loss(x) + loss(x)).backward()
+    assert torch.equal(x.grad, alone[0] + alone[0])
+    kept = xs[0].grad
+    loss(image(3).requires_grad_()).backward()
+    assert torch.equal(kept, alone[0])

@@ -378,6 +378,12 @@ class NetRun:
         iv = self.prog.spec.input_view
         return self.act[iv.buf.name][..., iv.coff:iv.coff + self.prog.spec.cin]
 
+    def input_grad(self):
+        """d(input) [N,H,W,cin] of the last backward: a view of this run's buffer, which its next backward overwrites; with
+        the 8-bit tape, whose gradient buffers all runs of the program share, a tensor of its own."""
+        dx = self.view_tensor(self.prog.spec.input_view, True)[..., :self.prog.spec.cin]
+        return dx.clone(memory_format=torch.contiguous_format) if self.tape8 else dx
+
     def grad_tensor(self, v):
         """Gradient view of output view v (a loss kernel may write it; then pass IN_PLACE to backward)."""
         self.ensure_grad()
@@ -836,7 +842,7 @@ class NetProgram:
         """grad_outputs: list (aligned with spec.outputs) of tensors or None.  Accumulates parameter
         gradients into chunk.grad, or with grad_accumulate=False OVERWRITES them (every parameter is
         written by one backward call, so a trainer's first call of the step needs no zeroed buffer
-        and the kernels skip the read-modify-write).  Returns d(input) if requested.  on_grads(names),
+        and the kernels skip the read-modify-write).  Returns d(input) if requested (NetRun.input_grad).  on_grads(names),
         if given, is called after each op with the full variable names whose gradient that op just
         wrote (the data-parallel exchange launches a bucket once all its parameters are final, ddp.py)."""
         main = torch.cuda.current_stream()
@@ -882,7 +888,6 @@ class NetProgram:
                                          acc, st), "grad_out")
         ws, dz = self._scratch(N)
         wsb = ws.numel() * 4
-        iv = spec.input_view
         if run.tape8:
             self._restore_tape8(run)
         _lib.check(lib.tde_zero_bytes(run.absmax.numel() * 4, ptr(run.absmax), st), "zero dz bounds")
@@ -1084,9 +1089,7 @@ class NetProgram:
             if on_grads is not None and names:
                 on_grads(names)
             self.join_wgrad()
-        if need_input_grad:
-            return run.view_tensor(iv, grad=True)[..., :spec.cin]
-        return None
+        return run.input_grad() if need_input_grad else None
 
 
 def ctypes_ref(d):
