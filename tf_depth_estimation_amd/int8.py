@@ -16,6 +16,7 @@ none of them records an autograd graph (an input that requires a gradient is ref
 The formulas stand in include/tde.h, "8-bit activations".
 """
 import contextlib
+import contextvars
 import ctypes
 import functools
 
@@ -408,19 +409,23 @@ def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
 
 
 # ---------------------------------------------------------------- whole networks
-_TAPE8 = [False]
+# the open tape8() blocks of this thread (of this task), innermost last: (block, on)
+_TAPE8 = contextvars.ContextVar("tape8", default=())
 
 
 @contextlib.contextmanager
 def tape8(on=True):
     """`with int8.tape8(): outs = disp_net(images)`: the reference-named network functions called inside keep their
-    training tape in 8 bits (program.NetRun(tape8=True)); the backward may run outside."""
-    was, _TAPE8[0] = _TAPE8[0], bool(on)
+    training tape in 8 bits (program.NetRun(tape8=True)); the backward may run outside.  It holds for the calls of the
+    thread (asyncio: the task) that entered it; each block ends with itself, whatever order blocks are left in."""
+    block = object()
+    _TAPE8.set(_TAPE8.get() + ((block, bool(on)),))
     try:
         yield
     finally:
-        _TAPE8[0] = was
+        _TAPE8.set(tuple(b for b in _TAPE8.get() if b[0] is not block))
 
 
 def tape8_active():
-    return _TAPE8[0]
+    blocks = _TAPE8.get()
+    return bool(blocks) and blocks[-1][1]
