@@ -28,6 +28,10 @@ from .program import same_pad
 
 BLOCK = 64            # TDE_TAPE8_BLOCK: channels of a row that share a tape scale
 MAX_CHANNELS = 4096   # of a Conv8 input
+# what the C entries take: they count rows and strides in 32 bits, where larger numbers would wrap on the way there
+MAX_ROWS = 1 << 30
+MAX_PIXELS = 1 << 26  # of a Conv8 input or output
+MAX_STRIDE = (1 << 31) - 1
 
 
 def _check(t, name, dtype=torch.float32):
@@ -46,7 +50,10 @@ def _rows(t, name):
         raise ValueError(f"{name} must have at least two dimensions, got {tuple(shape)}")
     C = shape[-1]
     if C and t.is_contiguous():
-        return t.numel() // C, C, C
+        rows = t.numel() // C
+        if rows > MAX_ROWS or C > MAX_STRIDE:
+            raise ValueError(f"{name}: {rows} rows of {C}: at most 2^30 rows of 2^31 - 1")
+        return rows, C, C
     rows, cs = 1, None
     for n, s in zip(reversed(shape[:-1]), reversed(t.stride()[:-1])):
         if n != 1:
@@ -58,6 +65,8 @@ def _rows(t, name):
     cs = C if cs is None else cs
     if rows and (C == 0 or (C > 1 and t.stride(-1) != 1) or cs < C):
         raise ValueError(f"{name} must be a pixel-major channel view of at least one channel (strides {t.stride()})")
+    if rows > MAX_ROWS or cs > MAX_STRIDE:
+        raise ValueError(f"{name}: {rows} rows {cs} apart: at most 2^30 rows and a pixel stride of 2^31 - 1")
     return rows, C, cs
 
 
@@ -82,10 +91,9 @@ def _out(out, shape, device, name="out"):
 # ---------------------------------------------------------------- integer product
 @functools.lru_cache(maxsize=None)
 def row_bytes(C):
-    n = _lib.load().tde_q8_row_bytes(C)
-    if n <= 0:
+    if not 1 <= C <= MAX_CHANNELS:
         raise ValueError(f"{C} channels: 1 to {MAX_CHANNELS} are supported")
-    return n
+    return _lib.load().tde_q8_row_bytes(C)
 
 
 class Rows8:
@@ -180,11 +188,16 @@ class Conv8:
         if shape[-1] != self.cin:
             raise ValueError(f"x has {shape[-1]} channels, the weights {self.cin}")
         if len(shape) == 2 and (self.kh, self.kw, self.stride) == (1, 1, 1):
-            return 1, 1, shape[0], torch.Size((shape[0], self.K))
-        if len(shape) != 4:
+            N, H, W, oshape = 1, 1, shape[0], (shape[0], self.K)
+        elif len(shape) != 4:
             raise ValueError(f"x must be [N, H, W, C], or [M, C] for a 1x1 stride-1 conv, got {tuple(shape)}")
-        N, H, W = shape[:3]
-        return N, H, W, torch.Size((N,) + self.out_size(H, W) + (self.K,))
+        else:
+            N, H, W = shape[:3]
+            oshape = (N,) + self.out_size(H, W) + (self.K,)
+        OH, OW = self.out_size(H, W)
+        if max(N * H * W, N * OH * OW) > MAX_PIXELS:
+            raise ValueError(f"x {tuple(shape)}: at most 2^26 input and output pixels")
+        return N, H, W, torch.Size(oshape)
 
     def _make_desc(self, N, H, W, ics, ocs):
         """The conv descriptor of a batch whose input and output have pixel strides ics and ocs (a transposed conv's is
@@ -252,7 +265,7 @@ class Tape8:
             raise ValueError("codes, scales and invstd must be contiguous")
         if any(t.data_ptr() % 16 for t in (codes, scales, invstd)):
             raise ValueError("codes, scales and invstd must start on 16 bytes")
-        self.shape, self.C, self.rows, self.groups = codes.shape, C, codes.numel() // C, invstd.shape[0]
+        self.shape, self.C, self.rows, self.groups = codes.shape, C, _rows(codes, "codes")[0], invstd.shape[0]
         _check_groups(self.rows, self.groups)
         self._buffer, self._views = codes, (codes, scales, invstd, mean)
         self._ptrs = (codes.data_ptr(), scales.data_ptr(), invstd.data_ptr())
@@ -355,7 +368,7 @@ def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel
     _check_beta(C, beta)
     if not z.is_contiguous() or z.data_ptr() % 16:
         raise ValueError("z must be a contiguous [..., C] tensor that starts on 16 bytes")
-    rows = z.numel() // C
+    rows = _rows(z, "z")[0]
     if rows == 0:
         raise ValueError("BatchNorm over no rows has no statistics")
     _check_groups(rows, groups)
