@@ -272,8 +272,10 @@ __global__ void __launch_bounds__(256) tape_fwd_apply_kernel(const TapeFwd p, co
   const bool on = c < p.C;
   const long base = (long)g * p.Mg;
   const int r0 = blockIdx.x * rpb, r1 = min(p.Mg, r0 + rpb);
-  // row of step i: uniform row rb + i R (addresses in scalar registers) + this lane's rl (32-bit offsets)
-  const unsigned zo = rl * p.C + c, yo = rl * p.ycs + c, so = rl * p.NB + b;
+  // row of step i: uniform row rb + i R (addresses in scalar registers) + this lane's rl (32-bit offsets, but in y, whose
+  // pixel stride may be any int)
+  const unsigned zo = rl * p.C + c, so = rl * p.NB + b;
+  const long yo = (long)rl * p.ycs + c;
   f4 v[APPLY_RB];
   auto load = [&](int rb) __attribute__((always_inline)) {
 #pragma unroll
@@ -488,7 +490,8 @@ __global__ void __launch_bounds__(256) tape_bwd_apply_kernel(const TapeBwd p, co
     const long base = (long)g * p.Mg;
     const int r0 = blockIdx.x * rpb, r1 = min(p.Mg, r0 + rpb);
     // (row addresses as in the forward)
-    const unsigned zo = rl * p.C + c, yo = rl * p.dycs + c, so = rl * p.NB + b;
+    const unsigned zo = rl * p.C + c, so = rl * p.NB + b;
+    const long yo = (long)rl * p.dycs + c;
     f4 v[APPLY_RB];
     int cd[APPLY_RB];
     float s[APPLY_RB];
