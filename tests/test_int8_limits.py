@@ -5,7 +5,8 @@ import types
 import pytest
 import torch
 
-from tf_depth_estimation_amd import int8
+from tests.test_int8_refusals import desc, p  # noqa: F401 (p: a fixture)
+from tf_depth_estimation_amd import _lib, int8
 
 
 def meta(shape, strides=None, dtype=torch.float32):
@@ -75,3 +76,24 @@ def test_the_calls_refuse(monkeypatch):
 def test_channels_past_the_limit(C):
     with pytest.raises(ValueError, match="channels"):
         int8.row_bytes(C)
+
+
+def test_the_c_entries_refuse_what_wraps(p):  # noqa: F811
+    """Sums of a channel offset near 2^31 and products of three sizes near 2^64 are taken without wrapping."""
+    lib = _lib.load()
+    for co in (2 ** 31 - 4, 2 ** 31 - 1):
+        assert lib.tde_q8_rows(2, 4, p, 8, co, p, p, None) == -1
+        assert lib.tde_q8_conv2d_bias_act(desc(y_coff=co), p, p, p, p, None, 1, p, None) == -1
+        assert lib.tde_q8_deconv2d_bias_act(desc(x_coff=co), p, p, p, p, None, 1, p, None) == -1
+        assert lib.tde_q8_conv2d_f32_bias_act(desc(x_coff=co), p, p, p, p, p, None, 1, p, None) == -1
+        assert lib.tde_q8_deconv2d_f32_bias_act(desc(y_coff=co), p, p, p, p, p, None, 1, p, None) == -1
+    co = 2 ** 31 - 4
+    assert lib.tde_tape8_restore(8, 4, p, p, 1, p, 8, co, None) == -1
+    assert lib.tde_tape8_bn_fwd(8, 4, 1, p, p, 1e-3, 0.99, 1, None, None, p, p, p, 8, co, p, p, p, 1 << 20, None) == -1
+    assert lib.tde_tape8_bn_bwd(8, 4, 1, p, p, p, p, p, 8, co, p, None, 0, None, p, 1 << 20, None) == -1
+    for big in (dict(N=1 << 22, H=1 << 21, W=1 << 21), dict(N=1 << 22, OH=1 << 21, OW=1 << 21),
+                dict(N=1 << 30, H=1 << 30, W=16)):
+        d = desc(**big)
+        assert lib.tde_q8_conv2d_bias_act(d, p, p, p, p, None, 1, p, None) == -1, big
+        assert lib.tde_q8_deconv2d_bias_act(d, p, p, p, p, None, 1, p, None) == -1, big
+        assert lib.tde_q8_one_launch(d, 0) == 0 and lib.tde_q8_one_launch(d, 1) == 0, big

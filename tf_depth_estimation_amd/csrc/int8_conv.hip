@@ -947,11 +947,11 @@ int q8_conv(Q8Conv p, hipStream_t st) {
 
 bool q8_rows_ok(int rows, int C, const float* x, int x_cstride, int x_coff, const int8_t* codes, const float* scales) {
   return rows > 0 && rows <= (1 << 30) && C > 0 && C <= Q8_MAXC && x && codes && scales && tde_aligned16(codes) &&
-         x_coff >= 0 && x_coff + C <= x_cstride;
+         x_coff >= 0 && (long)x_coff + C <= x_cstride;
 }
 // 16-byte loads of a channel view (a row's padding up to a multiple of four channels is read)
 bool q8_rows_vec(int C, const float* x, int x_cstride, int x_coff) {
-  return tde_aligned16(x) && x_cstride % 4 == 0 && x_coff % 4 == 0 && x_coff + (C + 3) / 4 * 4 <= x_cstride;
+  return tde_aligned16(x) && x_cstride % 4 == 0 && x_coff % 4 == 0 && (long)x_coff + (C + 3) / 4 * 4 <= x_cstride;
 }
 int q8_rows(int rows, int C, const float* x, int x_cstride, int x_coff, int8_t* codes, float* scales, hipStream_t st) {
   const int Cp = q8_row(C), nq = Cp / 4;
@@ -1031,12 +1031,13 @@ bool q8_geometry_ok(const tde_conv_desc_t* d, int cin, int cout) {
       d->pad_top < 0 || d->pad_left < 0 || d->pad_top >= d->KH || d->pad_left >= d->KW)
     return false;
   if (cin <= 0 || cin > Q8_MAXC || cout <= 0 || cout > 65535 || d->KH > 64 || d->KW > 64 || d->stride > 64) return false;
-  return (long)d->N * d->H * d->W <= Q8_MAXPIX && (long)d->N * d->OH * d->OW <= Q8_MAXPIX;
+  const auto fits = [&](int h, int w) { return (long)h * w <= Q8_MAXPIX && (long)d->N * ((long)h * w) <= Q8_MAXPIX; };
+  return fits(d->H, d->W) && fits(d->OH, d->OW);      // (the product of three ints may not fit 64 bits)
 }
 bool q8_args_ok(const tde_conv_desc_t* d, const int8_t* xc, const float* xs, const int8_t* wc, const float* ws, int relu,
                 const float* y, int cin, int cout, int ocs, int oco) {
   if (!wc || !ws || !y || !q8_geometry_ok(d, cin, cout)) return false;
-  if (ocs <= 0 || oco < 0 || oco + cout > ocs) return false;
+  if (ocs <= 0 || oco < 0 || (long)oco + cout > ocs) return false;
   return (relu == 0 || relu == 1) && tde_aligned16(xc) && tde_aligned16(wc) && tde_aligned16(ws) &&
          (reinterpret_cast<uintptr_t>(xs) & 3u) == 0 && (reinterpret_cast<uintptr_t>(y) & 3u) == 0;
 }
@@ -1069,7 +1070,7 @@ Q8Conv q8_deconv_args(const tde_conv_desc_t* d, const int8_t* x_codes, const flo
 // from the fp32 input (its channel view): in one launch, or quantised into codes and scales first (always where the output
 // may lie on the input, which a block of one launch could still have to read)
 int q8_conv_f32(const Q8Conv& p, const float* x, int C, int cs, int co, int8_t* codes, float* scales, hipStream_t st) {
-  TDE_CHECK_ARG(x && co >= 0 && co + C <= cs);
+  TDE_CHECK_ARG(x && co >= 0 && (long)co + C <= cs);
   const int cap = q8_rows_vec(C, x, cs, co) ? q8_small_rows(p) : 0;
   const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), x1 = x0 + (size_t)p.N * p.H * p.W * cs * sizeof(float);
   const uintptr_t y0 = reinterpret_cast<uintptr_t>(p.y), y1 = y0 + (size_t)p.N * p.OH * p.OW * p.ycs * sizeof(float);

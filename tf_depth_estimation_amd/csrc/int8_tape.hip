@@ -684,7 +684,7 @@ bool tape_shape_ok(int M, int C, int groups) {
   return M > 0 && M <= (1 << 30) && C > 0 && C % 4 == 0 && C <= 1024 && groups >= 1 && groups <= BN_MAX_GROUPS && M % groups == 0;
 }
 bool tape_view_ok(const float* v, int C, int cs, int co) {
-  return v && tde_aligned16(v) && cs % 4 == 0 && co % 4 == 0 && co >= 0 && co + C <= cs;
+  return v && tde_aligned16(v) && cs % 4 == 0 && co % 4 == 0 && co >= 0 && (long)co + C <= cs;
 }
 bool tape_ok(const int8_t* codes, const float* scales) {
   return codes && scales && tde_aligned16(codes) && tde_aligned16(scales);
