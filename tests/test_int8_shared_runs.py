@@ -1,5 +1,6 @@
 """What runs of one program with the 8-bit tape hand out does not lie in the buffers they share."""
 import types
+import weakref
 
 import pytest
 import torch
@@ -19,6 +20,28 @@ def test_input_gradients_are_their_own(cin):
         got.append(r.input_grad())
     for i, g in enumerate(got):
         assert tuple(g.shape) == (2, 64, 96, cin) and g.is_contiguous() and bool((g == i + 1).all())
+
+
+def test_a_switched_run_gives_its_buffers_back_first(monkeypatch):
+    """enable_tape8 makes the shared set when the run holds no more of its fp32 buffers than those that stay."""
+    prog = NetProgram(_netlib.disp_net_spec(64, 96, 3), types.SimpleNamespace(prefix="m"))
+    run = NetRun(prog, 2, device="cpu")
+    run.ensure_grad()
+    stays = prog.own_buffers()
+    outs = {v.buf.name for v in prog.spec.outputs}
+    gone = [weakref.ref(t) for n, t in run.act.items() if n not in stays] + [weakref.ref(t) for t in run.z.values()]
+    gone += [weakref.ref(t) for n, t in run.grad.items() if n not in outs]
+    before = sum(r() is not None for r in gone)
+    seen = []
+    make = NetProgram.shared_tape8
+
+    def shared(self, *a):
+        seen.append(sum(r() is not None for r in gone))
+        return make(self, *a)
+
+    monkeypatch.setattr(NetProgram, "shared_tape8", shared)
+    run.enable_tape8()
+    assert before == len(gone) > 20 and seen[0] == 0
 
 
 @pytest.fixture()

@@ -284,9 +284,13 @@ class NetRun:
             if isinstance(op, ConvBN) and (not op.bn or op.K % 4 or op.K > 1024):
                 raise ValueError(f"8-bit tape: layer {op.layer} needs BatchNorm over a multiple of 4 channels, at most "
                                  "1024 (BN-free networks keep the fp32 tape)")
+        own, out = self.prog.own_buffers(), {v.buf.name for v in spec.outputs}
+        # of an fp32 run's buffers only those that stay are held while the new ones are made
+        kept = {n: t for n, t in (getattr(self, "act", None) or {}).items() if n in own}
+        grad = getattr(self, "grad", None)
+        kept_grad = None if grad is None else {n: t for n, t in grad.items() if n in out}
+        self.act = self.z = self.grad = grad = None
         shared = self.prog.shared_tape8(N, self.device)
-        own = self.prog.own_buffers()
-        kept = getattr(self, "act", None) or {}
         self.act = {}
         for b in spec.bufs:
             if b.name not in own:
@@ -306,15 +310,14 @@ class NetRun:
                                 torch.empty(shape[:3] + ((op.K + 63) // 64,), device=self.device, dtype=torch.float32))
         if not hasattr(self, "absmax"):
             self._alloc_absmax()
-        grad = getattr(self, "grad", None)
-        self.grad = None
-        if grad is not None:
-            self.ensure_tape8_grad(grad)
+        if kept_grad is not None:
+            self.ensure_tape8_grad(kept_grad)
         self.tape8, self.tape_ready = True, False
 
     def enable_tape8(self):
         """Keep this run's training tape in 8 bits from the next forward on; its input, output and output gradient
-        buffers stay where they are."""
+        buffers stay where they are, the others are given back before the 8-bit ones are made (a run that finds no memory
+        for those cannot be used any more)."""
         if not self.tape8:
             self._alloc_tape8()
         return self
