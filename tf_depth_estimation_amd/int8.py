@@ -12,7 +12,8 @@ opt-in here.
     it for whole networks.
 
 Like the rest of the package these are calls on the current stream of the current device without a CPU fallback;
-none of them records an autograd graph (an input that requires a gradient is refused while gradients are enabled).
+none of them records an autograd graph (an input that requires a gradient is refused while gradients are enabled, one with a
+forward-mode tangent always).
 The formulas stand in include/tde.h, "8-bit activations".
 """
 import contextlib
@@ -21,6 +22,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import ConvDesc
@@ -41,6 +43,8 @@ def _check(t, name, dtype=torch.float32):
         raise ValueError(f"{name} is on {t.device}, not on the current device (cuda:{_lib.current_device()})")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: 8-bit operators record none (detach it, or use torch.no_grad())")
+    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a forward-mode tangent: 8-bit operators carry none")
 
 
 def _rows(t, name):
