@@ -149,7 +149,9 @@ class Conv8:
 
     weights: conv [KH, KW, Cin, Cout], or with deconv=True conv2d_transpose [KH, KW, Cout, Cin] (the TF checkpoint
     layouts), fp32.  They are quantised once (per output channel) by __init__ / load; later changes of the tensor are not
-    seen, as with NetProgram.fold_bn."""
+    seen, as with NetProgram.fold_bn.  load of weights of the same shape writes the buffers in place, so a captured graph of
+    calls goes on with the new ones; after a load of another shape (or of a bias where there was none) it must be captured
+    again."""
 
     def __init__(self, weights, bias=None, stride=1, relu=True, deconv=False):
         if not isinstance(stride, int) or not 1 <= stride <= 64:
@@ -172,12 +174,20 @@ class Conv8:
                 raise ValueError(f"bias must be ({K},), got {tuple(bias.shape)}")
         lib = _lib.load()
         w = weights.contiguous()
-        self.kh, self.kw, self.cin, self.K = kh, kw, cin, K
-        self.codes = torch.empty(lib.tde_q8_weights_size(kh * kw, cin, K), dtype=torch.int8, device=w.device)
-        self.scales = torch.empty((K + 15) // 16 * 16, dtype=torch.float32, device=w.device)
-        self.bias = None if bias is None else bias.detach().clone().contiguous()
-        self._geometry = functools.lru_cache(maxsize=64)(self._make_geometry)
-        self._desc = functools.lru_cache(maxsize=64)(self._make_desc)
+        if (kh, kw, cin, K, w.device) != getattr(self, "_loaded", None):
+            self.kh, self.kw, self.cin, self.K = kh, kw, cin, K
+            self.codes = torch.empty(lib.tde_q8_weights_size(kh * kw, cin, K), dtype=torch.int8, device=w.device)
+            self.scales = torch.empty((K + 15) // 16 * 16, dtype=torch.float32, device=w.device)
+            self.bias = None
+            self._geometry = functools.lru_cache(maxsize=64)(self._make_geometry)
+            self._desc = functools.lru_cache(maxsize=64)(self._make_desc)
+            self._loaded = (kh, kw, cin, K, w.device)
+        if bias is None:
+            self.bias = None
+        elif self.bias is None:
+            self.bias = bias.detach().clone().contiguous()
+        else:
+            self.bias.copy_(bias.detach())
         _lib.check(lib.tde_q8_weights(kh * kw, cin, K, 1 if self.deconv else 0, w.data_ptr(), self.codes.data_ptr(),
                                       self.scales.data_ptr(), _lib.raw_stream(w.get_device())), "Conv8 weights")
         return self
