@@ -97,3 +97,13 @@ def test_the_c_entries_refuse_what_wraps(p):  # noqa: F811
         assert lib.tde_q8_conv2d_bias_act(d, p, p, p, p, None, 1, p, None) == -1, big
         assert lib.tde_q8_deconv2d_bias_act(d, p, p, p, p, None, 1, p, None) == -1, big
         assert lib.tde_q8_one_launch(d, 0) == 0 and lib.tde_q8_one_launch(d, 1) == 0, big
+
+
+def test_weights_on_another_device(monkeypatch):
+    """Conv8 made on one device and called with a tensor of another, current one."""
+    monkeypatch.setattr(int8, "_check", lambda *a, **k: None)
+    monkeypatch.setattr(int8._lib, "current_device", lambda: 0)
+    c = conv(1, 1, 4, 4, 1)
+    c.codes = types.SimpleNamespace(get_device=lambda: 1, device="cuda:1")
+    with pytest.raises(ValueError, match="weights are on cuda:1"):
+        c(meta((5, 4)))

@@ -234,6 +234,9 @@ class Conv8:
         [N, OH, OW, Cout] ([M, Cout]), written into the channel view `out` if given (which may lie on x)."""
         rows8 = isinstance(x, Rows8)
         _check(x.buffer if rows8 else x, "x", torch.int8 if rows8 else torch.float32)
+        if self.codes.get_device() != _lib.current_device():
+            raise ValueError(f"the weights are on {self.codes.device}, not on the current device "
+                             f"(cuda:{_lib.current_device()})")
         ics = self.cin if rows8 else _rows(x, "x")[2]
         N, H, W, oshape = self._geometry(x.shape)
         y = _out(out, oshape, x.buffer.device if rows8 else x.device)
