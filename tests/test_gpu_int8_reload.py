@@ -1,4 +1,7 @@
-"""Conv8.load under a captured graph."""
+"""Conv8's weights: loaded under a captured graph, and given back."""
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -44,3 +47,17 @@ def test_load_reaches_a_captured_graph(shape, deconv, stride, x):
     w2 = torch.cat([w, w], dim=2 if deconv else 3)
     conv.load(w2, torch.cat([b, b]))
     assert torch.equal(conv(xb), torch.cat([want, want], dim=-1))
+
+
+def test_weights_are_given_back_with_the_layer():
+    """Without a garbage collection."""
+    gc.collect()
+    gc.disable()
+    try:
+        conv = int8.Conv8(torch.ones(1, 1, 8, 4, device="cuda"))
+        conv(torch.ones(5, 8, device="cuda"))
+        codes = weakref.ref(conv.codes)
+        del conv
+        assert codes() is None
+    finally:
+        gc.enable()

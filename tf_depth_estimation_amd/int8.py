@@ -20,6 +20,7 @@ import contextlib
 import contextvars
 import ctypes
 import functools
+import weakref
 
 import torch
 from torch.autograd import forward_ad
@@ -179,8 +180,9 @@ class Conv8:
             self.codes = torch.empty(lib.tde_q8_weights_size(kh * kw, cin, K), dtype=torch.int8, device=w.device)
             self.scales = torch.empty((K + 15) // 16 * 16, dtype=torch.float32, device=w.device)
             self.bias = None
-            self._geometry = functools.lru_cache(maxsize=64)(self._make_geometry)
-            self._desc = functools.lru_cache(maxsize=64)(self._make_desc)
+            me = weakref.ref(self)      # (a cache that held the layer would keep its weights until a garbage collection)
+            self._geometry = functools.lru_cache(maxsize=64)(lambda *a: me()._make_geometry(*a))
+            self._desc = functools.lru_cache(maxsize=64)(lambda *a: me()._make_desc(*a))
             self._loaded = (kh, kw, cin, K, w.device)
         if bias is None:
             self.bias = None
