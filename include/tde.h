@@ -330,7 +330,8 @@ int tde_q8_deconv2d_f32_bias_act(const tde_conv_desc_t* d, const float* x_small,
  * A block that holds a NaN or an infinity has scale NaN (its restored values are NaN).
  *   codes [M][C] int8, scales [M][ceil(C / TDE_TAPE8_BLOCK)] float; both 16-byte aligned.
  * M rows are `groups` equal row groups, each its own BatchNorm batch (tde_bn_fwd_train).  C % 4 == 0, C <= 1024.
- * Sums are fp64 in a fixed order: results do not change from run to run. */
+ * Sums are fp64 in a fixed order: results do not change from run to run.
+ * y may be z itself, and dz dy itself (dense, the same pointer); else they must lie apart. */
 #define TDE_TAPE8_BLOCK 64
 size_t tde_tape8_workspace_size(int M, int C);
 /* 1: tde_tape8_bn_fwd / tde_tape8_bn_bwd on this shape are one launch that needs no workspace (ws may be NULL). */

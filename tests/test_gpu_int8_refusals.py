@@ -32,3 +32,29 @@ def test_forward_mode_tangents():
             f(x.clone().requires_grad_())
     with pytest.raises((ValueError, RuntimeError)):
         torch.func.jvp(calls()["conv"], (x,), (torch.ones_like(x),))
+
+
+@pytest.mark.parametrize("M,C,groups", [(16, 8, 1), (96, 512, 2), (6000, 64, 2), (20000, 36, 1)])
+def test_outputs_in_place_or_apart(M, C, groups):
+    """y on z and dz on dy give what separate tensors do; anything in between is refused."""
+    z, beta = torch.randn(M, C, device="cuda"), torch.randn(C, device="cuda") * 0.3
+    y, tape = int8.bn_relu_forward(z, beta, groups=groups)
+    zz = z.clone()
+    y2, tape2 = int8.bn_relu_forward(zz, beta, groups=groups, out=zz)
+    assert y2 is zz and torch.equal(y2, y) and torch.equal(tape2.codes, tape.codes) and torch.equal(tape2.scales, tape.scales)
+    dy = torch.randn(M, C, device="cuda")
+    dz, db = int8.bn_relu_backward(tape, beta, dy)
+    dd = dy.clone()
+    dz2, db2 = int8.bn_relu_backward(tape, beta, dd, dz=dd)
+    assert dz2 is dd and torch.equal(dz2, dz) and torch.equal(db2, db)
+    buf = torch.zeros(2 * M * C + 8, device="cuda")
+    dense, wide = buf[:M * C].view(M, C), buf[:2 * M * C].view(M, 2 * C)[:, :C]
+    shifted, behind = buf[4:4 + M * C].view(M, C), buf[M * C:2 * M * C].view(M, C)
+    for out in (wide, shifted):
+        with pytest.raises(ValueError, match="overlap"):
+            int8.bn_relu_forward(dense, beta, groups=groups, out=out)
+        with pytest.raises(ValueError, match="overlap"):
+            int8.bn_relu_backward(tape, beta, out, dz=dense)
+    dense.copy_(z)
+    y3, _ = int8.bn_relu_forward(dense, beta, groups=groups, out=behind)
+    assert torch.equal(y3, y) and torch.equal(dense, z)

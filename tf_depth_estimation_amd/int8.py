@@ -353,6 +353,16 @@ def _check_view(t, cs, name):
         raise ValueError(f"{name}: the channel view must start on 16 bytes with a pixel stride of a multiple of 4")
 
 
+def _check_apart(a, acs, b, bcs, rows, C, what):
+    """Two [rows, C] fp32 views with pixel strides acs and bcs are one and the same, or lie apart: a kernel that writes one
+    while its other blocks read the other gives no defined result in between."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa == pb and acs == bcs:
+        return
+    if pa < pb + 4 * ((rows - 1) * bcs + C) and pb < pa + 4 * ((rows - 1) * acs + C):
+        raise ValueError(f"{what} overlap: they must lie apart, or be the same view")
+
+
 def _check_beta(C, beta):
     if C == 0 or C % 4 or C > 1024:
         raise ValueError(f"{C} channels: a multiple of 4 up to 1024 is expected")
@@ -380,7 +390,8 @@ def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel
     """Training BatchNorm (scale=False) + ReLU of z [..., C] (contiguous) that keeps an 8-bit tape: returns (y, Tape8).
 
     The rows are `groups` equal consecutive groups, each normalised over its own rows.  moving: (moving_mean,
-    moving_variance), updated in place in group order.  out: a channel view for y (16-byte aligned)."""
+    moving_variance), updated in place in group order.  out: a channel view for y (16-byte aligned), z itself or apart from
+    it."""
     _check(z, "z")
     shape, dev = z.shape, z.device
     C = shape[-1] if len(shape) >= 2 else 0
@@ -401,6 +412,8 @@ def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel
     y = _out(out, shape, dev)
     _, _, cs = _rows(y, "out")
     _check_view(y, cs, "out")
+    if out is not None:
+        _check_apart(z, C, y, cs, rows, C, "z and out")
     tape = Tape8._empty(shape, C, rows, groups, dev)
     codes, scales, invstd = tape._ptrs
     keep, ws, nb = _workspace(rows, C, groups, dev)
@@ -412,7 +425,8 @@ def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel
 
 def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
     """(dz, dbeta) of the layer whose forward made `tape`, from the gradient dy [..., C] (channel view) of its output;
-    beta as in that forward.  dz: a contiguous tensor to write; dbeta: a tensor to ADD to (a fresh one is written)."""
+    beta as in that forward.  dz: a contiguous tensor to write, dy itself or apart from it; dbeta: a tensor to ADD to (a
+    fresh one is written)."""
     if not isinstance(tape, Tape8):
         raise ValueError("tape must be a Tape8")
     _check(dy, "dy")
@@ -425,9 +439,12 @@ def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
     if rows == 0:
         raise ValueError("BatchNorm over no rows has no gradient")
     _check_view(dy, cs, "dy")
+    given = dz is not None
     dz = _out(dz, shape, dev, "dz")
     if not dz.is_contiguous() or dz.data_ptr() % 16:
         raise ValueError("dz must be contiguous and start on 16 bytes")
+    if given:
+        _check_apart(dy, cs, dz, C, rows, C, "dy and dz")
     acc = dbeta is not None
     dbeta = _out(dbeta, (C,), dev, "dbeta")
     if not dbeta.is_contiguous():
