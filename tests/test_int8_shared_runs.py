@@ -83,3 +83,40 @@ def test_input_gradients_through_autograd(cin, fresh_store):
     kept = xs[0].grad
     loss(image(3).requires_grad_()).backward()
     assert torch.equal(kept, alone[0])
+
+
+@pytest.mark.gpu
+def test_the_first_run_is_made_before_a_capture(fresh_store):
+    """The shared buffers are refused under capture; with them there, a run made, stepped forward and back inside a capture
+    replays as the eager run between whose steps it is replayed."""
+    N, H, W = 2, 64, 96
+    with variables.variable_scope("model"):
+        prog = _api.get_program("depth_net", _netlib.disp_net_spec, H, W, 3)
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(N, H, W, 3, generator=g).mul_(0.3).cuda()
+    gs = [torch.randn(N, v.H, v.W, v.C, generator=g).cuda() for v in prog.spec.outputs]
+    torch.cuda.synchronize()
+    with pytest.raises(ValueError, match="before the capture"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            NetRun(prog, N, tape8=True)
+    eager = NetRun(prog, N, tape8=True)
+
+    def step(run):
+        outs = prog.forward(run, x)
+        return outs + [prog.backward(run, gs, need_input_grad=True, grad_accumulate=False)]
+
+    step(eager)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(NetRun(prog, N, tape8=True))
+    for i in range(3):
+        x.copy_(torch.randn(x.shape, generator=g).mul_(0.3))
+        outs = prog.forward(eager, x)
+        graph.replay()                                   # the shared buffers are another run's now
+        torch.cuda.synchronize()
+        replayed, pgrad = [t.clone() for t in captured], prog.chunk.grad.clone()
+        dx = prog.backward(eager, gs, need_input_grad=True, grad_accumulate=False)
+        for a, b in zip(replayed, outs + [dx]):
+            assert torch.equal(a, b), i
+        assert torch.equal(pgrad, prog.chunk.grad), i

@@ -433,9 +433,12 @@ class NetProgram:
 
     def shared_tape8(self, N, device="cuda"):
         """The buffers all 8-bit-tape runs of this program at batch N work in: activations and gradients by buffer name,
-        and one pre-BN output of the largest layer."""
+        and one pre-BN output of the largest layer.  Made outside any capture: the zero channels that pad a buffer would be
+        written by a replay only, and a run in between would read what was there."""
         sh = self._tape8.get(N)
         if sh is None:
+            if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise ValueError(f"8-bit tape: the first run at batch {N} must be made before the capture (warm up once)")
             own, out = self.own_buffers(), {v.buf.name for v in self.spec.outputs}
 
             def new(b, zero=False):
