@@ -120,7 +120,7 @@ class Predictor:
         fp32 network's by the 8-bit rounding of weights and activations."""
         if int8 and not fold_bn:
             raise ValueError("int8 prediction runs on the folded weights: fold_bn=True")
-        self.int8, self.conv8 = bool(int8), None
+        self.int8, self.conv8, self.folded = bool(int8), None, None
         if net not in NETS:
             raise ValueError(f"unknown net {net!r}: one of {sorted(NETS)}")
         net_scope, builder, cin0, kw, _ = NETS[net]
@@ -145,7 +145,9 @@ class Predictor:
         """Re-fold the BN statistics and re-capture after the variables changed."""
         self.graph = None
         if self.fold:
-            self.prog.fold_bn()
+            # kept: the captured graph reads these weights, and another Predictor of this network (fp32 beside int8, another
+            # batch) puts its own in the program's place
+            self.folded = self.prog.fold_bn()
         if self.int8:
             self.conv8 = self._quantize_layers()
         s = _lib.owned_stream(self, "warmup")
