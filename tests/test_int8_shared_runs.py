@@ -120,3 +120,20 @@ def test_the_first_run_is_made_before_a_capture(fresh_store):
         for a, b in zip(replayed, outs + [dx]):
             assert torch.equal(a, b), i
         assert torch.equal(pgrad, prog.chunk.grad), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cin", [3, 4])
+@pytest.mark.parametrize("tape", [False, True])
+def test_two_backwards_of_one_call(cin, tape, fresh_store):
+    """retain_graph: the second backward adds to the gradient autograd took over from the first."""
+    from tf_depth_estimation_amd import nets_optflow_depth as nd
+    x = torch.randn(2, 64, 96, cin, generator=torch.Generator().manual_seed(1)).mul_(0.3).cuda().requires_grad_()
+    with variables.variable_scope("model"), int8.tape8(tape):
+        outs = nd.disp_net(x, True)[0]
+    losses = [(outs[0] * outs[0]).mean(), 5 * outs[0].mean()]
+    apart = [torch.autograd.grad(v, x, retain_graph=True)[0].clone() for v in losses]
+    assert not torch.equal(*apart)
+    for v in losses:
+        v.backward(retain_graph=True)
+    assert torch.equal(x.grad, apart[0] + apart[1])

@@ -44,7 +44,10 @@ class _NetFunction(torch.autograd.Function):
     def backward(ctx, *grads):
         need_x = ctx.needs_input_grad[1]
         dx = ctx.prog.backward(ctx.run, list(grads), need_input_grad=need_x)
-        return None, (dx.contiguous() if dx is not None else None), None, None, None
+        # autograd may keep the tensor itself as x.grad: never the run's buffer, which a second backward rewrites
+        if dx is not None and not ctx.run.tape8:
+            dx = dx.clone(memory_format=torch.contiguous_format)
+        return None, dx, None, None, None
 
 
 def run_net(net_scope, builder, x, is_training=True, **kw):
