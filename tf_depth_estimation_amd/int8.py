@@ -44,7 +44,7 @@ def _check(t, name, dtype=torch.float32):
         raise ValueError(f"{name} is on {t.device}, not on the current device (cuda:{_lib.current_device()})")
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires a gradient: 8-bit operators record none (detach it, or use torch.no_grad())")
-    if getattr(forward_ad, "_current_level", 0) >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:      # (-1: outside any level)
         raise ValueError(f"{name} has a forward-mode tangent: 8-bit operators carry none")
 
 
@@ -236,7 +236,7 @@ class Conv8:
         [N, OH, OW, Cout] ([M, Cout]), written into the channel view `out` if given (which may lie on x)."""
         rows8 = isinstance(x, Rows8)
         _check(x.buffer if rows8 else x, "x", torch.int8 if rows8 else torch.float32)
-        if self.codes.get_device() != _lib.current_device():
+        if self.codes.get_device() != (x.buffer if rows8 else x).get_device():
             raise ValueError(f"the weights are on {self.codes.device}, not on the current device "
                              f"(cuda:{_lib.current_device()})")
         ics = self.cin if rows8 else _rows(x, "x")[2]
@@ -335,10 +335,10 @@ class Tape8:
         dev = self._buffer.device
         y = _out(out, self.shape, dev)
         rows, _, cs = _rows(y, "out")
-        _check_view(y, cs, "out")
+        py = _check_view(y, cs, "out")
         if rows:
             codes, scales, _ = self._ptrs
-            _lib.check(_lib.load().tde_tape8_restore(rows, self.C, codes, scales, bool(relu), y.data_ptr(), cs, 0,
+            _lib.check(_lib.load().tde_tape8_restore(rows, self.C, codes, scales, bool(relu), py, cs, 0,
                                                      _lib.raw_stream(dev.index)), "Tape8.restore")
         return y
 
@@ -349,14 +349,16 @@ def _check_groups(rows, groups):
 
 
 def _check_view(t, cs, name):
-    if t.data_ptr() % 16 or cs % 4:
+    """The view's pointer."""
+    p = t.data_ptr()
+    if p % 16 or cs % 4:
         raise ValueError(f"{name}: the channel view must start on 16 bytes with a pixel stride of a multiple of 4")
+    return p
 
 
-def _check_apart(a, acs, b, bcs, rows, C, what):
-    """Two [rows, C] fp32 views with pixel strides acs and bcs are one and the same, or lie apart: a kernel that writes one
-    while its other blocks read the other gives no defined result in between."""
-    pa, pb = a.data_ptr(), b.data_ptr()
+def _check_apart(pa, acs, pb, bcs, rows, C, what):
+    """Two [rows, C] fp32 views at pa and pb with pixel strides acs and bcs are one and the same, or lie apart: a kernel that
+    writes one while its other blocks read the other gives no defined result in between."""
     if pa == pb and acs == bcs:
         return
     if pa < pb + 4 * ((rows - 1) * bcs + C) and pb < pa + 4 * ((rows - 1) * acs + C):
@@ -396,11 +398,12 @@ def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel
     shape, dev = z.shape, z.device
     C = shape[-1] if len(shape) >= 2 else 0
     _check_beta(C, beta)
-    if not z.is_contiguous() or z.data_ptr() % 16:
+    pz = z.data_ptr()
+    if not z.is_contiguous() or pz % 16:
         raise ValueError("z must be a contiguous [..., C] tensor that starts on 16 bytes")
-    rows = _rows(z, "z")[0]
-    if rows == 0:
-        raise ValueError("BatchNorm over no rows has no statistics")
+    rows = z.numel() // C
+    if not 0 < rows <= MAX_ROWS:
+        raise ValueError(f"z: {rows} rows: at most 2^30" if rows else "BatchNorm over no rows has no statistics")
     _check_groups(rows, groups)
     mm = mv = None
     if moving is not None:
@@ -411,14 +414,14 @@ def bn_relu_forward(z, beta, groups=1, eps=1e-3, decay=0.99, moving=None, bessel
         mm, mv = (t.data_ptr() for t in moving)
     y = _out(out, shape, dev)
     _, _, cs = _rows(y, "out")
-    _check_view(y, cs, "out")
+    py = _check_view(y, cs, "out")
     if out is not None:
-        _check_apart(z, C, y, cs, rows, C, "z and out")
+        _check_apart(pz, C, py, cs, rows, C, "z and out")
     tape = Tape8._empty(shape, C, rows, groups, dev)
     codes, scales, invstd = tape._ptrs
     keep, ws, nb = _workspace(rows, C, groups, dev)
-    _lib.check(_lib.load().tde_tape8_bn_fwd(rows, C, groups, z.data_ptr(), beta.data_ptr(), eps, decay, bool(bessel), mm,
-                                            mv, tape._mean_ptr, invstd, y.data_ptr(), cs, 0, codes, scales, ws, nb,
+    _lib.check(_lib.load().tde_tape8_bn_fwd(rows, C, groups, pz, beta.data_ptr(), eps, decay, bool(bessel), mm,
+                                            mv, tape._mean_ptr, invstd, py, cs, 0, codes, scales, ws, nb,
                                             _lib.raw_stream(dev.index)), "bn_relu_forward")
     return y, tape
 
@@ -438,21 +441,22 @@ def bn_relu_backward(tape, beta, dy, dz=None, dbeta=None):
     rows, _, cs = _rows(dy, "dy")
     if rows == 0:
         raise ValueError("BatchNorm over no rows has no gradient")
-    _check_view(dy, cs, "dy")
+    pdy = _check_view(dy, cs, "dy")
     given = dz is not None
     dz = _out(dz, shape, dev, "dz")
-    if not dz.is_contiguous() or dz.data_ptr() % 16:
+    pdz = dz.data_ptr()
+    if not dz.is_contiguous() or pdz % 16:
         raise ValueError("dz must be contiguous and start on 16 bytes")
     if given:
-        _check_apart(dy, cs, dz, C, rows, C, "dy and dz")
+        _check_apart(pdy, cs, pdz, C, rows, C, "dy and dz")
     acc = dbeta is not None
     dbeta = _out(dbeta, (C,), dev, "dbeta")
     if not dbeta.is_contiguous():
         raise ValueError("dbeta must be contiguous")
     keep, ws, nb = _workspace(rows, C, tape.groups, dev)
     codes, scales, invstd = tape._ptrs
-    _lib.check(_lib.load().tde_tape8_bn_bwd(rows, C, tape.groups, codes, scales, invstd, beta.data_ptr(), dy.data_ptr(),
-                                            cs, 0, dz.data_ptr(), dbeta.data_ptr(), acc, None, ws, nb,
+    _lib.check(_lib.load().tde_tape8_bn_bwd(rows, C, tape.groups, codes, scales, invstd, beta.data_ptr(), pdy, cs,
+                                            0, pdz, dbeta.data_ptr(), acc, None, ws, nb,
                                             _lib.raw_stream(dev.index)), "bn_relu_backward")
     return dz, dbeta
 
