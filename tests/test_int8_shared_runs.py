@@ -137,3 +137,22 @@ def test_two_backwards_of_one_call(cin, tape, fresh_store):
     for v in losses:
         v.backward(retain_graph=True)
     assert torch.equal(x.grad, apart[0] + apart[1])
+
+
+def test_a_refused_switch_leaves_the_run_whole(monkeypatch):
+    """enable_tape8 inside a capture, or of a network without BatchNorm: the fp32 run keeps every buffer."""
+    prog = NetProgram(_netlib.disp_net_spec(64, 96, 3), types.SimpleNamespace(prefix="m"))
+    run = NetRun(prog, 2, device="cpu")
+    run.ensure_grad()
+    before = [dict(d) for d in (run.act, run.z, run.grad)]
+
+    def capturing(self, N, device):
+        raise ValueError("before the capture")
+
+    monkeypatch.setattr(NetProgram, "check_tape8_capture", capturing, raising=False)
+    monkeypatch.setattr(NetProgram, "shared_tape8", capturing)
+    with pytest.raises(ValueError, match="before the capture"):
+        run.enable_tape8()
+    assert not run.tape8
+    for was, now in zip(before, (run.act, run.z, run.grad)):
+        assert now is not None and all(now[k] is t for k, t in was.items())

@@ -284,6 +284,7 @@ class NetRun:
             if isinstance(op, ConvBN) and (not op.bn or op.K % 4 or op.K > 1024):
                 raise ValueError(f"8-bit tape: layer {op.layer} needs BatchNorm over a multiple of 4 channels, at most "
                                  "1024 (BN-free networks keep the fp32 tape)")
+        self.prog.check_tape8_capture(N, self.device)
         own, out = self.prog.own_buffers(), {v.buf.name for v in spec.outputs}
         # of an fp32 run's buffers only those that stay are held while the new ones are made
         kept = {n: t for n, t in (getattr(self, "act", None) or {}).items() if n in own}
@@ -431,14 +432,18 @@ class NetProgram:
         return ({self.spec.input.name} | {v.buf.name for v in self.spec.outputs} |
                 {op.dst.buf.name for op in self.spec.ops if isinstance(op, Head)})
 
+    def check_tape8_capture(self, N, device):
+        """The shared buffers are made outside any capture: the zero channels that pad a buffer would be written by a replay
+        only, and a run in between would read what was there."""
+        if N not in self._tape8 and torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise ValueError(f"8-bit tape: the first run at batch {N} must be made before the capture (warm up once)")
+
     def shared_tape8(self, N, device="cuda"):
         """The buffers all 8-bit-tape runs of this program at batch N work in: activations and gradients by buffer name,
-        and one pre-BN output of the largest layer.  Made outside any capture: the zero channels that pad a buffer would be
-        written by a replay only, and a run in between would read what was there."""
+        and one pre-BN output of the largest layer."""
         sh = self._tape8.get(N)
         if sh is None:
-            if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
-                raise ValueError(f"8-bit tape: the first run at batch {N} must be made before the capture (warm up once)")
+            self.check_tape8_capture(N, device)
             own, out = self.own_buffers(), {v.buf.name for v in self.spec.outputs}
 
             def new(b, zero=False):
