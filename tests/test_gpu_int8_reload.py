@@ -61,3 +61,19 @@ def test_weights_are_given_back_with_the_layer():
         assert codes() is None
     finally:
         gc.enable()
+
+
+def test_load_in_and_out_of_inference_mode():
+    w, x = torch.randn(1, 1, 8, 4, device="cuda"), torch.randn(5, 8, device="cuda")
+    with torch.inference_mode():
+        conv = int8.Conv8(w, torch.zeros(4, device="cuda"), relu=False)
+        y = conv(x)
+    conv.load(w, torch.ones(4, device="cuda"))
+    assert torch.equal(conv(x), int8.Conv8(w, torch.ones(4, device="cuda"), relu=False)(x))
+    with torch.inference_mode():
+        conv.load(w, torch.zeros(4, device="cuda"))
+        assert torch.equal(conv(x), y)
+    other = int8.Conv8(w, torch.ones(4, device="cuda"), relu=False)
+    with torch.inference_mode():
+        other.load(w, torch.zeros(4, device="cuda"))
+    assert torch.equal(other(x), y)

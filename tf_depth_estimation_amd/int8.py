@@ -176,20 +176,21 @@ class Conv8:
         lib = _lib.load()
         w = weights.contiguous()
         if (kh, kw, cin, K, w.device) != getattr(self, "_loaded", None):
-            self.kh, self.kw, self.cin, self.K = kh, kw, cin, K
-            self.codes = torch.empty(lib.tde_q8_weights_size(kh * kw, cin, K), dtype=torch.int8, device=w.device)
-            self.scales = torch.empty((K + 15) // 16 * 16, dtype=torch.float32, device=w.device)
-            self.bias = None
+            codes = torch.empty(lib.tde_q8_weights_size(kh * kw, cin, K), dtype=torch.int8, device=w.device)
+            scales = torch.empty((K + 15) // 16 * 16, dtype=torch.float32, device=w.device)
             me = weakref.ref(self)      # (a cache that held the layer would keep its weights until a garbage collection)
             self._geometry = functools.lru_cache(maxsize=64)(lambda *a: me()._make_geometry(*a))
             self._desc = functools.lru_cache(maxsize=64)(lambda *a: me()._make_desc(*a))
+            self.codes, self.scales, self.bias = codes, scales, None
+            self.kh, self.kw, self.cin, self.K = kh, kw, cin, K
             self._loaded = (kh, kw, cin, K, w.device)
         if bias is None:
             self.bias = None
         elif self.bias is None:
             self.bias = bias.detach().clone().contiguous()
         else:
-            self.bias.copy_(bias.detach())
+            with torch.inference_mode():      # (a bias cloned in that mode takes no other writes)
+                self.bias.copy_(bias)
         _lib.check(lib.tde_q8_weights(kh * kw, cin, K, 1 if self.deconv else 0, w.data_ptr(), self.codes.data_ptr(),
                                       self.scales.data_ptr(), _lib.raw_stream(w.get_device())), "Conv8 weights")
         return self
